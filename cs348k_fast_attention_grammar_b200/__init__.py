@@ -10,6 +10,9 @@ through its C ABI, ``include/fa_b200.h``; there is no fallback path):
     mlp(x, w1, w2, act="gelu_tanh")                          # act(x@w1)@w2, bf16/fp16
     mlp_ln(x, w1, w2)                                        # LN(relu(x@w1)@w2 + x)
     gemm_act(a, b, act="none")                               # act(a@b)
+    rotary(x, positions, inv_freq)                           # rotary positions, 1..4 axes
+    paged_kv_append(k, v, k_cache, v_cache, ...)             # rotate and store new tokens
+    paged_attention(q, k_cache, v_cache, ...)                # new tokens over a paged cache
 
 ``kernel_module`` exposes the reference's ``fn(KT, Q, V)`` + ``KERNEL_META``
 protocol; ``parallel`` holds the batch x head sharding used by ``bench.py``.
@@ -28,7 +31,8 @@ from .operators import (  # noqa: F401
     mlp_from_host,
     mlp_ln,
 )
+from .paged import paged_attention, paged_kv_append, rotary  # noqa: F401
 
 __all__ = ["attention", "attention_bshd", "attention_f32", "attention_from_host", "mlp", "mlp_from_host", "mlp_ln",
-           "layer_norm_rows", "gemm_act",
+           "layer_norm_rows", "gemm_act", "rotary", "paged_kv_append", "paged_attention",
            "device_status", "FaError", "load", "lib_path"]

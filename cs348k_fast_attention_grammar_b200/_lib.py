@@ -16,6 +16,9 @@ from . import build as _build
 FA_OK = 0
 FA_F32_BF16 = 0
 FA_F32_SPLIT = 1
+FA_BF16 = 0
+FA_F16 = 1
+FA_F32 = 2
 FA_ACT_NONE = 0
 FA_ACT_RELU = 1
 FA_ACT_GELU_TANH = 2
@@ -44,6 +47,11 @@ SIGNATURES = {
                                _c_float, _vp]),
     "fa_layernorm_rows": (_c_int, [_vp, _vp, _c_int, _c_int, _i64, _i64, _c_float, _vp]),
     "fa_mlp_fwd_noalloc": (_c_int, [_vp, _vp, _vp, _vp, _c_int, _c_int, _c_int, _c_int, _vp]),
+    # Argument structs are packed by the caller and passed as bytes.
+    "fa_rotary": (_c_int, [ctypes.c_char_p, _vp]),
+    "fa_paged_append": (_c_int, [ctypes.c_char_p, _vp]),
+    "fa_paged_attn_workspace": (_i64, [ctypes.c_char_p]),
+    "fa_paged_attn": (_c_int, [ctypes.c_char_p, _vp, _i64, _vp]),
     "fa_device_status": (_c_int, []),
     "fa_selftest_wait_timeout": (_c_int, [_c_int, _vp]),
     "fa_selftest_exp2": (_c_int, [_vp, _vp, _c_int, _vp]),

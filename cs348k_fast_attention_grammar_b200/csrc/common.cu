@@ -184,6 +184,9 @@ extern "C" const char* fa_strerror(int status) {
     case FA_ERR_CUDA: return "a CUDA runtime call failed";
     case FA_ERR_SCRATCH:
       return "M * N exceeds the fixed hidden buffer of fa_mlp_fwd_noalloc (8,388,608 elements)";
+    case FA_ERR_PAGE:
+      return "a block table entry or sequence length points outside the cache (device status)";
+    case FA_ERR_WORKSPACE: return "the workspace is missing or too small";
     default: return "unknown fa_status";
   }
 }
@@ -199,5 +202,6 @@ extern "C" int fa_device_status(void) {
   const int zero = 0;
   if (cudaMemcpy(p, &zero, sizeof(int), cudaMemcpyHostToDevice) != cudaSuccess)
     return FA_ERR_CUDA;
+  if (v == fa::kDevBadPage) return FA_ERR_PAGE;
   return v == fa::kDevTimeout ? FA_ERR_TIMEOUT : FA_OK;
 }

@@ -1,0 +1,701 @@
+// Attention of new tokens over a paged key/value cache (fa_paged_attn):
+//     o = softmax(q K^T * scale) V      per token and head
+//
+// Query heads that share a key/value head are rows of one tile together with
+// the sequence's new tokens: row r of a sequence is token r / g, head r % g of
+// the group (g = Hq / Hkv), so each key is read once for all of them.
+//
+// paged_rows_kernel takes sequences of few rows (a generation step).  It is
+// bound by HBM: two passes' worth of arithmetic per key and row is far below
+// what even warp-level matrix instructions deliver, so the kernel is built
+// around its loads.  A CTA has four warps; per 64-key block each warp owns 16
+// keys, loads their K and V rows with 16-byte asynchronous copies into a ring
+// of its own (no barrier between warps), and keeps its own running maximum, sum
+// and output, joined over the warps when the CTA leaves a tile.
+//
+// The key blocks of all (sequence, key head, row tile) units, one after the
+// other, are cut into equal ranges, one per CTA, whatever the lengths: a unit
+// that crosses a range's border leaves (m, l, O) of its parts in the workspace
+// and paged_rows_join adds them up in the order of the keys, so results do not
+// depend on timing.
+#include <cuda_bf16.h>
+
+#include "fa_internal.h"
+#include "paged.cuh"
+#include "sm100_ptx.cuh"
+
+namespace fa {
+namespace {
+
+struct PagedParams {
+  const void* q;
+  void* o;
+  const void* kc;
+  const void* vc;
+  const int32_t* table;
+  const int32_t* lens;
+  const int32_t* cu;
+  int64_t q_st, q_sh, o_st, o_sh;       // elements: token, head
+  int64_t kc_p, kc_r, kc_h;             // page, row, head
+  int64_t vc_p, vc_r, vc_h;
+  int64_t table_stride;
+  int T, B, Hkv, g, D;
+  int pages, page_shift, max_pages;
+  int causal;
+  float scale_log2;
+  int* status;
+  float* part;                          // partial results of split units
+  int ctas;                             // ranges the key blocks are cut into
+  int min_blocks;                       // least key blocks of a range
+};
+
+// ---------------------------------------------------------------------------
+// Schedule of the row kernel
+// ---------------------------------------------------------------------------
+constexpr int kRowThreads = 128;
+constexpr int kRowWarps = 4;
+constexpr int kRowKeys = 64;            // keys of a block: 16 per warp
+
+// A sequence's rows and key blocks.
+struct SeqWork {
+  int begin, q_len, kv_len, tiles, blocks;
+};
+
+__device__ __forceinline__ SeqWork seq_work(const PagedParams& p, int b, int tile_rows) {
+  SeqWork w;
+  const SeqRows r = seq_rows(p.cu, b, p.T);
+  w.begin = r.begin;
+  w.q_len = r.end - r.begin;
+  const int len = p.lens[b];
+  w.kv_len = held_len(len, p.page_shift, p.max_pages);
+  if (len > w.kv_len && len > 0) atomicExch(p.status, kDevBadPage);
+  const int64_t rows = static_cast<int64_t>(w.q_len) * p.g;
+  w.tiles = static_cast<int>((rows + tile_rows - 1) / tile_rows);
+  w.blocks = max(1, (w.kv_len + kRowKeys - 1) / kRowKeys);
+  return w;
+}
+__device__ __forceinline__ int64_t weight(const PagedParams& p, const SeqWork& w) {
+  return static_cast<int64_t>(w.tiles) * p.Hkv * w.blocks;
+}
+
+// The sum of v over the CTA's threads below this one, and over all of them.
+__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* red, int64_t* total) {
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  int64_t x = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  __syncthreads();
+  if (lane == 31) red[w] = x;
+  __syncthreads();
+  int64_t before = 0, sum = 0;
+#pragma unroll
+  for (int i = 0; i < kRowWarps; ++i) {
+    if (i < w) before += red[i];
+    sum += red[i];
+  }
+  *total = sum;
+  return before + x - v;
+}
+
+// A CTA's range [start, end) of the key blocks and the sequence that `at`
+// (start, or the range's last block) falls into.
+struct Range {
+  int64_t start, end, per;
+  int64_t base;          // first key block of sequence b
+  int b;
+};
+
+template <bool LAST>
+__device__ __forceinline__ Range find_range(const PagedParams& p, int cta, int tile_rows) {
+  __shared__ int64_t red[kRowWarps];
+  __shared__ int64_t s_base;
+  __shared__ int s_b;
+  Range r;
+  int64_t total = 0;
+  int64_t first_w = 0, first_before = 0;      // the scan of the first kRowThreads sequences
+  for (int b0 = 0; b0 < p.B; b0 += kRowThreads) {
+    const int b = b0 + threadIdx.x;
+    const int64_t w = b < p.B ? weight(p, seq_work(p, b, tile_rows)) : 0;
+    int64_t sum;
+    const int64_t before = block_scan(w, red, &sum);
+    if (b0 == 0) {
+      first_w = w;
+      first_before = before;
+    }
+    total += sum;
+  }
+  r.per = max(static_cast<int64_t>(p.min_blocks), (total + p.ctas - 1) / p.ctas);
+  r.start = min(total, r.per * cta);
+  r.end = min(total, r.start + r.per);
+  if (threadIdx.x == 0) s_b = p.B;
+  __syncthreads();
+  const int64_t at = LAST ? r.end - 1 : r.start;
+  if (r.start < r.end) {
+    int64_t base = 0;
+    for (int b0 = 0; b0 < p.B; b0 += kRowThreads) {
+      const int b = b0 + threadIdx.x;
+      int64_t w = first_w, before = first_before, sum = 0;
+      if (p.B > kRowThreads) {
+        w = b < p.B ? weight(p, seq_work(p, b, tile_rows)) : 0;
+        before = block_scan(w, red, &sum);
+      }
+      if (w > 0 && base + before <= at && at < base + before + w) {
+        s_b = b;
+        s_base = base + before;
+      }
+      base += sum;
+    }
+  }
+  __syncthreads();
+  r.b = s_b;
+  r.base = r.b < p.B ? s_base : 0;
+  return r;
+}
+
+// ---------------------------------------------------------------------------
+// Warp-level pieces
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
+               "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+template <bool F16>
+__device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
+                                          uint32_t b1) {
+  if (F16)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Keys [0, limit) that token i of the sequence sees.
+__device__ __forceinline__ int seen_keys(const PagedParams& p, const SeqWork& w, int i) {
+  return p.causal ? max(0, w.kv_len - w.q_len + i + 1) : w.kv_len;
+}
+
+template <int DT, int MT>
+struct RowCfg {
+  static constexpr int kRows = 16 * MT;
+  static constexpr int kStages = 3;
+  static constexpr int kTile = 16 * DT * 2;              // 16 keys of K or of V
+  static constexpr int kStage = 2 * kTile;
+  static constexpr int kWarp = kStages * kStage;
+  static constexpr int kRing = kRowWarps * kWarp;
+  static constexpr int kSmem = kRing + 2 * kRowWarps * kRows * 4;   // + m, l of each warp
+  static constexpr int kSlot = kRows * (DT + 2);         // floats of a partial result
+  static_assert(kRowWarps * kRows * DT * 4 <= kRing, "the joined output reuses the ring");
+};
+
+template <int DT, int MT, bool F16>
+__global__ void __launch_bounds__(kRowThreads)
+    paged_rows_kernel(const PagedParams p) {
+  using C = RowCfg<DT, MT>;
+  constexpr int CH = DT / 8;            // 16-byte chunks of a row
+  constexpr int RPI = 32 / CH;          // rows one warp-wide copy covers
+  extern __shared__ __align__(128) uint8_t smem[];
+  grid_dependents_launch();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t ring = smem_u32(smem) + warp * C::kWarp;
+  float* s_o = reinterpret_cast<float*>(smem);
+  float* s_m = reinterpret_cast<float*>(smem + C::kRing);
+  float* s_l = s_m + kRowWarps * C::kRows;
+
+  const Range rg = find_range<false>(p, blockIdx.x, C::kRows);
+  if (rg.start >= rg.end) return;
+  const int page_mask = (1 << p.page_shift) - 1;
+  const int crow = lane / CH, cchunk = lane % CH;
+  const bool cin = cchunk * 8 < p.D;
+  const char* const kc = static_cast<const char*>(p.kc);
+  const char* const vc = static_cast<const char*>(p.vc);
+
+  int b = rg.b;
+  int64_t base = rg.base, cur = rg.start;
+  SeqWork w = seq_work(p, b, C::kRows);
+  while (true) {
+    const int64_t in_seq = cur - base;
+    const int unit = static_cast<int>(in_seq / w.blocks);
+    const int blk0 = static_cast<int>(in_seq - static_cast<int64_t>(unit) * w.blocks);
+    const int nblk = static_cast<int>(min(static_cast<int64_t>(w.blocks - blk0), rg.end - cur));
+    const int h = unit / w.tiles;
+    const int row0 = (unit - h * w.tiles) * C::kRows;
+    const int rows = min(C::kRows, w.q_len * p.g - row0);      // of this tile
+
+    // Q fragments and what each of this thread's rows sees.
+    uint32_t qf[MT][DT / 16][4];
+    int lim[MT][2];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        const int r = mt * 16 + hf * 8 + lane / 4;
+        const bool in = r < rows;
+        const int tok = (row0 + r) / p.g, hd = (row0 + r) - tok * p.g;
+        lim[mt][hf] = in ? seen_keys(p, w, tok) : 0;
+        const uint16_t* src = static_cast<const uint16_t*>(p.q) +
+                              static_cast<int64_t>(w.begin + tok) * p.q_st +
+                              static_cast<int64_t>(h * p.g + hd) * p.q_sh + (lane & 3) * 2;
+#pragma unroll
+        for (int kk = 0; kk < DT / 16; ++kk)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const int d = kk * 16 + c * 8;
+            qf[mt][kk][2 * c + hf] =
+                in && d < p.D ? *reinterpret_cast<const uint32_t*>(src + d) : 0u;
+          }
+      }
+    const int tile_seen = min(w.kv_len, seen_keys(p, w, (row0 + rows - 1) / p.g));
+
+    float m[MT][2], l[MT][2], o[MT][DT / 8][4];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      m[mt][0] = m[mt][1] = -INFINITY;
+      l[mt][0] = l[mt][1] = 0.f;
+#pragma unroll
+      for (int n = 0; n < DT / 8; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[mt][n][e] = 0.f;
+    }
+
+    // This warp's 16-key steps of the blocks: those that some row sees.
+    const int key00 = blk0 * kRowKeys + warp * 16;
+    const int steps = key00 < tile_seen
+                          ? min(nblk, (tile_seen - key00 + kRowKeys - 1) / kRowKeys)
+                          : 0;
+    const int32_t* trow = p.table + b * p.table_stride;
+    auto page_of = [&](int s) {
+      if (s >= steps) return 0;
+      const int pg = page_at(trow, key00 + s * kRowKeys, p.page_shift, p.max_pages, p.pages);
+      if (pg < 0) atomicExch(p.status, kDevBadPage);
+      return pg;
+    };
+    int ids = page_of(lane), ids_next = page_of(32 + lane);
+    const int64_t kh = (h * p.kc_h + crow * p.kc_r + cchunk * 8) * 2;
+    const int64_t vh = (h * p.vc_h + crow * p.vc_r + cchunk * 8) * 2;
+    auto issue = [&](int s) {
+      if (s < steps) {
+        if (s > 0 && (s & 31) == 0) {
+          ids = ids_next;
+          ids_next = page_of(s + 32 + lane);
+        }
+        const int pg = __shfl_sync(0xffffffffu, ids, s & 31);
+        const int key0 = key00 + s * kRowKeys;
+        const int in = key0 & page_mask;
+        const int64_t pgc = pg < 0 ? 0 : pg;
+        const char* ks = kc + kh + (pgc * p.kc_p + in * p.kc_r) * 2;
+        const char* vs = vc + vh + (pgc * p.vc_p + in * p.vc_r) * 2;
+        const int left = pg < 0 || !cin ? 0 : w.kv_len - key0 - crow;   // rows it - RPI < left
+        const uint32_t st = ring + (s % C::kStages) * C::kStage;
+#pragma unroll
+        for (int it = 0; it < 16 / RPI; ++it) {
+          const int r = it * RPI + crow;
+          const uint32_t at = st + r * (DT * 2) + ((cchunk ^ (r & 7)) * 16);
+          const int n = it * RPI < left ? 16 : 0;
+          cp_async16(at, ks + (n ? it * RPI * p.kc_r * 2 : 0), n);
+          cp_async16(at + C::kTile, vs + (n ? it * RPI * p.vc_r * 2 : 0), n);
+        }
+      }
+      cp_async_commit();
+    };
+#pragma unroll
+    for (int s = 0; s < C::kStages - 1; ++s) issue(s);
+
+    for (int s = 0; s < steps; ++s) {
+      cp_async_wait<C::kStages - 2>();
+      __syncwarp();
+      issue(s + C::kStages - 1);
+      const uint32_t st = ring + (s % C::kStages) * C::kStage;
+      const int key0 = key00 + s * kRowKeys;
+      // S = Q K^T for 16 keys: two 8-key column tiles.
+      float sc[MT][2][4];
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[mt][n][e] = 0.f;
+      {
+        const int r = (lane >> 4) * 8 + (lane & 7);
+        const uint32_t row = st + r * (DT * 2);
+#pragma unroll
+        for (int kk = 0; kk < DT / 16; ++kk) {
+          uint32_t kf[4];
+          ldsm4(row + (((kk * 2 + ((lane >> 3) & 1)) ^ (r & 7)) * 16), kf);
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) {
+            mma_16816<F16>(sc[mt][0], qf[mt][kk], kf[0], kf[1]);
+            mma_16816<F16>(sc[mt][1], qf[mt][kk], kf[2], kf[3]);
+          }
+        }
+      }
+      // Online softmax in the exp2 domain.  The reference maximum is raised
+      // only when a row outgrows it by 2^8, which keeps rescales rare and the
+      // weights within the 16-bit types' range; O / l is exact for any of them.
+      uint32_t pf[MT][4];
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int key = key0 + n * 8 + (lane & 3) * 2 + (e & 1);
+            float x = sc[mt][n][e] * p.scale_log2;
+            if (key >= lim[mt][e >> 1]) x = -INFINITY;
+            sc[mt][n][e] = x;
+            mx[e >> 1] = fmaxf(mx[e >> 1], x);
+          }
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          mx[hf] = fmaxf(mx[hf], __shfl_xor_sync(0xffffffffu, mx[hf], 1));
+          mx[hf] = fmaxf(mx[hf], __shfl_xor_sync(0xffffffffu, mx[hf], 2));
+        }
+        if (__any_sync(0xffffffffu, mx[0] > m[mt][0] + 8.f || mx[1] > m[mt][1] + 8.f)) {
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf) {
+            const float mn = fmaxf(m[mt][hf], mx[hf]);
+            const float al = mn == -INFINITY ? 1.f : ex2_approx(m[mt][hf] - mn);
+            m[mt][hf] = mn;
+            l[mt][hf] *= al;
+#pragma unroll
+            for (int n = 0; n < DT / 8; ++n) {
+              o[mt][n][2 * hf] *= al;
+              o[mt][n][2 * hf + 1] *= al;
+            }
+          }
+        }
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf) {
+            const float ref = m[mt][hf] == -INFINITY ? 0.f : m[mt][hf];
+            const float p0 = ex2_approx(sc[mt][n][2 * hf] - ref);
+            const float p1 = ex2_approx(sc[mt][n][2 * hf + 1] - ref);
+            l[mt][hf] += p0 + p1;
+            pf[mt][2 * n + hf] = pack_16x2<F16>(p0, p1);
+          }
+      }
+      // O += P V.
+      {
+        const int r = ((lane >> 3) & 1) * 8 + (lane & 7);
+        const uint32_t row = st + C::kTile + r * (DT * 2);
+#pragma unroll
+        for (int nn = 0; nn < DT / 16; ++nn) {
+          uint32_t vf[4];
+          ldsm4_t(row + (((nn * 2 + (lane >> 4)) ^ (r & 7)) * 16), vf);
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) {
+            mma_16816<F16>(o[mt][2 * nn], pf[mt], vf[0], vf[1]);
+            mma_16816<F16>(o[mt][2 * nn + 1], pf[mt], vf[2], vf[3]);
+          }
+        }
+      }
+    }
+    cp_async_wait<0>();
+
+    // Join the warps: everything against the largest of the four maxima.
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        l[mt][hf] += __shfl_xor_sync(0xffffffffu, l[mt][hf], 1);
+        l[mt][hf] += __shfl_xor_sync(0xffffffffu, l[mt][hf], 2);
+        if ((lane & 3) == 0) {
+          const int r = mt * 16 + hf * 8 + lane / 4;
+          s_m[warp * C::kRows + r] = m[mt][hf];
+          s_l[warp * C::kRows + r] = l[mt][hf];
+        }
+      }
+    __syncthreads();        // also: every warp is done with its ring
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        const int r = mt * 16 + hf * 8 + lane / 4;
+        float top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kRowWarps; ++i) top = fmaxf(top, s_m[i * C::kRows + r]);
+        const float al = m[mt][hf] == -INFINITY ? 0.f : ex2_approx(m[mt][hf] - top);
+#pragma unroll
+        for (int n = 0; n < DT / 8; ++n)
+          *reinterpret_cast<float2*>(s_o + (warp * C::kRows + r) * DT + n * 8 + (lane & 3) * 2) =
+              make_float2(o[mt][n][2 * hf] * al, o[mt][n][2 * hf + 1] * al);
+      }
+    __syncthreads();
+    const bool first = blk0 == 0, last = blk0 + nblk == w.blocks;
+    float* slot = p.part + static_cast<int64_t>(2 * blockIdx.x + (first ? 1 : 0)) * C::kSlot;
+    for (int i = threadIdx.x; i < rows * (DT / 4); i += kRowThreads) {
+      const int r = i / (DT / 4), d = (i - r * (DT / 4)) * 4;
+      float top = -INFINITY, sum = 0.f;
+#pragma unroll
+      for (int k = 0; k < kRowWarps; ++k) top = fmaxf(top, s_m[k * C::kRows + r]);
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int k = 0; k < kRowWarps; ++k) {
+        const float mk = s_m[k * C::kRows + r];
+        sum += mk == -INFINITY ? 0.f : s_l[k * C::kRows + r] * ex2_approx(mk - top);
+        const float4 x = *reinterpret_cast<const float4*>(s_o + (k * C::kRows + r) * DT + d);
+        acc.x += x.x;
+        acc.y += x.y;
+        acc.z += x.z;
+        acc.w += x.w;
+      }
+      if (first && last) {
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        const int tok = (row0 + r) / p.g, hd = (row0 + r) - tok * p.g;
+        uint16_t* dst = static_cast<uint16_t*>(p.o) +
+                        static_cast<int64_t>(w.begin + tok) * p.o_st +
+                        static_cast<int64_t>(h * p.g + hd) * p.o_sh + d;
+        if (d < p.D)
+          *reinterpret_cast<uint2*>(dst) = make_uint2(pack_16x2<F16>(acc.x * inv, acc.y * inv),
+                                                      pack_16x2<F16>(acc.z * inv, acc.w * inv));
+      } else {
+        *reinterpret_cast<float4*>(slot + r * DT + d) = acc;
+        if (d == 0) {
+          slot[C::kRows * DT + r] = top;
+          slot[C::kRows * DT + C::kRows + r] = sum;
+        }
+      }
+    }
+    cur += nblk;
+    if (cur >= rg.end) break;
+    __syncthreads();        // the ring is free again
+    if (last && unit + 1 == w.tiles * p.Hkv) {
+      base += weight(p, w);
+      do {
+        w = seq_work(p, ++b, C::kRows);
+      } while (w.tiles == 0);
+    }
+  }
+}
+
+// Adds up the parts of the unit that CTA blockIdx.x's range ends in, when the
+// unit begins in that range and goes on behind it.  One warp per row.
+template <int DT, int MT, bool F16>
+__global__ void __launch_bounds__(kRowThreads)
+    paged_rows_join(const PagedParams p) {
+  using C = RowCfg<DT, MT>;
+  const int lane = threadIdx.x & 31;
+  const int r = blockIdx.y * kRowWarps + (threadIdx.x >> 5);
+  const Range rg = find_range<true>(p, blockIdx.x, C::kRows);
+  grid_dependency_wait();               // the parts are complete
+  if (rg.start >= rg.end) return;
+  const SeqWork w = seq_work(p, rg.b, C::kRows);
+  const int unit = static_cast<int>((rg.end - 1 - rg.base) / w.blocks);
+  const int64_t us = rg.base + static_cast<int64_t>(unit) * w.blocks, ue = us + w.blocks;
+  if (us < rg.start || ue <= rg.end) return;
+  const int h = unit / w.tiles;
+  const int row0 = (unit - h * w.tiles) * C::kRows;
+  if (row0 + r >= w.q_len * p.g) return;
+  const int parts = 1 + static_cast<int>((ue - rg.end + rg.per - 1) / rg.per);
+  // Part 0 is slot 1 of this CTA, part i slot 0 of the i-th CTA behind it.
+  auto slot = [&](int i) {
+    return p.part + static_cast<int64_t>(2 * (blockIdx.x + i) + (i == 0 ? 1 : 0)) * C::kSlot;
+  };
+  float top = -INFINITY;
+  for (int i = lane; i < parts; i += 32) top = fmaxf(top, slot(i)[C::kRows * DT + r]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  float sum = 0.f;
+  float acc[DT / 32];
+#pragma unroll
+  for (int e = 0; e < DT / 32; ++e) acc[e] = 0.f;
+#pragma unroll 4
+  for (int i = 0; i < parts; ++i) {
+    const float* s = slot(i);
+    const float mi = s[C::kRows * DT + r];
+    const float al = mi == -INFINITY ? 0.f : ex2_approx(mi - top);
+    sum += s[C::kRows * DT + C::kRows + r] * al;
+    if constexpr (DT == 128) {
+      const float4 x = *reinterpret_cast<const float4*>(s + r * DT + lane * 4);
+      acc[0] += x.x * al;
+      acc[1] += x.y * al;
+      acc[2] += x.z * al;
+      acc[3] += x.w * al;
+    } else {
+      const float2 x = *reinterpret_cast<const float2*>(s + r * DT + lane * 2);
+      acc[0] += x.x * al;
+      acc[1] += x.y * al;
+    }
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  const int tok = (row0 + r) / p.g, hd = (row0 + r) - tok * p.g;
+  uint16_t* dst = static_cast<uint16_t*>(p.o) + static_cast<int64_t>(w.begin + tok) * p.o_st +
+                  static_cast<int64_t>(h * p.g + hd) * p.o_sh;
+  if constexpr (DT == 128) {
+    if (lane * 4 < p.D)
+      *reinterpret_cast<uint2*>(dst + lane * 4) =
+          make_uint2(pack_16x2<F16>(acc[0] * inv, acc[1] * inv),
+                     pack_16x2<F16>(acc[2] * inv, acc[3] * inv));
+  } else {
+    if (lane * 2 < p.D)
+      *reinterpret_cast<uint32_t*>(dst + lane * 2) = pack_16x2<F16>(acc[0] * inv, acc[1] * inv);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+constexpr int kRowCtasPerSm = 2;
+
+template <int DT, int MT, bool F16>
+int launch_rows(const PagedParams& p, cudaStream_t stream) {
+  using C = RowCfg<DT, MT>;
+  static KernelPrep prep;
+  int dev = 0;
+  const int rc = prepare_kernel(
+      prep, reinterpret_cast<const void*>(paged_rows_kernel<DT, MT, F16>), C::kSmem, &dev);
+  if (rc != FA_OK) return rc;
+  paged_rows_kernel<DT, MT, F16><<<p.ctas, kRowThreads, C::kSmem, stream>>>(p);
+  if (cudaGetLastError() != cudaSuccess) return FA_ERR_LAUNCH;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(p.ctas, C::kRows / kRowWarps);
+  cfg.blockDim = dim3(kRowThreads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, paged_rows_join<DT, MT, F16>, p) == cudaSuccess ? FA_OK
+                                                                                  : FA_ERR_LAUNCH;
+}
+
+template <int DT, int MT>
+int launch_rows_t(const PagedParams& p, bool f16, cudaStream_t stream) {
+  return f16 ? launch_rows<DT, MT, true>(p, stream) : launch_rows<DT, MT, false>(p, stream);
+}
+
+bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+// Strides of `n` dimensions: multiples of 8 elements where the dimension has
+// more than one entry, not negative, and not 0 where written.
+bool strides_ok(const int64_t* st, const int64_t* sizes, int n, bool written) {
+  for (int i = 0; i < n; ++i)
+    if (sizes[i] > 1 && (st[i] < (written ? 1 : 0) || st[i] % 8 != 0)) return false;
+  return true;
+}
+
+int check_paged_attn(const fa_paged_attn_args* a) {
+  constexpr int64_t kMax = 0x7fffffffLL;
+  if (!a || !a->q || !a->o || !a->k_cache || !a->v_cache || !a->block_table || !a->kv_lens)
+    return FA_ERR_NULL;
+  if (a->dtype != FA_BF16 && a->dtype != FA_F16) return FA_ERR_ARG;
+  if (a->T <= 0 || a->B <= 0 || a->Hq <= 0 || a->Hkv <= 0 || a->T > kMax || a->B >= kMax ||
+      a->Hkv > 65536 || a->Hq > 65536 || a->Hq % a->Hkv || a->Hq / a->Hkv > 128 ||
+      a->T * (a->Hq / a->Hkv) > kMax || a->max_q_len <= 0)
+    return FA_ERR_SHAPE;
+  if (!a->cu_seqlens && a->T != a->B) return FA_ERR_SHAPE;
+  if (a->D < 8 || a->D > 128 || a->D % 8) return FA_ERR_HEAD_DIM;
+  if (a->pages <= 0 || a->pages > kMax || a->max_pages <= 0 || a->max_pages > kMax ||
+      a->page_size < 16 || a->page_size > 1024 || (a->page_size & (a->page_size - 1)))
+    return FA_ERR_SHAPE;
+  if (a->B > 1 && a->table_stride < a->max_pages) return FA_ERR_STRIDE;
+  const int64_t qs[2] = {a->T, a->Hq}, cs[3] = {a->pages, a->page_size, a->Hkv};
+  if (!strides_ok(a->q_strides, qs, 2, false) || !strides_ok(a->o_strides, qs, 2, true) ||
+      !strides_ok(a->k_cache_strides, cs, 3, false) ||
+      !strides_ok(a->v_cache_strides, cs, 3, false) || !aligned16(a->q) || !aligned16(a->o) ||
+      !aligned16(a->k_cache) || !aligned16(a->v_cache))
+    return FA_ERR_ALIGN;
+  return FA_OK;
+}
+
+// Rows of the row kernel's tiles: 16 where every sequence's rows fit, else 32.
+int row_tiles(const fa_paged_attn_args* a) {
+  return a->max_q_len * (a->Hq / a->Hkv) <= 16 ? 1 : 2;
+}
+
+}  // namespace
+}  // namespace fa
+
+extern "C" int64_t fa_paged_attn_workspace(const fa_paged_attn_args* a) {
+  using namespace fa;
+  int rc = check_paged_attn(a);
+  if (rc != FA_OK) return -rc;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return -FA_ERR_CUDA;
+  const int sms = sm_count(dev);
+  if (sms <= 0) return -FA_ERR_CUDA;
+  const int dt = a->D <= 64 ? 64 : 128;
+  return static_cast<int64_t>(2 * kRowCtasPerSm * sms) * 16 * row_tiles(a) * (dt + 2) * 4;
+}
+
+extern "C" int fa_paged_attn(const fa_paged_attn_args* a, void* workspace,
+                             int64_t workspace_bytes, void* stream) {
+  using namespace fa;
+  int rc = check_paged_attn(a);
+  if (rc != FA_OK) return rc;
+  int dev = 0;
+  if ((rc = prepare_device(nullptr, 0, &dev)) != FA_OK) return rc;
+  const int64_t need = fa_paged_attn_workspace(a);
+  if (need < 0) return static_cast<int>(-need);
+  if (!workspace || workspace_bytes < need) return FA_ERR_WORKSPACE;
+  if (!aligned16(workspace)) return FA_ERR_ALIGN;
+  PagedParams p = {};
+  p.q = a->q;
+  p.o = a->o;
+  p.kc = a->k_cache;
+  p.vc = a->v_cache;
+  p.table = a->block_table;
+  p.lens = a->kv_lens;
+  p.cu = a->cu_seqlens;
+  p.q_st = a->q_strides[0];
+  p.q_sh = a->q_strides[1];
+  p.o_st = a->o_strides[0];
+  p.o_sh = a->o_strides[1];
+  p.kc_p = a->k_cache_strides[0];
+  p.kc_r = a->k_cache_strides[1];
+  p.kc_h = a->k_cache_strides[2];
+  p.vc_p = a->v_cache_strides[0];
+  p.vc_r = a->v_cache_strides[1];
+  p.vc_h = a->v_cache_strides[2];
+  p.table_stride = a->table_stride;
+  p.T = static_cast<int>(a->T);
+  p.B = static_cast<int>(a->B);
+  p.Hkv = static_cast<int>(a->Hkv);
+  p.g = static_cast<int>(a->Hq / a->Hkv);
+  p.D = static_cast<int>(a->D);
+  p.pages = static_cast<int>(a->pages);
+  p.page_shift = __builtin_ctzll(static_cast<unsigned long long>(a->page_size));
+  p.max_pages = static_cast<int>(a->max_pages);
+  p.causal = a->causal != 0;
+  p.scale_log2 = static_cast<float>(a->scale * 1.4426950408889634);
+  p.status = device_status_ptr();
+  if (p.status == nullptr) return FA_ERR_CUDA;
+  p.part = static_cast<float*>(workspace);
+  p.ctas = kRowCtasPerSm * sm_count(dev);
+  p.min_blocks = 4;
+  const bool f16 = a->dtype == FA_F16;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (row_tiles(a) == 1)
+    return p.D <= 64 ? launch_rows_t<64, 1>(p, f16, s) : launch_rows_t<128, 1>(p, f16, s);
+  return p.D <= 64 ? launch_rows_t<64, 2>(p, f16, s) : launch_rows_t<128, 2>(p, f16, s);
+}

@@ -1,0 +1,468 @@
+// Rotary positions, alone (fa_rotary) and on the way into a paged key/value
+// cache (fa_paged_append):
+//     (a, b) -> (a cos t - b sin t, b cos t + a sin t),   t = position * inv_freq[i]
+//
+// Both are bound by HBM: each value is read once and written once.  A CTA of
+// 256 threads takes a few rows (tokens).  It loads its first vectors, computes
+// the rows' sines and cosines once into shared memory while those loads are in
+// flight, then rotates and stores; a thread's item is two 16-byte vectors R / 2
+// channels apart, so that the planes (i, i + R / 2) stay inside one thread and
+// the planes (2i, 2i + 1) inside one vector.  Every head of a row shares the
+// row's angles.
+//
+// An angle of a far position needs more than fp32: position * inv_freq is
+// formed in fp64 in turns (inv_freq / 2 pi), the whole turns are dropped
+// exactly, and the remainder (at most half a turn) goes to sincospif in fp32.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "fa_internal.h"
+#include "paged.cuh"
+#include "sm100_ptx.cuh"
+
+namespace fa {
+namespace {
+
+constexpr int kRotThreads = 256;
+constexpr int kRotItems = 2;            // items a thread loads ahead of the angles
+constexpr int kRotMaxRows = 64;         // rows of one CTA
+constexpr int kRotMaxAngles = 2048;     // angles of one CTA (16 KiB of shared memory)
+
+struct Angles {
+  const void* pos;
+  const void* freq;
+  int64_t pos_sa, pos_sb, pos_ss;       // elements: axis, batch, row
+  int sec_end[4];
+  int axes, R, pos64, freq64;
+  float sign;                           // -1 turns the other way
+};
+
+// One tensor's head vectors of a row: `heads` of them, rotated or copied.
+struct Part {
+  const void* src;
+  void* dst;
+  int64_t src_sb, src_sh, src_ss;       // elements
+  int64_t dst_sb, dst_sh, dst_ss;
+  int heads, rotate, items;             // items per head
+};
+
+struct RotParams {
+  Angles ang;
+  Part part[3];                         // append: keys, values, queries; rotary: one part
+  int parts, D;
+  int64_t rows;
+  int S;                                // rows of one batch entry
+  int rows_per_cta, items_per_row;
+  // append only
+  const int32_t* table;
+  const int32_t* kv_lens;
+  const int32_t* cu;
+  int B, pages, page_shift, max_pages;
+  int64_t table_stride;
+  int64_t kc_page, vc_page;             // cache page strides (elements)
+  int* status;
+};
+
+template <int TYPE>
+struct Elem;                            // TYPE: fa_dtype
+template <>
+struct Elem<FA_BF16> {
+  static constexpr int kSize = 2;
+};
+template <>
+struct Elem<FA_F16> {
+  static constexpr int kSize = 2;
+};
+template <>
+struct Elem<FA_F32> {
+  static constexpr int kSize = 4;
+};
+
+template <int TYPE>
+__device__ __forceinline__ void unpack(const uint4& u, float (&f)[16 / Elem<TYPE>::kSize]) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (TYPE == FA_F32) {
+      f[i] = __uint_as_float(w[i]);
+    } else {
+      f[2 * i] = unpack_16<TYPE == FA_F16>(w[i], false);
+      f[2 * i + 1] = unpack_16<TYPE == FA_F16>(w[i], true);
+    }
+  }
+}
+
+template <int TYPE>
+__device__ __forceinline__ uint4 pack(const float (&f)[16 / Elem<TYPE>::kSize]) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (TYPE == FA_F32) w[i] = __float_as_uint(f[i]);
+    else w[i] = pack_16x2<TYPE == FA_F16>(f[2 * i], f[2 * i + 1]);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+__device__ __forceinline__ float2 cos_sin(const Angles& a, int64_t b, int64_t s, int i,
+                                          bool own_pos, int place) {
+  double pos;
+  if (own_pos) {
+    pos = static_cast<double>(place);
+  } else {
+    int axis = 0;
+    while (axis + 1 < a.axes && i >= a.sec_end[axis]) ++axis;
+    const int64_t at = axis * a.pos_sa + b * a.pos_sb + s * a.pos_ss;
+    pos = a.pos64 ? static_cast<double>(static_cast<const int64_t*>(a.pos)[at])
+                  : static_cast<double>(static_cast<const int32_t*>(a.pos)[at]);
+  }
+  const double f = a.freq64 ? static_cast<const double*>(a.freq)[i]
+                            : static_cast<double>(static_cast<const float*>(a.freq)[i]);
+  const double turns = pos * (f * 0.15915494309189535);
+  float2 cs;
+  sincospif(static_cast<float>(2.0 * (turns - rint(turns))), &cs.y, &cs.x);
+  cs.y *= a.sign;
+  return cs;
+}
+
+// An item: up to two vectors of one head.
+struct Item {
+  const char* src;
+  char* dst;
+  int off0, off1;       // byte offsets of the vectors, -1: none
+  int row, chunk;
+  bool rotate;
+};
+
+// APPEND: rows are packed new tokens, keys and values go to their pages.
+template <int TYPE, bool APPEND, bool INTERLEAVED>
+__global__ void __launch_bounds__(kRotThreads)
+    rotary_kernel(const RotParams p) {
+  constexpr int kSize = Elem<TYPE>::kSize;
+  constexpr int V = 16 / kSize;
+  __shared__ float2 cs[kRotMaxAngles];
+  __shared__ int64_t s_kdst[kRotMaxRows], s_vdst[kRotMaxRows];   // element offsets, -1: no place
+  __shared__ int s_place[kRotMaxRows];
+  __shared__ int s_live[kRotMaxRows];
+
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * p.rows_per_cta;
+  const int rows = static_cast<int>(min(static_cast<int64_t>(p.rows_per_cta), p.rows - row0));
+  const int half = p.ang.R / 2;
+  const int rot_items = half / V;
+  const int total = rows * p.items_per_row;
+
+  auto locate = [&](int it) {
+    Item x;
+    x.row = it / p.items_per_row;
+    int r = it - x.row * p.items_per_row;
+    int part = 0;
+    if (APPEND) {
+      while (part + 1 < p.parts && r >= p.part[part].heads * p.part[part].items) {
+        r -= p.part[part].heads * p.part[part].items;
+        ++part;
+      }
+    }
+    const Part& q = p.part[part];
+    const int head = r / q.items;
+    x.chunk = r - head * q.items;
+    x.rotate = q.rotate != 0;
+    const int64_t row = row0 + x.row;
+    const int64_t b = APPEND ? 0 : row / p.S;
+    const int64_t s = APPEND ? row : row - b * p.S;
+    x.src = static_cast<const char*>(q.src) + (b * q.src_sb + s * q.src_ss + head * q.src_sh) * kSize;
+    x.dst = static_cast<char*>(q.dst) + (b * q.dst_sb + head * q.dst_sh) * kSize;
+    if (!APPEND || part == 2) {
+      x.dst += s * q.dst_ss * kSize;
+    } else {
+      const int64_t at = part == 0 ? s_kdst[x.row] : s_vdst[x.row];
+      x.dst = at < 0 ? nullptr : x.dst + at * kSize;
+    }
+    if (APPEND && !s_live[x.row]) x.dst = nullptr;
+    if (x.rotate && x.chunk < rot_items) {
+      x.off0 = x.chunk * 16;
+      x.off1 = (half + x.chunk * V) * kSize;
+    } else {
+      const int c0 = x.rotate ? p.ang.R + 2 * (x.chunk - rot_items) * V : 2 * x.chunk * V;
+      x.off0 = c0 * kSize;
+      x.off1 = c0 + V < p.D ? (c0 + V) * kSize : -1;
+      x.rotate = false;
+    }
+    return x;
+  };
+
+  if (APPEND) {
+    // Where each row goes.
+    if (threadIdx.x < rows) {
+      const int r = threadIdx.x;
+      const int t = static_cast<int>(row0) + r;
+      const int b = seq_of_row(p.cu, p.B, t);
+      s_live[r] = b >= 0;
+      s_kdst[r] = s_vdst[r] = -1;
+      s_place[r] = 0;
+      if (b >= 0) {
+        const int end = p.cu == nullptr ? b + 1 : p.cu[b + 1];
+        const int place = p.kv_lens[b] - (end - t);
+        s_place[r] = place;
+        if (place >= 0) {
+          const int page = page_at(p.table + b * p.table_stride, place, p.page_shift, p.max_pages,
+                                   p.pages);
+          if (page >= 0) {
+            const int in = place & ((1 << p.page_shift) - 1);
+            s_kdst[r] = page * p.kc_page + in * p.part[0].dst_ss;
+            s_vdst[r] = page * p.vc_page + in * p.part[1].dst_ss;
+          } else {
+            atomicExch(p.status, kDevBadPage);
+          }
+        }
+      }
+    }
+    __syncthreads();
+  }
+
+  // The first items' loads are in flight while the angles are computed.
+  uint4 a[kRotItems], c[kRotItems];
+#pragma unroll
+  for (int u = 0; u < kRotItems; ++u) {
+    const int it = threadIdx.x + u * kRotThreads;
+    if (it < total) {
+      const Item x = locate(it);
+      if (x.dst != nullptr) {
+        a[u] = *reinterpret_cast<const uint4*>(x.src + x.off0);
+        if (x.off1 >= 0) c[u] = *reinterpret_cast<const uint4*>(x.src + x.off1);
+      }
+    }
+  }
+  for (int i = threadIdx.x; i < rows * half; i += kRotThreads) {
+    const int r = i / half;
+    const int64_t row = row0 + r;
+    const int64_t b = APPEND ? 0 : row / p.S;
+    if (!APPEND || s_live[r])
+      cs[i] = cos_sin(p.ang, b, row - b * p.S, i - r * half, p.ang.pos == nullptr,
+                      APPEND ? s_place[r] : 0);
+  }
+  __syncthreads();
+
+  auto finish = [&](const Item& x, const uint4& u0, const uint4& u1) {
+    if (!x.rotate) {
+      *reinterpret_cast<uint4*>(x.dst + x.off0) = u0;
+      if (x.off1 >= 0) *reinterpret_cast<uint4*>(x.dst + x.off1) = u1;
+      return;
+    }
+    float f[V], g[V];
+    unpack<TYPE>(u0, f);
+    unpack<TYPE>(u1, g);
+    const float2* w = cs + x.row * half;
+    if (INTERLEAVED) {
+      const int i0 = x.chunk * V / 2, i1 = half / 2 + x.chunk * V / 2;
+#pragma unroll
+      for (int e = 0; e < V; e += 2) {
+        const float2 r = w[i0 + e / 2], q = w[i1 + e / 2];
+        const float f0 = f[e], g0 = g[e];
+        f[e] = fmaf(f0, r.x, -f[e + 1] * r.y);
+        f[e + 1] = fmaf(f[e + 1], r.x, f0 * r.y);
+        g[e] = fmaf(g0, q.x, -g[e + 1] * q.y);
+        g[e + 1] = fmaf(g[e + 1], q.x, g0 * q.y);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const float2 r = w[x.chunk * V + e];
+        const float f0 = f[e];
+        f[e] = fmaf(f0, r.x, -g[e] * r.y);
+        g[e] = fmaf(g[e], r.x, f0 * r.y);
+      }
+    }
+    *reinterpret_cast<uint4*>(x.dst + x.off0) = pack<TYPE>(f);
+    *reinterpret_cast<uint4*>(x.dst + x.off1) = pack<TYPE>(g);
+  };
+#pragma unroll
+  for (int u = 0; u < kRotItems; ++u) {
+    const int it = threadIdx.x + u * kRotThreads;
+    if (it < total) {
+      const Item x = locate(it);
+      if (x.dst != nullptr) finish(x, a[u], c[u]);
+    }
+  }
+  for (int it = threadIdx.x + kRotItems * kRotThreads; it < total; it += kRotThreads) {
+    const Item x = locate(it);
+    if (x.dst == nullptr) continue;
+    const uint4 u0 = *reinterpret_cast<const uint4*>(x.src + x.off0);
+    uint4 u1 = u0;
+    if (x.off1 >= 0) u1 = *reinterpret_cast<const uint4*>(x.src + x.off1);
+    finish(x, u0, u1);
+  }
+}
+
+int launch_rotary(RotParams& p, int dtype, bool append, bool interleaved, cudaStream_t stream) {
+  int dev = 0;
+  const int rc = prepare_device(nullptr, 0, &dev);
+  if (rc != FA_OK) return rc;
+  const int V = dtype == FA_F32 ? 4 : 8;
+  const int half = p.ang.R / 2;
+  p.items_per_row = 0;
+  for (int i = 0; i < p.parts; ++i) {
+    Part& q = p.part[i];
+    const int rest = q.rotate ? p.D - p.ang.R : p.D;
+    q.items = (q.rotate ? half / V : 0) + (rest / V + 1) / 2;
+    p.items_per_row += q.heads * q.items;
+  }
+  // Rows per CTA: as many as its threads take in one go, within the shared
+  // memory for their angles.
+  int rows = kRotThreads * kRotItems / p.items_per_row;
+  if (half > 0) rows = rows < kRotMaxAngles / half ? rows : kRotMaxAngles / half;
+  rows = rows < kRotMaxRows ? rows : kRotMaxRows;
+  p.rows_per_cta = rows > 1 ? rows : 1;
+  const int64_t grid = (p.rows + p.rows_per_cta - 1) / p.rows_per_cta;
+  if (grid > 0x7fffffffLL) return FA_ERR_SHAPE;
+  const unsigned g = static_cast<unsigned>(grid);
+  if (append) {
+    p.status = device_status_ptr();
+    if (p.status == nullptr) return FA_ERR_CUDA;
+  }
+#define FA_ROT(T, A, I) rotary_kernel<T, A, I><<<g, kRotThreads, 0, stream>>>(p)
+  if (append) {
+    if (dtype == FA_BF16) interleaved ? FA_ROT(FA_BF16, true, true) : FA_ROT(FA_BF16, true, false);
+    else interleaved ? FA_ROT(FA_F16, true, true) : FA_ROT(FA_F16, true, false);
+  } else if (dtype == FA_BF16) {
+    interleaved ? FA_ROT(FA_BF16, false, true) : FA_ROT(FA_BF16, false, false);
+  } else if (dtype == FA_F16) {
+    interleaved ? FA_ROT(FA_F16, false, true) : FA_ROT(FA_F16, false, false);
+  } else {
+    interleaved ? FA_ROT(FA_F32, false, true) : FA_ROT(FA_F32, false, false);
+  }
+#undef FA_ROT
+  return cudaGetLastError() == cudaSuccess ? FA_OK : FA_ERR_LAUNCH;
+}
+
+constexpr int64_t kMaxDim = 0x7fffffffLL;
+
+bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+// Strides of `n` dimensions of the given sizes: multiples of 16 bytes where the
+// dimension has more than one entry, not negative, and not 0 where written.
+bool strides_ok(const int64_t* st, const int64_t* sizes, int n, int elem, bool written) {
+  for (int i = 0; i < n; ++i)
+    if (sizes[i] > 1 && (st[i] < (written ? 1 : 0) || (st[i] * elem) % 16 != 0)) return false;
+  return true;
+}
+
+int check_sections(int64_t axes, const int64_t* end, int64_t R) {
+  if (axes < 1 || axes > 4) return FA_ERR_ARG;
+  int64_t last = 0;
+  for (int a = 0; a < axes; ++a) {
+    if (end[a] <= last) return FA_ERR_ARG;
+    last = end[a];
+  }
+  return last == R / 2 ? FA_OK : FA_ERR_ARG;
+}
+
+void set_angles(Angles& a, const void* pos, const void* freq, int64_t axes, const int64_t* end,
+                int64_t R, int64_t pos64, int64_t freq64, bool inverse) {
+  a.pos = pos;
+  a.freq = freq;
+  a.axes = static_cast<int>(axes);
+  for (int i = 0; i < 4; ++i) a.sec_end[i] = i < axes ? static_cast<int>(end[i]) : 0;
+  a.R = static_cast<int>(R);
+  a.pos64 = pos64 != 0;
+  a.freq64 = freq64 != 0;
+  a.sign = inverse ? -1.f : 1.f;
+}
+
+}  // namespace
+}  // namespace fa
+
+extern "C" int fa_rotary(const fa_rotary_args* a, void* stream) {
+  using namespace fa;
+  if (!a || !a->x || !a->out || !a->positions || !a->inv_freq) return FA_ERR_NULL;
+  if (a->dtype < FA_BF16 || a->dtype > FA_F32) return FA_ERR_ARG;
+  if (a->B <= 0 || a->H <= 0 || a->S <= 0 || a->B > kMaxDim || a->H > 65536 || a->S > kMaxDim)
+    return FA_ERR_SHAPE;
+  if (a->D < 16 || a->D > 1024 || a->D % 8 || a->R < 16 || a->R > a->D || a->R % 16)
+    return FA_ERR_HEAD_DIM;
+  const int rc = check_sections(a->axes, a->section_end, a->R);
+  if (rc != FA_OK) return rc;
+  const int elem = a->dtype == FA_F32 ? 4 : 2;
+  const int64_t sizes[3] = {a->B, a->H, a->S};
+  if (!strides_ok(a->x_strides, sizes, 3, elem, false) ||
+      !strides_ok(a->out_strides, sizes, 3, elem, true) ||
+      !aligned16(a->x) || !aligned16(a->out))
+    return FA_ERR_ALIGN;
+  RotParams p = {};
+  set_angles(p.ang, a->positions, a->inv_freq, a->axes, a->section_end, a->R, a->pos_is_i64,
+             a->freq_is_f64, a->inverse != 0);
+  p.ang.pos_sa = a->pos_strides[0];
+  p.ang.pos_sb = a->pos_strides[1];
+  p.ang.pos_ss = a->pos_strides[2];
+  p.parts = 1;
+  p.part[0] = {a->x, a->out, a->x_strides[0], a->x_strides[1], a->x_strides[2],
+               a->out_strides[0], a->out_strides[1], a->out_strides[2],
+               static_cast<int>(a->H), 1, 0};
+  p.D = static_cast<int>(a->D);
+  p.rows = a->B * a->S;
+  p.S = static_cast<int>(a->S);
+  return launch_rotary(p, static_cast<int>(a->dtype), false, a->interleaved != 0,
+                       static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int fa_paged_append(const fa_paged_append_args* a, void* stream) {
+  using namespace fa;
+  if (!a || !a->k || !a->v || !a->k_cache || !a->v_cache || !a->block_table || !a->kv_lens)
+    return FA_ERR_NULL;
+  if ((a->R > 0 && !a->inv_freq) || (a->q != nullptr) != (a->q_out != nullptr)) return FA_ERR_NULL;
+  if (a->dtype != FA_BF16 && a->dtype != FA_F16) return FA_ERR_ARG;
+  if (a->T <= 0 || a->B <= 0 || a->Hkv <= 0 || a->T > kMaxDim || a->B >= kMaxDim ||
+      a->Hkv > 65536 || (a->q && (a->Hq <= 0 || a->Hq > 65536)))
+    return FA_ERR_SHAPE;
+  if (!a->cu_seqlens && a->T != a->B) return FA_ERR_SHAPE;
+  if (a->D < 8 || a->D > 1024 || a->D % 8 || a->R < 0 || a->R > a->D || a->R % 16)
+    return FA_ERR_HEAD_DIM;
+  if (a->pages <= 0 || a->pages > kMaxDim || a->max_pages <= 0 || a->max_pages > kMaxDim ||
+      a->page_size < 16 || a->page_size > 1024 || (a->page_size & (a->page_size - 1)))
+    return FA_ERR_SHAPE;
+  if (a->B > 1 && a->table_stride < a->max_pages) return FA_ERR_STRIDE;
+  if (a->R > 0) {
+    const int rc = check_sections(a->axes, a->section_end, a->R);
+    if (rc != FA_OK) return rc;
+    if (a->axes > 1 && !a->positions) return FA_ERR_NULL;
+  }
+  const int64_t ks[2] = {a->T, a->Hkv}, qs[2] = {a->T, a->Hq};
+  const int64_t cs[3] = {a->pages, a->page_size, a->Hkv};
+  if (!strides_ok(a->k_strides, ks, 2, 2, false) || !strides_ok(a->v_strides, ks, 2, 2, false) ||
+      !strides_ok(a->k_cache_strides, cs, 3, 2, true) ||
+      !strides_ok(a->v_cache_strides, cs, 3, 2, true) ||
+      !aligned16(a->k) || !aligned16(a->v) || !aligned16(a->k_cache) || !aligned16(a->v_cache))
+    return FA_ERR_ALIGN;
+  if (a->q && (!strides_ok(a->q_strides, qs, 2, 2, false) ||
+               !strides_ok(a->q_out_strides, qs, 2, 2, true) || !aligned16(a->q) || !aligned16(a->q_out)))
+    return FA_ERR_ALIGN;
+  RotParams p = {};
+  set_angles(p.ang, a->positions, a->inv_freq, a->axes, a->section_end, a->R, a->pos_is_i64,
+             a->freq_is_f64, false);
+  p.ang.pos_sa = a->pos_strides[0];
+  p.ang.pos_ss = a->pos_strides[1];
+  const int rotate = a->R > 0;
+  p.part[0] = {a->k, a->k_cache, 0, a->k_strides[1], a->k_strides[0], 0, a->k_cache_strides[2],
+               a->k_cache_strides[1], static_cast<int>(a->Hkv), rotate, 0};
+  p.part[1] = {a->v, a->v_cache, 0, a->v_strides[1], a->v_strides[0], 0, a->v_cache_strides[2],
+               a->v_cache_strides[1], static_cast<int>(a->Hkv), 0, 0};
+  p.parts = 2;
+  if (a->q) {
+    p.part[2] = {a->q, a->q_out, 0, a->q_strides[1], a->q_strides[0], 0, a->q_out_strides[1],
+                 a->q_out_strides[0], static_cast<int>(a->Hq), rotate, 0};
+    p.parts = 3;
+  }
+  p.D = static_cast<int>(a->D);
+  p.rows = a->T;
+  p.S = static_cast<int>(a->T);
+  p.table = a->block_table;
+  p.kv_lens = a->kv_lens;
+  p.cu = a->cu_seqlens;
+  p.B = static_cast<int>(a->B);
+  p.pages = static_cast<int>(a->pages);
+  p.page_shift = __builtin_ctzll(static_cast<unsigned long long>(a->page_size));
+  p.max_pages = static_cast<int>(a->max_pages);
+  p.table_stride = a->table_stride;
+  p.kc_page = a->k_cache_strides[0];
+  p.vc_page = a->v_cache_strides[0];
+  return launch_rotary(p, static_cast<int>(a->dtype), true, a->interleaved != 0,
+                       static_cast<cudaStream_t>(stream));
+}

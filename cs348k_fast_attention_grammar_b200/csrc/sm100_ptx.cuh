@@ -17,6 +17,7 @@ namespace fa {
 enum : int {
   kDevOk = 0,
   kDevTimeout = 1,   // an mbarrier wait exceeded kWaitLimitNs
+  kDevBadPage = 2,   // a block table entry or a length points outside the cache
 };
 
 // One second is ~1000x longer than any legitimate wait in these kernels.

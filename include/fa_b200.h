@@ -57,8 +57,17 @@ typedef enum fa_status {
   FA_ERR_ARG = 10,         /* an enum argument is out of range                  */
   FA_ERR_TIMEOUT = 11,     /* a kernel wait ran out (read by fa_device_status)  */
   FA_ERR_CUDA = 12,        /* another CUDA runtime call failed                  */
-  FA_ERR_SCRATCH = 13      /* problem exceeds fa_mlp_fwd_noalloc's fixed buffer */
+  FA_ERR_SCRATCH = 13,     /* problem exceeds fa_mlp_fwd_noalloc's fixed buffer */
+  FA_ERR_PAGE = 14,        /* a block table entry or a length points outside the
+                              cache (read by fa_device_status)                  */
+  FA_ERR_WORKSPACE = 15    /* the workspace is missing or too small             */
 } fa_status;
+
+typedef enum fa_dtype {
+  FA_BF16 = 0,
+  FA_F16 = 1,
+  FA_F32 = 2
+} fa_dtype;
 
 typedef enum fa_f32_precision {
   FA_F32_BF16 = 0,         /* fp32 operands rounded to bf16 (8 significant bits) */
@@ -214,6 +223,121 @@ int fa_mlp_fwd_noalloc(const void* x, const void* w1, const void* w2, void* y, i
                        int N, int act, void* stream);
 
 /*
+ * Rotary positions.  The first R of each head's D channels are rotated in
+ * R / 2 planes (a, b):
+ *     (a, b) -> (a cos t - b sin t, b cos t + a sin t),  t = position * inv_freq[i]
+ * (t negated when `inverse`, which is also the gradient); the rest is copied.
+ * Plane i is channels (i, i + R / 2), or (2i, 2i + 1) when `interleaved`.
+ * Frequencies [section_end[a-1], section_end[a]) take the position of axis a
+ * (images and video: time, height, width); one axis takes all of them.
+ * Angles are formed in fp64 and reduced before the fp32 sine and cosine, so far
+ * positions keep full precision; each value is rounded once.
+ */
+typedef struct fa_rotary_args {
+  const void* x;           /* [B, H, S, D], D contiguous                        */
+  void* out;               /* the same shape; may be x itself                   */
+  const void* positions;   /* int32 or int64 [axes, B, S], strides below        */
+  const void* inv_freq;    /* fp32 or fp64 [R / 2], contiguous                  */
+  int64_t dtype;           /* fa_dtype of x and out                             */
+  int64_t B, H, S, D, R;   /* D a multiple of 8, R a multiple of 16, R <= D     */
+  int64_t x_strides[3];    /* elements: b, h, s; multiples of 16 bytes          */
+  int64_t out_strides[3];
+  int64_t axes;            /* 1 .. 4                                            */
+  int64_t section_end[4];  /* rising; section_end[axes - 1] = R / 2             */
+  int64_t pos_strides[3];  /* elements: axis, b, s (0 repeats)                  */
+  int64_t pos_is_i64, freq_is_f64;
+  int64_t interleaved, inverse;
+} fa_rotary_args;
+
+int fa_rotary(const fa_rotary_args* args, void* stream);
+
+/*
+ * Paged key/value cache.  Caches are [pages, page_size, Hkv, D] (any strides,
+ * D contiguous); key j of sequence b is row j % page_size of page
+ * block_table[b, j / page_size].  New tokens of all sequences are packed along
+ * T: those of sequence b are rows [cu_seqlens[b], cu_seqlens[b + 1]) (row b
+ * alone when cu_seqlens is NULL), and kv_lens[b] is the sequence's length with
+ * them counted, so new token i of q_len sits at kv_lens[b] - q_len + i.
+ *
+ * fa_paged_append writes the keys, rotated as in fa_rotary when R > 0, and the
+ * values of new tokens to their places, and the rotated queries, where there
+ * are any, to q_out.  Without `positions` a token is rotated by its place in
+ * the sequence.  Rows outside every sequence are neither read nor written; a
+ * token before its sequence's start (kv_lens[b] < q_len, as in padding
+ * sequences of length 0) is not stored.  A place outside the table or a page
+ * outside the cache is not written either and leaves FA_ERR_PAGE in the device
+ * status word.  Two tokens with the same place leave either's values there.
+ */
+typedef struct fa_paged_append_args {
+  const void* k;           /* [T, Hkv, D]                                       */
+  const void* v;
+  const void* q;           /* [T, Hq, D] or NULL                                */
+  void* q_out;             /* may be q itself                                   */
+  void* k_cache;
+  void* v_cache;
+  const int32_t* block_table;  /* [B, max_pages], row stride table_stride       */
+  const int32_t* kv_lens;      /* [B]                                           */
+  const int32_t* cu_seqlens;   /* [B + 1] or NULL (then T = B)                  */
+  const void* positions;       /* int32 or int64 [axes, T] or NULL              */
+  const void* inv_freq;        /* [R / 2]; NULL when R = 0                      */
+  int64_t dtype;               /* FA_BF16 or FA_F16, all tensors alike          */
+  int64_t T, B, Hq, Hkv, D, R; /* R = 0: no rotation                            */
+  int64_t pages, page_size;    /* page_size a power of two, 16 .. 1024          */
+  int64_t max_pages, table_stride;
+  int64_t k_strides[2], v_strides[2], q_strides[2], q_out_strides[2]; /* token, head */
+  int64_t k_cache_strides[3], v_cache_strides[3];                     /* page, row, head */
+  int64_t axes;
+  int64_t section_end[4];
+  int64_t pos_strides[2];      /* axis, token                                   */
+  int64_t pos_is_i64, freq_is_f64;
+  int64_t interleaved;
+} fa_paged_append_args;
+
+int fa_paged_append(const fa_paged_append_args* args, void* stream);
+
+/*
+ * Attention of new tokens (one or a chunk per sequence) over the paged cache
+ * that holds them:  o = softmax(q K^T * scale) V  per token and head, query
+ * heads in Hkv groups that share a key/value head.  With `causal` a token sees
+ * the keys up to its own place, else all kv_lens[b].  A token that sees no key
+ * gets zeros.  Rows outside every sequence are neither read nor written.
+ * A page outside the cache reads as zeros and a length behind the table is cut
+ * there; both leave FA_ERR_PAGE in the device status word.  Cached values that
+ * a sequence's tokens see must be finite (a value that only some of a chunk's
+ * tokens see may reach the others as value * 0); rows behind kv_lens[b] may
+ * hold anything.
+ *   max_q_len : an upper bound of the tokens per sequence that only guides
+ *               which kernels run (T where unknown); results hold for any value.
+ *   workspace : fa_paged_attn_workspace(args) bytes, 16-byte aligned, used by
+ *               this call alone until it has run.
+ */
+typedef struct fa_paged_attn_args {
+  const void* q;           /* [T, Hq, D]                                        */
+  void* o;                 /* [T, Hq, D]                                        */
+  const void* k_cache;     /* [pages, page_size, Hkv, D]                        */
+  const void* v_cache;
+  const int32_t* block_table;  /* [B, max_pages], row stride table_stride       */
+  const int32_t* kv_lens;      /* [B]                                           */
+  const int32_t* cu_seqlens;   /* [B + 1] or NULL (then T = B)                  */
+  int64_t dtype;               /* FA_BF16 or FA_F16, all tensors alike          */
+  int64_t T, B, Hq, Hkv, D;    /* D 8 .. 128, a multiple of 8; Hq / Hkv <= 128  */
+  int64_t pages, page_size;    /* page_size a power of two, 16 .. 1024          */
+  int64_t max_pages, table_stride;
+  int64_t q_strides[2], o_strides[2];                                 /* token, head */
+  int64_t k_cache_strides[3], v_cache_strides[3];                     /* page, row, head */
+  int64_t max_q_len;
+  int64_t causal;
+  double scale;
+} fa_paged_attn_args;
+
+/* Bytes of workspace that fa_paged_attn needs for these arguments, or minus an
+ * fa_status.  Depends on the sizes alone, not on what the arrays hold. */
+int64_t fa_paged_attn_workspace(const fa_paged_attn_args* args);
+
+int fa_paged_attn(const fa_paged_attn_args* args, void* workspace, int64_t workspace_bytes,
+                  void* stream);
+
+/*
  * Failure-detection self test: launches one CTA that waits on an mbarrier no
  * one ever arrives on, with a limit of limit_us microseconds (1 .. 10^6).  The
  * bounded wait gives up, records FA_ERR_TIMEOUT in the device status word and
@@ -238,7 +362,8 @@ int fa_selftest_exp2(const float* x, float* out, int n, void* stream);
 
 /*
  * Reads and clears the device-side status word of the current device
- * (FA_OK, or FA_ERR_TIMEOUT when a kernel's bounded wait ran out).
+ * (FA_OK, FA_ERR_TIMEOUT when a kernel's bounded wait ran out, or FA_ERR_PAGE
+ * when a paged operator met a place outside the cache).
  * Synchronises the device.
  */
 int fa_device_status(void);
