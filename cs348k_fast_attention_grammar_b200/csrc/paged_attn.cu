@@ -20,34 +20,13 @@
 // depend on timing.
 #include <cuda_bf16.h>
 
-#include "fa_internal.h"
-#include "paged.cuh"
-#include "sm100_ptx.cuh"
+#include <climits>
+#include <cmath>
+
+#include "paged_attn.h"
 
 namespace fa {
 namespace {
-
-struct PagedParams {
-  const void* q;
-  void* o;
-  const void* kc;
-  const void* vc;
-  const int32_t* table;
-  const int32_t* lens;
-  const int32_t* cu;
-  int64_t q_st, q_sh, o_st, o_sh;       // elements: token, head
-  int64_t kc_p, kc_r, kc_h;             // page, row, head
-  int64_t vc_p, vc_r, vc_h;
-  int64_t table_stride;
-  int T, B, Hkv, g, D;
-  int pages, page_shift, max_pages;
-  int causal;
-  float scale_log2;
-  int* status;
-  float* part;                          // partial results of split units
-  int ctas;                             // ranges the key blocks are cut into
-  int min_blocks;                       // least key blocks of a range
-};
 
 // ---------------------------------------------------------------------------
 // Schedule of the row kernel
@@ -56,25 +35,19 @@ constexpr int kRowThreads = 128;
 constexpr int kRowWarps = 4;
 constexpr int kRowKeys = 64;            // keys of a block: 16 per warp
 
-// A sequence's rows and key blocks.
-struct SeqWork {
-  int begin, q_len, kv_len, tiles, blocks;
+// A sequence's row tiles and key blocks.
+struct RowWork : SeqWork {
+  int tiles, blocks;
 };
 
-__device__ __forceinline__ SeqWork seq_work(const PagedParams& p, int b, int tile_rows) {
-  SeqWork w;
-  const SeqRows r = seq_rows(p.cu, b, p.T);
-  w.begin = r.begin;
-  w.q_len = r.end - r.begin;
-  const int len = p.lens[b];
-  w.kv_len = held_len(len, p.page_shift, p.max_pages);
-  if (len > w.kv_len && len > 0) atomicExch(p.status, kDevBadPage);
-  const int64_t rows = static_cast<int64_t>(w.q_len) * p.g;
-  w.tiles = static_cast<int>((rows + tile_rows - 1) / tile_rows);
+__device__ __forceinline__ RowWork row_work(const PagedParams& p, int b, int tile_rows) {
+  RowWork w;
+  static_cast<SeqWork&>(w) = seq_work(p, b);
+  w.tiles = static_cast<int>((w.rows + tile_rows - 1) / tile_rows);
   w.blocks = max(1, (w.kv_len + kRowKeys - 1) / kRowKeys);
   return w;
 }
-__device__ __forceinline__ int64_t weight(const PagedParams& p, const SeqWork& w) {
+__device__ __forceinline__ int64_t weight(const PagedParams& p, const RowWork& w) {
   return static_cast<int64_t>(w.tiles) * p.Hkv * w.blocks;
 }
 
@@ -118,7 +91,7 @@ __device__ __forceinline__ Range find_range(const PagedParams& p, int cta, int t
   int64_t first_w = 0, first_before = 0;      // the scan of the first kRowThreads sequences
   for (int b0 = 0; b0 < p.B; b0 += kRowThreads) {
     const int b = b0 + threadIdx.x;
-    const int64_t w = b < p.B ? weight(p, seq_work(p, b, tile_rows)) : 0;
+    const int64_t w = b < p.B ? weight(p, row_work(p, b, tile_rows)) : 0;
     int64_t sum;
     const int64_t before = block_scan(w, red, &sum);
     if (b0 == 0) {
@@ -139,7 +112,7 @@ __device__ __forceinline__ Range find_range(const PagedParams& p, int cta, int t
       const int b = b0 + threadIdx.x;
       int64_t w = first_w, before = first_before, sum = 0;
       if (p.B > kRowThreads) {
-        w = b < p.B ? weight(p, seq_work(p, b, tile_rows)) : 0;
+        w = b < p.B ? weight(p, row_work(p, b, tile_rows)) : 0;
         before = block_scan(w, red, &sum);
       }
       if (w > 0 && base + before <= at && at < base + before + w) {
@@ -197,11 +170,6 @@ __device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4],
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Keys [0, limit) that token i of the sequence sees.
-__device__ __forceinline__ int seen_keys(const PagedParams& p, const SeqWork& w, int i) {
-  return p.causal ? max(0, w.kv_len - w.q_len + i + 1) : w.kv_len;
-}
-
 template <int DT, int MT>
 struct RowCfg {
   static constexpr int kRows = 16 * MT;
@@ -239,7 +207,7 @@ __global__ void __launch_bounds__(kRowThreads)
 
   int b = rg.b;
   int64_t base = rg.base, cur = rg.start;
-  SeqWork w = seq_work(p, b, C::kRows);
+  RowWork w = row_work(p, b, C::kRows);
   while (true) {
     const int64_t in_seq = cur - base;
     const int unit = static_cast<int>(in_seq / w.blocks);
@@ -491,7 +459,7 @@ __global__ void __launch_bounds__(kRowThreads)
     if (last && unit + 1 == w.tiles * p.Hkv) {
       base += weight(p, w);
       do {
-        w = seq_work(p, ++b, C::kRows);
+        w = row_work(p, ++b, C::kRows);
       } while (w.tiles == 0);
     }
   }
@@ -508,7 +476,7 @@ __global__ void __launch_bounds__(kRowThreads)
   const Range rg = find_range<true>(p, blockIdx.x, C::kRows);
   grid_dependency_wait();               // the parts are complete
   if (rg.start >= rg.end) return;
-  const SeqWork w = seq_work(p, rg.b, C::kRows);
+  const RowWork w = row_work(p, rg.b, C::kRows);
   const int unit = static_cast<int>((rg.end - 1 - rg.base) / w.blocks);
   const int64_t us = rg.base + static_cast<int64_t>(unit) * w.blocks, ue = us + w.blocks;
   if (us < rg.start || ue <= rg.end) return;
@@ -605,18 +573,20 @@ bool strides_ok(const int64_t* st, const int64_t* sizes, int n, bool written) {
 }
 
 int check_paged_attn(const fa_paged_attn_args* a) {
-  constexpr int64_t kMax = 0x7fffffffLL;
+  constexpr int64_t kMax = 0x7fffffffLL, kMaxPlaces = kMax - 4096;
   if (!a || !a->q || !a->o || !a->k_cache || !a->v_cache || !a->block_table || !a->kv_lens)
     return FA_ERR_NULL;
   if (a->dtype != FA_BF16 && a->dtype != FA_F16) return FA_ERR_ARG;
   if (a->T <= 0 || a->B <= 0 || a->Hq <= 0 || a->Hkv <= 0 || a->T > kMax || a->B >= kMax ||
       a->Hkv > 65536 || a->Hq > 65536 || a->Hq % a->Hkv || a->Hq / a->Hkv > 128 ||
-      a->T * (a->Hq / a->Hkv) > kMax || a->max_q_len <= 0)
+      a->T * a->Hq > kMax || a->max_q_len <= 0)
     return FA_ERR_SHAPE;
   if (!a->cu_seqlens && a->T != a->B) return FA_ERR_SHAPE;
   if (a->D < 8 || a->D > 128 || a->D % 8) return FA_ERR_HEAD_DIM;
+  if (!std::isfinite(a->scale)) return FA_ERR_ARG;
   if (a->pages <= 0 || a->pages > kMax || a->max_pages <= 0 || a->max_pages > kMax ||
-      a->page_size < 16 || a->page_size > 1024 || (a->page_size & (a->page_size - 1)))
+      a->page_size < 16 || a->page_size > 1024 || (a->page_size & (a->page_size - 1)) ||
+      a->max_pages * a->page_size > kMaxPlaces)
     return FA_ERR_SHAPE;
   if (a->B > 1 && a->table_stride < a->max_pages) return FA_ERR_STRIDE;
   const int64_t qs[2] = {a->T, a->Hq}, cs[3] = {a->pages, a->page_size, a->Hkv};
@@ -628,9 +598,37 @@ int check_paged_attn(const fa_paged_attn_args* a) {
   return FA_OK;
 }
 
-// Rows of the row kernel's tiles: 16 where every sequence's rows fit, else 32.
-int row_tiles(const fa_paged_attn_args* a) {
-  return a->max_q_len * (a->Hq / a->Hkv) <= 16 ? 1 : 2;
+// Which kernels run.  The row kernel takes sequences of up to kRowMax rows and
+// the tile kernel the others; only one of them runs where the longest sequence
+// is short, where all are alike (T = B * max_q_len) or there is only one, and it
+// then takes whatever it finds.
+constexpr int kRowMax = 32;
+
+struct Choice {
+  bool rows, tiles;
+  int row_tiles;        // the row kernel's tiles: 16 rows where every sequence fits, else 32
+};
+
+Choice choose(const fa_paged_attn_args* a) {
+  const int64_t g = a->Hq / a->Hkv;
+  const int64_t longest = a->max_q_len < a->T ? a->max_q_len : a->T;
+  Choice c = {true, true, 2};
+  // The tile kernel's copies need real strides, its exponent a scale that keeps order.
+  const bool flat = (a->q_strides[0] == 0 && a->T > 1) || (a->q_strides[1] == 0 && a->Hq > 1) ||
+                    (a->k_cache_strides[0] == 0 && a->pages > 1) || a->k_cache_strides[1] == 0 ||
+                    (a->k_cache_strides[2] == 0 && a->Hkv > 1) ||
+                    (a->v_cache_strides[0] == 0 && a->pages > 1) || a->v_cache_strides[1] == 0 ||
+                    (a->v_cache_strides[2] == 0 && a->Hkv > 1);
+  if (longest * g <= kRowMax || flat || a->scale < 0) c.tiles = false;
+  else if (a->B == 1 || a->T == a->B * longest) c.rows = false;
+  if (longest * g <= 16) c.row_tiles = 1;
+  return c;
+}
+
+int64_t rows_bytes(const fa_paged_attn_args* a, const Choice& c, int sms) {
+  if (!c.rows) return 0;
+  const int dt = a->D <= 64 ? 64 : 128;
+  return static_cast<int64_t>(2 * kRowCtasPerSm * sms) * 16 * c.row_tiles * (dt + 2) * 4;
 }
 
 }  // namespace
@@ -644,8 +642,8 @@ extern "C" int64_t fa_paged_attn_workspace(const fa_paged_attn_args* a) {
   if (cudaGetDevice(&dev) != cudaSuccess) return -FA_ERR_CUDA;
   const int sms = sm_count(dev);
   if (sms <= 0) return -FA_ERR_CUDA;
-  const int dt = a->D <= 64 ? 64 : 128;
-  return static_cast<int64_t>(2 * kRowCtasPerSm * sms) * 16 * row_tiles(a) * (dt + 2) * 4;
+  const Choice c = choose(a);
+  return rows_bytes(a, c, sms) + (c.tiles ? paged_tiles_bytes(a, sms) : 0);
 }
 
 extern "C" int fa_paged_attn(const fa_paged_attn_args* a, void* workspace,
@@ -690,12 +688,25 @@ extern "C" int fa_paged_attn(const fa_paged_attn_args* a, void* workspace,
   p.scale_log2 = static_cast<float>(a->scale * 1.4426950408889634);
   p.status = device_status_ptr();
   if (p.status == nullptr) return FA_ERR_CUDA;
-  p.part = static_cast<float*>(workspace);
-  p.ctas = kRowCtasPerSm * sm_count(dev);
-  p.min_blocks = 4;
+  const int sms = sm_count(dev);
   const bool f16 = a->dtype == FA_F16;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (row_tiles(a) == 1)
-    return p.D <= 64 ? launch_rows_t<64, 1>(p, f16, s) : launch_rows_t<128, 1>(p, f16, s);
-  return p.D <= 64 ? launch_rows_t<64, 2>(p, f16, s) : launch_rows_t<128, 2>(p, f16, s);
+  const Choice c = choose(a);
+  if (c.rows) {
+    p.part = static_cast<float*>(workspace);
+    p.ctas = kRowCtasPerSm * sms;
+    p.min_blocks = 4;
+    p.row_lo = 1;
+    p.row_hi = c.tiles ? kRowMax : INT_MAX;
+    if (c.row_tiles == 1)
+      rc = p.D <= 64 ? launch_rows_t<64, 1>(p, f16, s) : launch_rows_t<128, 1>(p, f16, s);
+    else
+      rc = p.D <= 64 ? launch_rows_t<64, 2>(p, f16, s) : launch_rows_t<128, 2>(p, f16, s);
+    if (rc != FA_OK) return rc;
+  }
+  if (!c.tiles) return FA_OK;
+  p.row_lo = c.rows ? kRowMax + 1 : 1;
+  p.row_hi = INT_MAX;
+  p.ctas = sms;
+  return launch_paged_tiles(a, p, static_cast<char*>(workspace) + rows_bytes(a, c, sms), s);
 }

@@ -1,0 +1,62 @@
+// What the row and tile kernels of the paged attention share.
+#pragma once
+
+#include "fa_internal.h"
+#include "paged.cuh"
+#include "sm100_ptx.cuh"
+
+namespace fa {
+
+struct PagedParams {
+  const void* q;
+  void* o;
+  const void* kc;
+  const void* vc;
+  const int32_t* table;
+  const int32_t* lens;
+  const int32_t* cu;
+  int64_t q_st, q_sh, o_st, o_sh;       // elements: token, head
+  int64_t kc_p, kc_r, kc_h;             // page, row, head
+  int64_t vc_p, vc_r, vc_h;
+  int64_t table_stride;
+  int T, B, Hkv, g, D;
+  int pages, page_shift, max_pages;
+  int causal;
+  float scale_log2;
+  int* status;
+  float* part;                          // partial results of split units
+  int ctas;                             // ranges the key blocks are cut into
+  int min_blocks;                       // least key blocks of a range
+  int row_lo, row_hi;                   // takes sequences of row_lo .. row_hi rows (q_len * g)
+};
+
+// A sequence's new tokens and keys; rows = 0 where a kernel leaves it to the other.
+struct SeqWork {
+  int begin, q_len, kv_len;
+  int64_t rows;
+};
+
+__device__ __forceinline__ SeqWork seq_work(const PagedParams& p, int b) {
+  SeqWork w;
+  const SeqRows r = seq_rows(p.cu, b, p.T);
+  w.begin = r.begin;
+  w.q_len = r.end - r.begin;
+  const int len = p.lens[b];
+  w.kv_len = held_len(len, p.page_shift, p.max_pages);
+  if (len > w.kv_len && len > 0) atomicExch(p.status, kDevBadPage);
+  w.rows = static_cast<int64_t>(w.q_len) * p.g;
+  if (w.rows < p.row_lo || w.rows > p.row_hi) w.rows = 0;
+  return w;
+}
+
+// Keys [0, limit) that token i of the sequence sees.
+__device__ __forceinline__ int seen_keys(const PagedParams& p, const SeqWork& w, int i) {
+  return p.causal ? max(0, w.kv_len - w.q_len + i + 1) : w.kv_len;
+}
+
+// The tile kernel: bytes of its workspace, and its launches (p.ctas = SMs).
+int64_t paged_tiles_bytes(const fa_paged_attn_args* a, int sms);
+int launch_paged_tiles(const fa_paged_attn_args* a, const PagedParams& p, void* workspace,
+                       cudaStream_t stream);
+
+}  // namespace fa

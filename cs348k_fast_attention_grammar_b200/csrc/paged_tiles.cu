@@ -1,0 +1,976 @@
+// The tensor-core kernel of the paged attention, for chunks of new tokens.
+//
+// A tile is 128 rows of one (sequence, key head): floor(128 / g) consecutive new
+// tokens with their g query heads, token by token (g = Hq / Hkv), so the heads
+// that share a key head share its loads and one tile serves any group.  A unit
+// is two tiles; per 128 keys the tensor core computes, in this order,
+//   O_0 += P_0(j-1) V_{j-1};  S_0 = Q_0 K_j^T;  O_1 += P_1(j-1) V_{j-1};  S_1 = Q_1 K_j^T
+// so one tile's products run while the other's softmax does.  Warp roles (384
+// threads, one CTA per SM):
+//   warps 0-3, 4-7  softmax of tile 0 and 1 (a thread = a row = a TMEM lane)
+//   warp 8          loads: Q tiles once per unit, K and V by pages into a ring
+//   warp 9          TMEM allocation and the single thread that issues tcgen05.mma
+// S_t lives in TMEM columns [128 t, 128 t + 128), P_t over its first half as 16-bit
+// pairs, O_t at 256 + D t.  The kernel is bound by the chain S -> softmax -> P of
+// each tile, about 2900 clocks per 128 keys for 2048 clocks of tensor work.
+//
+// Pages: a load box is min(page_size, 128) rows of one page, so a 128-key tile
+// takes 128 / page_size boxes whose pages come from the block table, one lane of
+// the loading warp per page.  Boxes behind the sequence's last key are not loaded;
+// rows of V behind it are zeroed in shared memory, because 0 * NaN of a slot that
+// was never written would reach the output.
+//
+// Work (decided on the device by paged_plan_kernel, from the lengths):
+//  * many units (4 per SM or more): CTAs take whole units from a counter, heads
+//    in groups whose K and V fit half the L2, longest units first;
+//  * few units: the key blocks of all units, laid end to end, are cut into one
+//    equal range per CTA.  A unit that crosses a border leaves (m, l, O) of its
+//    parts in the workspace and paged_tiles_join adds them in the order of the
+//    keys.  A unit counts one block more than it has, for its start and end.
+// Results depend on the lengths alone, never on timing.
+#include <cuda_bf16.h>
+
+#include <climits>
+
+#include "paged_attn.h"
+#include "sm100_tmem_wide.cuh"
+
+namespace fa {
+namespace {
+
+constexpr int kRows = 128;           // rows of a tile (TMEM lanes)
+constexpr int kKeys = 128;           // keys of a block
+constexpr int kThreads = 384;
+constexpr int kRegsCtrl = 56, kRegsSoftmax = 224;
+static_assert(128 * kRegsCtrl + 256 * kRegsSoftmax <= 384 * 168,
+              "the register split exceeds the launch's pool");
+constexpr int kUnitsPerSm = 4;       // from here on units are not split
+constexpr int kPlanThreads = 1024;
+constexpr int64_t kGroupBytes = 32ll << 20;   // K and V of the heads worked on at once
+
+// A unit, or the part of one that a CTA computes.
+struct Piece {
+  int b, h;
+  int tok0;              // the unit's first token within the sequence
+  int q_begin, q_len, kv_len;
+  int blk0;              // first key block
+  int nt[2];             // key blocks of each tile from there (0: it sees none of them)
+  int slot;              // where its part goes, -1: the whole unit
+  int pad[2];
+};
+static_assert(sizeof(Piece) == 48, "pieces are copied as three 16-byte words");
+
+// The plan, at the workspace's start.
+enum : int { kSplit = 0, kUnits = 1, kNext = 2, kHeader = 4 };
+struct TileParams : PagedParams {
+  int tq;                // tokens of a tile
+  int box_rows;          // rows of a load box
+  int min_cells;         // least key blocks of a CTA's range
+  int split_units;       // units from which on none is split
+  int* plan;             // header
+  int* prefix;           // [B + 1]: units (per head) of the sequences before
+  int* first;            // [ctas + 1]: first piece of each CTA
+  int2* join;            // [ctas]: first piece and number of parts of the unit to add up
+  Piece* pieces;
+};
+
+struct PlanOffsets {
+  int64_t prefix, first, join, pieces, parts, bytes;
+};
+
+__host__ __device__ constexpr int64_t up128(int64_t n) { return (n + 127) / 128 * 128; }
+
+// ---------------------------------------------------------------------------
+// Work
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ int units_of(const TileParams& p, const SeqWork& w) {
+  return w.rows == 0 ? 0 : (w.q_len + 2 * p.tq - 1) / (2 * p.tq);
+}
+// Key blocks that the tokens [tok0, tok0 + n) of the sequence see.
+__device__ __forceinline__ int blocks_of(const TileParams& p, const SeqWork& w, int tok0, int n) {
+  if (tok0 >= w.q_len) return 0;
+  const int seen = seen_keys(p, w, min(tok0 + n, w.q_len) - 1);
+  return (seen + kKeys - 1) / kKeys;
+}
+__device__ __forceinline__ Piece make_piece(const TileParams& p, const SeqWork& w, int b, int h,
+                                            int u, int blk0, int blk1, int slot) {
+  Piece x;
+  x.b = b;
+  x.h = h;
+  x.tok0 = u * 2 * p.tq;
+  x.q_begin = w.begin;
+  x.q_len = w.q_len;
+  x.kv_len = w.kv_len;
+  x.blk0 = blk0;
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+    x.nt[t] = max(0, min(blocks_of(p, w, x.tok0 + t * p.tq, p.tq), blk1) - blk0);
+  x.slot = slot;
+  x.pad[0] = x.pad[1] = 0;
+  return x;
+}
+// The sequence whose units (times heads) hold unit i.
+__device__ __forceinline__ int seq_of_unit(const int* prefix, int B, int64_t heads, int64_t i) {
+  int lo = 0, hi = B;                   // prefix[lo] * heads <= i < prefix[hi] * heads
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (prefix[mid] * heads <= i) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+// Unit i of the whole list: sequences in order, a sequence's heads in groups
+// that stay in the L2, in a group the longest units (the last tokens) first.
+__device__ __forceinline__ Piece whole_unit(const TileParams& p, int64_t i) {
+  const int b = seq_of_unit(p.prefix, p.B, p.Hkv, i);
+  const SeqWork w = seq_work(p, b);
+  const int nu = p.prefix[b + 1] - p.prefix[b];
+  const int r = static_cast<int>(i - static_cast<int64_t>(p.prefix[b]) * p.Hkv);
+  const int64_t head_bytes = static_cast<int64_t>(max(1, w.kv_len)) * p.D * 4;
+  const int fit = static_cast<int>(max(int64_t{1}, min(int64_t{p.Hkv}, kGroupBytes / head_bytes)));
+  const int groups = (p.Hkv + fit - 1) / fit;
+  const int hg = (p.Hkv + groups - 1) / groups;      // heads of a group, spread evenly
+  const int g = r / (hg * nu);
+  const int in = r - g * hg * nu;
+  const int here = min(hg, p.Hkv - g * hg);
+  const int u = nu - 1 - in / here;
+  return make_piece(p, w, b, g * hg + in % here, u, 0, INT_MAX, -1);
+}
+
+// Exclusive prefix sum over the CTA's 1024 threads; *total: the sum.
+__device__ __forceinline__ int64_t plan_scan(int64_t v, int64_t* red, int64_t* total) {
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  int64_t x = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  __syncthreads();
+  if (lane == 31) red[w] = x;
+  __syncthreads();
+  if (w == 0) {
+    int64_t y = red[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t z = __shfl_up_sync(0xffffffffu, y, o);
+      if (lane >= o) y += z;
+    }
+    red[lane] = y;
+  }
+  __syncthreads();
+  *total = red[31];
+  return (w > 0 ? red[w - 1] : 0) + x - v;
+}
+
+// One CTA.  Counts every sequence's units; where they are few, cuts their key
+// blocks into the CTAs' ranges.
+__global__ void __launch_bounds__(kPlanThreads)
+    paged_plan_kernel(const TileParams p) {
+  __shared__ int64_t red[32];
+  __shared__ int64_t cells_before[kPlanThreads + 1];    // of (sequence, unit) pairs, one head
+  __shared__ int count[kPlanThreads];
+  grid_dependents_launch();
+  const int tid = threadIdx.x;
+  int64_t pairs = 0;
+  for (int b0 = 0; b0 < p.B; b0 += kPlanThreads) {
+    const int b = b0 + tid;
+    const int n = b < p.B ? units_of(p, seq_work(p, b)) : 0;
+    int64_t sum;
+    const int64_t before = pairs + plan_scan(n, red, &sum);
+    if (b < p.B) p.prefix[b] = static_cast<int>(before);
+    pairs += sum;
+  }
+  const int64_t units = pairs * p.Hkv;
+  const bool split = units < p.split_units;             // then units <= kPlanThreads
+  if (tid == 0) {
+    p.prefix[p.B] = static_cast<int>(pairs);
+    p.plan[kSplit] = split;
+    p.plan[kUnits] = static_cast<int>(units);
+    p.plan[kNext] = 0;
+  }
+  if (!split) return;
+  __syncthreads();
+
+  // Cells: a unit's key blocks and one more.
+  int64_t cells = 0;
+  if (tid < pairs) {
+    const int b = seq_of_unit(p.prefix, p.B, 1, tid);
+    const SeqWork w = seq_work(p, b);
+    cells = 1 + blocks_of(p, w, (tid - p.prefix[b]) * 2 * p.tq, 2 * p.tq);
+  }
+  int64_t per_head;
+  const int64_t before = plan_scan(cells, red, &per_head);
+  cells_before[tid] = before;
+  if (tid == kPlanThreads - 1) cells_before[kPlanThreads] = per_head;
+  count[tid] = 0;
+  __syncthreads();
+  const int64_t per = max(static_cast<int64_t>(p.min_cells),
+                          (per_head * p.Hkv + p.ctas - 1) / p.ctas);
+
+  // Units in the order (sequence, head, unit): where each begins, the CTAs it spans.
+  int b = 0, h = 0, u = 0, c0 = 0, parts = 0;
+  int64_t at = 0, end = 0;
+  SeqWork w = {};
+  if (tid < units) {
+    b = seq_of_unit(p.prefix, p.B, p.Hkv, tid);
+    w = seq_work(p, b);
+    const int nu = p.prefix[b + 1] - p.prefix[b];
+    const int r = tid - p.prefix[b] * p.Hkv;
+    h = r / nu;
+    u = r - h * nu;
+    const int64_t s0 = cells_before[p.prefix[b]], s1 = cells_before[p.prefix[b + 1]];
+    const int64_t me = cells_before[p.prefix[b] + u], next = cells_before[p.prefix[b] + u + 1];
+    at = s0 * p.Hkv + (s1 - s0) * h + (me - s0);
+    end = at + (next - me);
+    // the first cell stands for the unit's start: its blocks begin behind it
+    c0 = static_cast<int>((end - at > 1 ? at + 1 : at) / per);
+    parts = static_cast<int>((end - 1) / per) - c0 + 1;
+  }
+  int64_t total;
+  const int at_piece = static_cast<int>(plan_scan(parts, red, &total));
+  if (tid < p.ctas) p.join[tid] = make_int2(0, 0);
+  __syncthreads();
+  for (int i = 0; i < parts; ++i) {
+    const int64_t lo = max(at + 1, (c0 + i) * per), hi = min(end, (c0 + i + 1) * per);
+    const int blk0 = static_cast<int>(min(lo, hi) - at - 1), blk1 = static_cast<int>(hi - at - 1);
+    const int slot = parts == 1 ? -1 : 2 * (c0 + i) + (i == 0 ? 1 : 0);
+    p.pieces[at_piece + i] = make_piece(p, w, b, h, u, max(0, blk0), max(0, blk1), slot);
+    atomicAdd(&count[c0 + i], 1);
+  }
+  if (parts > 1) p.join[c0] = make_int2(at_piece, parts);
+  __syncthreads();
+  const int64_t first = plan_scan(tid < p.ctas ? count[tid] : 0, red, &total);
+  if (tid <= p.ctas) p.first[tid] = static_cast<int>(first);
+}
+
+// ---------------------------------------------------------------------------
+// Exponentials: a quarter of them on the FMA pipe
+// ---------------------------------------------------------------------------
+// 2^x for two values: x = j + f with j the nearest whole number (the addition of
+// 1.5 * 2^23 leaves it in the low mantissa bits), 2^f by the degree-3 minimax
+// polynomial of fit_exp2_poly.py (relative error 7.5e-5), j added to the exponent.
+// x is held at -125, so a masked score gives 2^-125 instead of 0.
+__device__ __forceinline__ void exp2_pair(float x0, float x1, float& r0, float& r1) {
+  const uint64_t x = f2_pack(fmaxf(x0, -125.f), fmaxf(x1, -125.f));
+  const uint64_t t = fadd2(x, f2_pack(12582912.f, 12582912.f));
+  const uint64_t j = fadd2(t, f2_pack(-12582912.f, -12582912.f));
+  const uint64_t f = ffma2(j, f2_pack(-1.f, -1.f), x);
+  uint64_t q = ffma2(f2_pack(0.0551716685295105f, 0.0551716685295105f), f,
+                     f2_pack(0.2426111251115799f, 0.2426111251115799f));
+  q = ffma2(q, f, f2_pack(0.6932609677314758f, 0.6932609677314758f));
+  q = ffma2(q, f, f2_pack(0.9999280571937561f, 0.9999280571937561f));
+  float p0, p1, t0, t1;
+  f2_unpack(q, p0, p1);
+  f2_unpack(t, t0, t1);
+  r0 = __int_as_float(__float_as_int(p0) + (__float_as_int(t0) << 23));
+  r1 = __int_as_float(__float_as_int(p1) + (__float_as_int(t1) << 23));
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// ---------------------------------------------------------------------------
+// The kernel
+// ---------------------------------------------------------------------------
+template <int D>
+struct Cfg {
+  static constexpr int kTileBytes = kRows * D * 2;
+  static constexpr int kStages = D == 128 ? 4 : 8;       // K and V tiles in the ring
+  static constexpr int kQOff = 0;
+  static constexpr int kKVOff = 2 * kTileBytes;
+  static constexpr int kBarOff = kKVOff + kStages * kTileBytes;
+  // q, kv_full[], kv_empty[], s_full[2], p_full[2], o_full[2], drain, p_half[2],
+  // q_empty, unit_full[2], unit_empty[2], v_raw
+  static constexpr int kNumBars = 1 + 2 * kStages + 15;
+  static constexpr int kPieceOff = kBarOff + (kNumBars * 8 + 15) / 16 * 16;
+  static constexpr int kMiscOff = kPieceOff + 2 * sizeof(Piece);
+  static constexpr int kSmemBytes = kMiscOff + 16 + 1024;   // + alignment slack
+  static constexpr int kSlot = 2 * kRows * (D + 2);         // floats of a unit's part
+  __device__ static constexpr uint32_t col_s(int t) { return 128u * t; }
+  __device__ static constexpr uint32_t col_o(int t) { return 256u + D * t; }
+};
+
+// A wait on the way out: ends with the phase or after a short limit.
+__device__ __forceinline__ void last_wait(uint32_t bar, uint32_t parity) {
+  const unsigned long long t0 = globaltimer_ns();
+  while (!mbar_try_wait(bar, parity))
+    if (globaltimer_ns() - t0 > 50ull * 1000ull * 1000ull) return;
+}
+
+template <int D, bool F16>
+__global__ void __launch_bounds__(kThreads, 1)
+    paged_tiles_kernel(const __grid_constant__ CUtensorMap tmQ,
+                       const __grid_constant__ CUtensorMap tmK,
+                       const __grid_constant__ CUtensorMap tmV, const TileParams p) {
+  using C = Cfg<D>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  uint8_t* gbase = smem_raw + (base - raw);
+  const uint32_t sQ = base + C::kQOff;
+  const uint32_t sKV = base + C::kKVOff;
+  const uint32_t bars = base + C::kBarOff;
+  constexpr int kB0 = 1 + 2 * C::kStages;
+  const uint32_t bar_q = bars;
+  auto bar_kv_full = [&](int s) { return bars + 8u * (1 + s); };
+  auto bar_kv_empty = [&](int s) { return bars + 8u * (1 + C::kStages + s); };
+  auto bar_s_full = [&](int t) { return bars + 8u * (kB0 + t); };
+  auto bar_p_full = [&](int t) { return bars + 8u * (kB0 + 2 + t); };
+  auto bar_o_full = [&](int t) { return bars + 8u * (kB0 + 4 + t); };
+  const uint32_t bar_drain = bars + 8u * (kB0 + 6);
+  auto bar_p_half = [&](int t) { return bars + 8u * (kB0 + 7 + t); };   // keys 0-63 of P_t
+  const uint32_t bar_q_empty = bars + 8u * (kB0 + 9);   // the unit's last S products are done
+  auto bar_unit_full = [&](int s) { return bars + 8u * (kB0 + 10 + s); };
+  auto bar_unit_empty = [&](int s) { return bars + 8u * (kB0 + 12 + s); };
+  const uint32_t bar_v_raw = bars + 8u * (kB0 + 14);    // a V tile whose end is to be zeroed
+  // Ring of two pieces; h = -1 ends the CTA's work.
+  volatile Piece* ring = reinterpret_cast<volatile Piece*>(gbase + C::kPieceOff);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gbase + C::kMiscOff);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(gbase + C::kMiscOff + 4);
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+
+  grid_dependents_launch();
+  if (threadIdx.x == 0) {
+    mbar_init(bar_q, 1);
+    for (int s = 0; s < C::kStages; ++s) {
+      mbar_init(bar_kv_full(s), 1);
+      mbar_init(bar_kv_empty(s), 1);
+    }
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(bar_s_full(t), 1);
+      mbar_init(bar_p_full(t), kRows);
+      mbar_init(bar_p_half(t), kRows);
+      mbar_init(bar_o_full(t), 1);
+      mbar_init(bar_unit_full(t), 1);
+      mbar_init(bar_unit_empty(t), 1 + 8);
+    }
+    mbar_init(bar_drain, 1);
+    mbar_init(bar_q_empty, 1);
+    mbar_init(bar_v_raw, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 9) {
+    tmem_alloc(smem_u32(tmem_slot), 512);
+    tmem_relinquish();
+  }
+  if (warp == 8 && lane == 0) {
+    tma_prefetch_desc(&tmQ);
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
+  }
+  // Rows of the Q tiles that no load writes (128 - g * floor(128 / g)) stay zero.
+  for (int i = threadIdx.x; i < 2 * C::kTileBytes / 16; i += kThreads)
+    *reinterpret_cast<uint4*>(gbase + C::kQOff + i * 16) = make_uint4(0, 0, 0, 0);
+  fence_proxy_async_smem();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  grid_dependency_wait();               // the plan is complete
+
+  // Warp-uniform bounded wait: every lane waits, and the warp goes on only if
+  // all saw the phase, so that giving up never splits a warp.
+  auto wwait = [&](uint32_t bar, uint32_t parity) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, p.status));
+  };
+
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsCtrl) : "memory");
+    if (warp == 8) {
+      // =================== loads ===================
+      const uint64_t pol_q = l2_policy_evict_first();
+      const uint64_t pol_kv = l2_policy_evict_last();
+      const bool split = p.plan[kSplit] != 0;
+      int64_t next = split ? p.first[blockIdx.x] : static_cast<int>(blockIdx.x);
+      const int64_t stop = split ? p.first[blockIdx.x + 1] : p.plan[kUnits];
+      const int boxes = kKeys / p.box_rows;
+      const int page_mask = (1 << p.page_shift) - 1;
+      const uint32_t box_bytes = static_cast<uint32_t>(p.box_rows) * 128u;
+      int issued = 0;       // K and V tiles, over all pieces (ring position)
+      int uc = 0;           // pieces with keys
+      int raws = 0;         // V tiles whose end was zeroed
+      for (int take = 0;; ++take) {
+        const int us = take & 1;
+        if (take >= 2 && !wwait(bar_unit_empty(us), ((take >> 1) - 1) & 1)) break;
+        Piece x;
+        if (next < stop) x = split ? p.pieces[next] : whole_unit(p, next);
+        else x.h = -1;
+        if (lane == 0) {
+          volatile Piece* d = ring + us;
+          d->b = x.b;
+          d->h = x.h;
+          d->tok0 = x.tok0;
+          d->q_begin = x.q_begin;
+          d->q_len = x.q_len;
+          d->kv_len = x.kv_len;
+          d->blk0 = x.blk0;
+          d->nt[0] = x.nt[0];
+          d->nt[1] = x.nt[1];
+          d->slot = x.slot;
+          mbar_arrive(bar_unit_full(us));
+        }
+        if (x.h < 0) break;
+        const int n = max(x.nt[0], x.nt[1]);
+        if (n > 0) {
+          // The Q tiles are free once the last piece's S products are done.
+          if (uc > 0 && !wwait(bar_q_empty, (uc - 1) & 1)) break;
+          if (lane == 0) {
+            const uint32_t bytes = static_cast<uint32_t>(p.tq) * p.g * 128u * (D / 64);
+            mbar_arrive_expect_tx(bar_q, bytes * ((x.nt[0] > 0 ? 1 : 0) + (x.nt[1] > 0 ? 1 : 0)));
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+              if (x.nt[t] > 0)
+#pragma unroll
+                for (int dk = 0; dk < D / 64; ++dk)
+                  tma_load_4d(sQ + t * C::kTileBytes + dk * 16384, &tmQ, bar_q, dk * 64, 0,
+                              x.q_begin + x.tok0 + t * p.tq, x.h, pol_q);
+          }
+          ++uc;
+          const int32_t* trow = p.table + x.b * p.table_stride;
+          // Page of this lane's box of block j; one outside the cache reads as zeros.
+          auto page_for = [&](int j) {
+            const int key = j * kKeys + lane * p.box_rows;
+            if (lane >= boxes || key >= x.kv_len) return p.pages;
+            const int pg = page_at(trow, key, p.page_shift, p.max_pages, p.pages);
+            if (pg < 0) atomicExch(p.status, kDevBadPage);
+            return pg < 0 ? p.pages : pg;
+          };
+          int page = page_for(x.blk0);
+          bool ok = true;
+          for (int j = x.blk0; ok && j < x.blk0 + n; ++j) {
+            const int page_next = j + 1 < x.blk0 + n ? page_for(j + 1) : 0;
+            const int keys = min(kKeys, x.kv_len - j * kKeys);          // > 0
+            const int used = (keys + p.box_rows - 1) / p.box_rows;
+            const int in = (j * kKeys) & page_mask & ~(p.box_rows - 1);
+#pragma unroll
+            for (int kv = 0; kv < 2; ++kv) {
+              const int s = issued % C::kStages;
+              if (!wwait(bar_kv_empty(s), ((issued / C::kStages) & 1) ^ 1u)) {
+                ok = false;
+                break;
+              }
+              const uint32_t dst = sKV + s * C::kTileBytes;
+              // A V tile that ends inside is handed on after its end is zeroed.
+              const bool cut = kv == 1 && keys < kKeys;
+              const uint32_t bar = cut ? bar_v_raw : bar_kv_full(s);
+              if (lane == 0) mbar_arrive_expect_tx(bar, used * box_bytes * (D / 64));
+              __syncwarp();
+              if (lane < used) {
+                const void* map = kv ? static_cast<const void*>(&tmV)
+                                     : static_cast<const void*>(&tmK);
+#pragma unroll
+                for (int dk = 0; dk < D / 64; ++dk)
+                  tma_load_4d(dst + dk * 16384 + lane * box_bytes, map, bar, dk * 64, in, x.h,
+                              page, pol_kv);
+              }
+              ++issued;
+              if (cut) {
+                if (!wwait(bar_v_raw, raws & 1)) {
+                  ok = false;
+                  break;
+                }
+                ++raws;
+                uint8_t* v = gbase + C::kKVOff + s * C::kTileBytes;
+                for (int i = keys * 8 + lane; i < kKeys * 8; i += 32)
+#pragma unroll
+                  for (int dk = 0; dk < D / 64; ++dk)
+                    *reinterpret_cast<uint4*>(v + dk * 16384 + i * 16) = make_uint4(0, 0, 0, 0);
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar_kv_full(s));
+              }
+            }
+            page = page_next;
+          }
+          if (!ok) break;
+        }
+        if (split) {
+          ++next;
+        } else {
+          int got = 0;
+          if (lane == 0) got = atomicAdd(p.plan + kNext, 1);
+          next = static_cast<int64_t>(gridDim.x) + __shfl_sync(0xffffffffu, got, 0);
+        }
+      }
+      if (*abort_flag && lane == 0) {
+        // Let the copies in flight land before the CTA exits.
+        if (uc > 0) last_wait(bar_q, (uc - 1) & 1);
+        last_wait(bar_v_raw, raws & 1);
+        for (int i = max(0, issued - C::kStages); i < issued; ++i)
+          last_wait(bar_kv_full(i % C::kStages), (i / C::kStages) & 1);
+      }
+      __syncwarp();
+    } else if (warp == 9) {
+      // =================== MMA issuer ===================
+      if (elect_one()) {
+        constexpr uint32_t kIdQK = idesc_f32acc(kRows, kKeys, false, false, F16);
+        constexpr uint32_t kIdPV = idesc_f32acc(kRows, D, false, true, F16);
+        bool ok = true;
+        int it = 0;              // K and V tiles taken, over all pieces
+        int uq = 0;              // pieces with keys
+        int pb[2] = {0, 0};      // key blocks of tile t in earlier pieces (P phases)
+        for (int uc = 0; ok; ++uc) {
+          const int us = uc & 1;
+          if (!mbar_wait(bar_unit_full(us), (uc >> 1) & 1, abort_flag, p.status)) break;
+          const int h = ring[us].h;
+          const int nt[2] = {ring[us].nt[0], ring[us].nt[1]};
+          mbar_arrive(bar_unit_empty(us));
+          if (h < 0) break;
+          const int n = max(nt[0], nt[1]);
+          if (n == 0) continue;
+          if (!mbar_wait(bar_q, uq & 1, abort_flag, p.status)) break;
+          ++uq;
+          tc_fence_after();
+          int vslot = 0;
+          for (int j = 0; ok && j <= n; ++j) {
+            int kslot = 0;
+            if (j < n) {
+              kslot = it % C::kStages;
+              if (!mbar_wait(bar_kv_full(kslot), (it / C::kStages) & 1, abort_flag, p.status)) {
+                ok = false;
+                break;
+              }
+              ++it;
+              tc_fence_after();
+            }
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+              if (j >= 1 && j - 1 < nt[t]) {
+                // O_t += P_t(j-1) V_{j-1}: P from TMEM, V with D contiguous; the
+                // first 64 keys go as soon as their half of P is stored.
+                const uint32_t vbase = sKV + vslot * C::kTileBytes;
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                  const uint32_t bar = half == 0 ? bar_p_half(t) : bar_p_full(t);
+                  if (!mbar_wait(bar, (pb[t] + j - 1) & 1, abort_flag, p.status)) {
+                    ok = false;
+                    break;
+                  }
+                  tc_fence_after();
+#pragma unroll
+                  for (int kk = half * 4; kk < half * 4 + 4; ++kk)
+                    mma_ts(tmem + C::col_o(t), tmem + C::col_s(t) + kk * 8,
+                           sdesc_sw128(vbase + kk * 2048, 16384, 1024), kIdPV,
+                           (j - 1 > 0 || kk > 0) ? 1u : 0u);
+                }
+                if (!ok) break;
+                if (j - 1 == nt[t] - 1) mma_commit(bar_o_full(t));
+              }
+              if (j < nt[t]) {
+                // S_t = Q_t K_j^T, both with D contiguous.
+                const uint32_t qbase = sQ + t * C::kTileBytes;
+                const uint32_t kbase = sKV + kslot * C::kTileBytes;
+#pragma unroll
+                for (int kk = 0; kk < D / 16; ++kk) {
+                  const uint32_t off = (kk >> 2) * 16384 + (kk & 3) * 32;
+                  mma_ss(tmem + C::col_s(t), sdesc_sw128(qbase + off, 16, 1024),
+                         sdesc_sw128(kbase + off, 16, 1024), kIdQK, kk > 0 ? 1u : 0u);
+                }
+                mma_commit(bar_s_full(t));
+              }
+            }
+            if (!ok) break;
+            if (j >= 1) mma_commit(bar_kv_empty(vslot));
+            if (j < n) {
+              mma_commit(bar_kv_empty(kslot));
+              if (j == n - 1) mma_commit(bar_q_empty);
+              vslot = it % C::kStages;
+              if (!mbar_wait(bar_kv_full(vslot), (it / C::kStages) & 1, abort_flag, p.status)) {
+                ok = false;
+                break;
+              }
+              ++it;
+              tc_fence_after();
+            }
+          }
+          pb[0] += nt[0];
+          pb[1] += nt[1];
+        }
+        // Every issued MMA and its arrivals complete before teardown.
+        mma_commit(bar_drain);
+        last_wait(bar_drain, 0);
+      }
+      __syncwarp();
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax) : "memory");
+    // =================== softmax, rescaling, output ===================
+    const int t = warp >> 2;
+    const int wq = warp & 3;
+    const int row = wq * 32 + lane;
+    const uint32_t lane_off = static_cast<uint32_t>(wq * 32) << 16;
+    const uint32_t tS = tmem + lane_off + C::col_s(t);
+    const uint32_t tO = tmem + lane_off + C::col_o(t);
+    const float sl2 = p.scale_log2;
+    const uint64_t sl2x2 = f2_pack(sl2, sl2);
+    const int row_tok = row / p.g, row_head = row - row_tok * p.g;
+    bool ok = true;
+    int sb = 0;   // key blocks of this tile in earlier pieces (S phases)
+    int ou = 0;   // earlier pieces in which this tile had keys (O phases)
+    for (int uc = 0; ok; ++uc) {
+      const int us = uc & 1;
+      if (!wwait(bar_unit_full(us), (uc >> 1) & 1)) break;
+      const int h = ring[us].h, q_begin = ring[us].q_begin, q_len = ring[us].q_len;
+      const int kv_len = ring[us].kv_len, blk0 = ring[us].blk0, slot = ring[us].slot;
+      const int tok_t = ring[us].tok0 + t * p.tq, nt = ring[us].nt[t];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar_unit_empty(us));
+      if (h < 0) break;
+      const int tok = tok_t + row_tok;
+      const bool live = row_tok < p.tq && tok < q_len;
+      // Keys [0, lim) are seen by this row; no row of the tile sees fewer than lim0.
+      const int lim0 = p.causal ? kv_len - q_len + tok_t + 1 : kv_len;
+      const int lim = p.causal && live ? lim0 + row_tok : kv_len;
+      float m_ref = -INFINITY;   // reference maximum (scaled, log2 domain)
+      float l = 0.f;             // sum of exp2(s * sl2 - m_ref)
+      for (int j = 0; j < nt; ++j) {
+        if (!wwait(bar_s_full(t), (sb + j) & 1)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        uint32_t sr[128];
+        tmem_ld128_wait(tS, sr);
+        const int k0 = (blk0 + j) * kKeys;
+        if (k0 + kKeys > lim0 || k0 + kKeys > kv_len) {
+#pragma unroll
+          for (int c = 0; c < kKeys; ++c)
+            if (k0 + c >= lim) sr[c] = __float_as_uint(-INFINITY);
+        }
+        float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int c = 0; c < kKeys; c += 8)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            mx4[i] = max3(mx4[i], __uint_as_float(sr[c + 2 * i]), __uint_as_float(sr[c + 2 * i + 1]));
+        const float m_blk = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * sl2;
+        // The reference is raised only when a row outgrows it by 2^8, so that
+        // O is rarely rescaled; O / l is exact for any reference.
+        const bool need = m_ref == -INFINITY ? m_blk > -INFINITY : m_blk - m_ref > 8.f;
+        if (__any_sync(0xffffffffu, need)) {
+          const float m_use = need ? m_blk : m_ref;
+          const float alpha = m_use == -INFINITY   ? 1.f
+                              : m_ref == -INFINITY ? 0.f
+                                                   : ex2_approx(m_ref - m_use);
+          if (j > 0) {
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) {
+              uint32_t o[32];
+              tmem_ld32_wait(tO + c * 32, o);
+#pragma unroll
+              for (int e = 0; e < 32; ++e)
+                o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+              tmem_st32(tO + c * 32, o);
+            }
+          }
+          l *= alpha;
+          m_ref = m_use;
+        }
+        const float neg_m = m_ref == -INFINITY ? 0.f : -m_ref;
+        const uint64_t negm2 = f2_pack(neg_m, neg_m);
+        uint64_t rs2[2] = {0ull, 0ull};
+        uint32_t pk[2][32];
+        auto exp_half = [&](int half) {
+#pragma unroll
+          for (int cc = 0; cc < 32; ++cc) {
+            const int c = half * 32 + cc;
+            float x0, x1, p0, p1;
+            f2_unpack(ffma2(f2_pack(__uint_as_float(sr[2 * c]), __uint_as_float(sr[2 * c + 1])),
+                            sl2x2, negm2),
+                      x0, x1);
+            if (c % 4 == 3) {
+              exp2_pair(x0, x1, p0, p1);
+            } else {
+              p0 = ex2_approx(x0);
+              p1 = ex2_approx(x1);
+            }
+            rs2[c & 1] = fadd2(rs2[c & 1], f2_pack(p0, p1));
+            pk[half][cc] = pack_16x2<F16>(p0, p1);
+          }
+        };
+        exp_half(0);
+        tmem_st32(tS, pk[0]);
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(bar_p_half(t));
+        exp_half(1);
+        float a0, a1, b0, b1;
+        f2_unpack(rs2[0], a0, a1);
+        f2_unpack(rs2[1], b0, b1);
+        l += (a0 + a1) + (b0 + b1);
+        tmem_st32(tS + 32, pk[1]);
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(bar_p_full(t));
+      }
+      if (!ok) break;
+      if (nt > 0) {
+        if (!wwait(bar_o_full(t), ou & 1)) break;
+        tc_fence_after();
+        ++ou;
+      }
+      // A row that saw no key holds 2^-125 of it per masked exponential: zero.
+      // (l is NaN where the scores were, and stays so.)
+      if (m_ref == -INFINITY && l == l) l = 0.f;
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      if (slot < 0) {
+        uint16_t* dst = static_cast<uint16_t*>(p.o) + static_cast<int64_t>(q_begin + tok) * p.o_st +
+                        static_cast<int64_t>(h * p.g + row_head) * p.o_sh;
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t o[32];
+          if (nt > 0) {
+            tmem_ld32_wait(tO + c * 32, o);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = 0u;
+          }
+          if (live) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              if (c * 32 + e * 8 >= p.D) continue;
+              uint32_t w[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                w[i] = pack_16x2<F16>(__uint_as_float(o[e * 8 + 2 * i]) * inv,
+                                      __uint_as_float(o[e * 8 + 2 * i + 1]) * inv);
+              *reinterpret_cast<uint4*>(dst + c * 32 + e * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          }
+        }
+      } else {
+        float* part = p.part + static_cast<int64_t>(slot) * C::kSlot;
+        const int r = t * kRows + row;
+        if (nt > 0) {
+#pragma unroll
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t o[32];
+            tmem_ld32_wait(tO + c * 32, o);
+            if (live) {
+              uint4* dst = reinterpret_cast<uint4*>(part + r * D + c * 32);
+#pragma unroll
+              for (int e = 0; e < 8; ++e)
+                dst[e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+            }
+          }
+        }
+        if (live) {
+          part[2 * kRows * D + r] = m_ref;
+          part[2 * kRows * D + 2 * kRows + r] = l;
+        }
+      }
+      sb += nt;
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// Adds up the parts of the unit that begins in CTA blockIdx.x's range and goes
+// on behind it; one warp per row.  Bound by HBM: each part is read once.
+constexpr int kJoinWarps = 8;
+template <int D, bool F16>
+__global__ void __launch_bounds__(32 * kJoinWarps)
+    paged_tiles_join(const TileParams p) {
+  using C = Cfg<D>;
+  grid_dependency_wait();
+  if (p.plan[kSplit] == 0) return;
+  const int2 jn = p.join[blockIdx.x];
+  if (jn.y == 0) return;
+  const int lane = threadIdx.x & 31;
+  const int r = blockIdx.y * kJoinWarps + (threadIdx.x >> 5);
+  const Piece& x = p.pieces[jn.x];
+  const int t = r / kRows, row_tok = (r - t * kRows) / p.g;
+  const int head = r - t * kRows - row_tok * p.g;
+  const int tok = x.tok0 + t * p.tq + row_tok;
+  if (row_tok >= p.tq || tok >= x.q_len) return;
+  auto part = [&](int i) {
+    return p.part + static_cast<int64_t>(2 * (blockIdx.x + i) + (i == 0 ? 1 : 0)) * C::kSlot;
+  };
+  float top = -INFINITY;
+  for (int i = lane; i < jn.y; i += 32) top = fmaxf(top, part(i)[2 * kRows * D + r]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  constexpr int E = D / 32;
+  float sum = 0.f, acc[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) acc[e] = 0.f;
+#pragma unroll 4
+  for (int i = 0; i < jn.y; ++i) {
+    const float* s = part(i);
+    const float mi = s[2 * kRows * D + r], li = s[2 * kRows * D + 2 * kRows + r];
+    if (mi == -INFINITY) {              // saw none of these keys: O was not written
+      sum += li;
+      continue;
+    }
+    const float al = ex2_approx(mi - top);
+    sum += li * al;
+    if constexpr (E == 4) {
+      const float4 v = *reinterpret_cast<const float4*>(s + r * D + lane * 4);
+      acc[0] += v.x * al;
+      acc[1] += v.y * al;
+      acc[2] += v.z * al;
+      acc[3] += v.w * al;
+    } else {
+      const float2 v = *reinterpret_cast<const float2*>(s + r * D + lane * 2);
+      acc[0] += v.x * al;
+      acc[1] += v.y * al;
+    }
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  uint16_t* dst = static_cast<uint16_t*>(p.o) +
+                  static_cast<int64_t>(x.q_begin + tok) * p.o_st +
+                  static_cast<int64_t>(x.h * p.g + head) * p.o_sh;
+  if (lane * E < p.D) {
+    if constexpr (E == 4)
+      *reinterpret_cast<uint2*>(dst + lane * 4) =
+          make_uint2(pack_16x2<F16>(acc[0] * inv, acc[1] * inv),
+                     pack_16x2<F16>(acc[2] * inv, acc[3] * inv));
+    else
+      *reinterpret_cast<uint32_t*>(dst + lane * 2) = pack_16x2<F16>(acc[0] * inv, acc[1] * inv);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+int tile_tokens(const fa_paged_attn_args* a) {
+  return static_cast<int>(kRows / (a->Hq / a->Hkv));
+}
+
+// Whether the device may find few enough units to split some: rows outside
+// every sequence and short sequences make units fewer than T gives, so only a
+// T of twice the limit rules it out.
+bool may_split(const fa_paged_attn_args* a, int sms) {
+  const int64_t least = a->T / (2 * tile_tokens(a)) * a->Hkv;
+  return least < 2ll * kUnitsPerSm * sms;
+}
+
+PlanOffsets plan_offsets(const fa_paged_attn_args* a, int sms) {
+  PlanOffsets o;
+  o.prefix = up128(kHeader * 4);
+  o.first = o.prefix + up128((a->B + 1) * 4);
+  o.join = o.first + up128((sms + 1) * 4);
+  o.pieces = o.join + up128(sms * 8);
+  const bool split = may_split(a, sms);
+  const int64_t most = split ? kUnitsPerSm * sms + sms : 0;
+  o.parts = o.pieces + up128(most * static_cast<int64_t>(sizeof(Piece)));
+  const int d = a->D <= 64 ? 64 : 128;
+  o.bytes = o.parts + (split ? 2ll * sms * 2 * kRows * (d + 2) * 4 : 0);
+  return o;
+}
+
+// 4-D tensor map of 16-bit elements, innermost dimension first, boxes of 64
+// channels (128-byte swizzle).  A dimension of one entry gets a legal stride.
+int make_map(CUtensorMap* map, const void* ptr, const int64_t (&dims)[4],
+             const int64_t (&strides)[3], const uint32_t (&box)[3], bool f16) {
+  EncodeTiledFn enc = encode_tiled_fn();
+  if (enc == nullptr) return FA_ERR_DRIVER;
+  cuuint64_t d[4], s[3];
+  cuuint32_t b[4] = {64, box[0], box[1], box[2]}, one[4] = {1, 1, 1, 1};
+  for (int i = 0; i < 4; ++i) d[i] = static_cast<cuuint64_t>(dims[i]);
+  for (int i = 0; i < 3; ++i) s[i] = dims[i + 1] > 1 ? static_cast<cuuint64_t>(strides[i]) * 2 : 256;
+  const CUresult r =
+      enc(map, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
+          const_cast<void*>(ptr), d, s, b, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? FA_OK : FA_ERR_TMA;
+}
+
+template <typename... Args>
+int launch_after(void (*kern)(Args...), dim3 grid, int threads, int smem, cudaStream_t stream,
+                 const Args&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, args...) == cudaSuccess ? FA_OK : FA_ERR_LAUNCH;
+}
+
+template <int D, bool F16>
+int launch_tiles(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
+                 const TileParams& p, bool split, cudaStream_t stream) {
+  using C = Cfg<D>;
+  static KernelPrep prep;
+  int dev = 0;
+  int rc = prepare_kernel(prep, reinterpret_cast<const void*>(paged_tiles_kernel<D, F16>),
+                          C::kSmemBytes, &dev);
+  if (rc != FA_OK) return rc;
+  paged_plan_kernel<<<1, kPlanThreads, 0, stream>>>(p);
+  if (cudaGetLastError() != cudaSuccess) return FA_ERR_LAUNCH;
+  rc = launch_after(paged_tiles_kernel<D, F16>, dim3(p.ctas), kThreads, C::kSmemBytes, stream, mq,
+                    mk, mv, p);
+  if (rc != FA_OK || !split) return rc;
+  return launch_after(paged_tiles_join<D, F16>, dim3(p.ctas, 2 * kRows / kJoinWarps),
+                      32 * kJoinWarps, 0, stream, p);
+}
+
+}  // namespace
+
+int64_t paged_tiles_bytes(const fa_paged_attn_args* a, int sms) {
+  return plan_offsets(a, sms).bytes;
+}
+
+int launch_paged_tiles(const fa_paged_attn_args* a, const PagedParams& q, void* workspace,
+                       cudaStream_t stream) {
+  TileParams p;
+  static_cast<PagedParams&>(p) = q;
+  p.tq = tile_tokens(a);
+  p.box_rows = a->page_size < kKeys ? static_cast<int>(a->page_size) : kKeys;
+  // (the exponent's scale is kept off zero: -inf * 0 of a masked score is no number)
+  if (p.scale_log2 < 1e-30f) p.scale_log2 = 1e-30f;
+  const bool split = may_split(a, p.ctas);
+  const PlanOffsets o = plan_offsets(a, p.ctas);
+  char* ws = static_cast<char*>(workspace);
+  p.plan = reinterpret_cast<int*>(ws);
+  p.prefix = reinterpret_cast<int*>(ws + o.prefix);
+  p.first = reinterpret_cast<int*>(ws + o.first);
+  p.join = reinterpret_cast<int2*>(ws + o.join);
+  p.pieces = reinterpret_cast<Piece*>(ws + o.pieces);
+  p.part = reinterpret_cast<float*>(ws + o.parts);
+  p.min_cells = 4;
+  p.split_units = split ? kUnitsPerSm * p.ctas : 0;
+  if (p.split_units > kPlanThreads) p.split_units = kPlanThreads;
+  CUtensorMap mq, mk, mv;
+  const bool f16 = a->dtype == FA_F16;
+  const int64_t g = a->Hq / a->Hkv;
+  int rc = make_map(&mq, a->q, {a->D, g, a->T, a->Hkv},
+                    {a->q_strides[1], a->q_strides[0], a->q_strides[1] * g},
+                    {static_cast<uint32_t>(g), static_cast<uint32_t>(p.tq), 1}, f16);
+  if (rc != FA_OK) return rc;
+  const uint32_t rows = static_cast<uint32_t>(p.box_rows);
+  const int64_t dims[4] = {a->D, a->page_size, a->Hkv, a->pages};
+  rc = make_map(&mk, a->k_cache, dims,
+                {a->k_cache_strides[1], a->k_cache_strides[2], a->k_cache_strides[0]},
+                {rows, 1, 1}, f16);
+  if (rc != FA_OK) return rc;
+  rc = make_map(&mv, a->v_cache, dims,
+                {a->v_cache_strides[1], a->v_cache_strides[2], a->v_cache_strides[0]},
+                {rows, 1, 1}, f16);
+  if (rc != FA_OK) return rc;
+  if (a->D <= 64)
+    return f16 ? launch_tiles<64, true>(mq, mk, mv, p, split, stream)
+               : launch_tiles<64, false>(mq, mk, mv, p, split, stream);
+  return f16 ? launch_tiles<128, true>(mq, mk, mv, p, split, stream)
+             : launch_tiles<128, false>(mq, mk, mv, p, split, stream);
+}
+
+}  // namespace fa

@@ -322,7 +322,7 @@ typedef struct fa_paged_attn_args {
   int64_t dtype;               /* FA_BF16 or FA_F16, all tensors alike          */
   int64_t T, B, Hq, Hkv, D;    /* D 8 .. 128, a multiple of 8; Hq / Hkv <= 128  */
   int64_t pages, page_size;    /* page_size a power of two, 16 .. 1024          */
-  int64_t max_pages, table_stride;
+  int64_t max_pages, table_stride; /* max_pages * page_size < 2^31 - 4096       */
   int64_t q_strides[2], o_strides[2];                                 /* token, head */
   int64_t k_cache_strides[3], v_cache_strides[3];                     /* page, row, head */
   int64_t max_q_len;

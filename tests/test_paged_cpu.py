@@ -171,9 +171,9 @@ def test_attention_status_codes():
     lib, code = _lib.load(), _codes()
 
     def call(ptrs=(P,) * 7, dtype=0, T=3, B=3, Hq=4, Hkv=2, D=64, pages=4, page=16, width=2, ts=2,
-             st=(256, 64, 256, 64), cs=(2048, 128, 64) * 2, longest=1):
+             st=(256, 64, 256, 64), cs=(2048, 128, 64) * 2, longest=1, scale=0.125):
         args = paged._ATTN.pack(*ptrs, dtype, T, B, Hq, Hkv, D, pages, page, width, ts, *st, *cs,
-                                longest, 1, 0.125)
+                                longest, 1, scale)
         rc = lib.fa_paged_attn(args, P, 1 << 40, None)
         assert lib.fa_paged_attn_workspace(args) == -rc
         return rc
@@ -181,10 +181,11 @@ def test_attention_status_codes():
     assert lib.fa_paged_attn(None, None, 0, None) == code["FA_ERR_NULL"]
     for i in range(6):
         assert call(ptrs=tuple(0 if j == i else P for j in range(7))) == code["FA_ERR_NULL"]
-    assert call(dtype=2) == code["FA_ERR_ARG"]
+    for change in (dict(dtype=2), dict(scale=float("inf")), dict(scale=float("nan"))):
+        assert call(**change) == code["FA_ERR_ARG"]
     for change in (dict(T=0), dict(B=0), dict(Hq=5), dict(Hkv=0), dict(Hq=258), dict(pages=0),
                    dict(width=0), dict(page=8), dict(page=24), dict(page=2048), dict(longest=0),
-                   dict(T=1 << 31), dict(ptrs=(P,) * 6 + (0,), T=4)):
+                   dict(T=1 << 31), dict(width=1 << 27, ts=1 << 27), dict(ptrs=(P,) * 6 + (0,), T=4)):
         assert call(**change) == code["FA_ERR_SHAPE"]
     for D in (0, 4, 60, 136):
         assert call(D=D) == code["FA_ERR_HEAD_DIM"]

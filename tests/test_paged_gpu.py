@@ -94,6 +94,13 @@ def test_chunk_over_long_cache():
     _check([300, 17], [3000, 8191], 8, 1, 128, 16, F16, causal=False)
 
 
+@pytest.mark.parametrize("causal", [True, False])
+def test_units_that_fill_the_device(causal):
+    """640 and more units of 256 rows: none is split."""
+    _check([300, 40, 520, 0, 1, 290], [300, 200, 520, 7, 90, 811], 64, 64, 64, 16, causal=causal)
+    _check([300, 1100], [300, 1300], 128, 64, 128, 64, F16, causal=causal)
+
+
 def test_rows_that_see_nothing():
     """kv_lens below the number of new tokens (0 among them): the tokens before the start see
     no key under the causal mask and get zeros."""
