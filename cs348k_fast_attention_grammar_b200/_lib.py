@@ -8,6 +8,7 @@ are newer (the same build ``__graft_entry__.build()`` runs).
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import os
 import threading
 
@@ -47,7 +48,7 @@ SIGNATURES = {
                                _c_float, _vp]),
     "fa_layernorm_rows": (_c_int, [_vp, _vp, _c_int, _c_int, _i64, _i64, _c_float, _vp]),
     "fa_mlp_fwd_noalloc": (_c_int, [_vp, _vp, _vp, _vp, _c_int, _c_int, _c_int, _c_int, _vp]),
-    # Argument structs are packed by the caller and passed as bytes.
+    # (argument structs as bytes, packed as the header lays them out)
     "fa_rotary": (_c_int, [ctypes.c_char_p, _vp]),
     "fa_paged_append": (_c_int, [ctypes.c_char_p, _vp]),
     "fa_paged_attn_workspace": (_i64, [ctypes.c_char_p]),
@@ -59,6 +60,7 @@ SIGNATURES = {
 
 _lock = threading.Lock()
 _lib = None
+_binding = None
 
 
 class FaError(RuntimeError):
@@ -86,6 +88,23 @@ def load(build_if_stale: bool = True) -> ctypes.CDLL:
             fn.argtypes = args
         _lib = lib
         return lib
+
+
+def load_binding():
+    """The torch binding (csrc/torch_binding.cpp), bound to the loaded library."""
+    global _binding
+    lib = load()
+    with _lock:
+        if _binding is None:
+            import torch  # noqa: F401  (its libraries are what the binding links to)
+            spec = importlib.util.spec_from_file_location("_fa_torch", _build.BINDING_PATH)
+            module = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(module)
+            module.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value
+                          for name in ("fa_rotary", "fa_paged_append", "fa_paged_attn_workspace",
+                                       "fa_paged_attn")), check)
+            _binding = module
+        return _binding
 
 
 def strerror(code: int) -> str:

@@ -1,11 +1,13 @@
-"""Build libfa_b200.so in-tree with nvcc for sm_100a.
+"""Build libfa_b200.so in-tree with nvcc for sm_100a, and the torch binding.
 
     python -m cs348k_fast_attention_grammar_b200.build [--force] [--verbose]
 
 The library is a plain C-ABI shared object (no torch types in its
 signatures), so it is compiled by nvcc directly rather than as a torch
 extension.  It links the CUDA runtime statically and needs no libcuda at link
-time (tensor maps are encoded through cudaGetDriverEntryPoint).
+time (tensor maps are encoded through cudaGetDriverEntryPoint).  _fa_torch.so
+is a CPython module (g++, torch's headers) that holds no kernels: the host side
+of the operators whose small calls are host bound.
 """
 
 from __future__ import annotations
@@ -23,6 +25,9 @@ LIB_NAME = "libfa_b200.so"
 LIB_PATH = os.path.join(PKG_DIR, LIB_NAME)
 SOURCES = ["common.cu", "attn_fwd.cu", "gemm.cu", "rotary.cu", "paged_attn.cu",
            "paged_tiles.cu"]
+BINDING_NAME = "_fa_torch.so"
+BINDING_PATH = os.path.join(PKG_DIR, BINDING_NAME)
+BINDING_SOURCE = os.path.join(CSRC, "torch_binding.cpp")
 HEADERS = ["sm100_ptx.cuh", "sm100_tmem_wide.cuh", "sm100_2sm.cuh", "fa_internal.h",
            "paged.cuh", "paged_attn.h"]
 PUBLIC_HEADER = os.path.join(os.path.dirname(PKG_DIR), "include", "fa_b200.h")
@@ -44,15 +49,49 @@ def _inputs():
             [os.path.join(CSRC, h) for h in HEADERS] + [PUBLIC_HEADER])
 
 
-def is_stale() -> bool:
-    if not os.path.exists(LIB_PATH):
+def _older(path, inputs) -> bool:
+    if not os.path.exists(path):
         return True
-    t = os.path.getmtime(LIB_PATH)
-    return any(os.path.getmtime(p) > t for p in _inputs() if os.path.exists(p))
+    t = os.path.getmtime(path)
+    return any(os.path.getmtime(p) > t for p in inputs if os.path.exists(p))
+
+
+def _library_stale() -> bool:
+    return _older(LIB_PATH, _inputs())
+
+
+def _binding_stale() -> bool:
+    return _older(BINDING_PATH, [BINDING_SOURCE, PUBLIC_HEADER])
+
+
+def is_stale() -> bool:
+    return _library_stale() or _binding_stale()
+
+
+def _library_command(verbose: bool) -> list:
+    cmd = [nvcc_path()] + ARCH_FLAGS + NVCC_FLAGS + ["--threads", "0"]
+    if verbose:
+        cmd.insert(1, "-Xptxas=-v")
+    return cmd + [os.path.join(CSRC, s) for s in SOURCES]
+
+
+def _binding_command() -> list:
+    import sysconfig
+
+    import torch
+    root = os.path.join(os.path.dirname(torch.__file__))
+    cuda = os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(nvcc_path()))), "include")
+    return ([os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
+             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+             "-I" + sysconfig.get_paths()["include"], "-I" + os.path.join(root, "include"),
+             "-I" + os.path.join(root, "include", "torch", "csrc", "api", "include"),
+             "-I" + cuda, BINDING_SOURCE, "-L" + os.path.join(root, "lib"), "-ltorch_python",
+             "-ltorch_cpu", "-ltorch", "-lc10", "-lc10_cuda"])
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
-    """Compile the library if it is missing or older than its sources.
+    """Compile the library and the binding if they are missing or older than
+    their sources; returns the library's path.
 
     Safe when several processes (the ranks of one job) call it at once: an
     exclusive lock on a file beside the library lets one of them compile, the
@@ -63,22 +102,33 @@ def build(force: bool = False, verbose: bool = False) -> str:
     with open(LIB_PATH + ".lock", "a+") as lock:
         fcntl.flock(lock, fcntl.LOCK_EX)
         try:
-            if not force and not is_stale():
-                return LIB_PATH          # another process built it meanwhile
-            tmp = f"{LIB_PATH}.{os.getpid()}.tmp"
-            cmd = ([nvcc_path()] + ARCH_FLAGS + NVCC_FLAGS +
-                   [os.path.join(CSRC, s) for s in SOURCES] + ["-o", tmp])
-            if verbose:
-                cmd.insert(1, "-Xptxas=-v")
-                print(" ".join(cmd), file=sys.stderr)
-            r = subprocess.run(cmd, capture_output=True, text=True)
-            if verbose or r.returncode != 0:
-                sys.stderr.write(r.stdout + r.stderr)
-            if r.returncode != 0:
-                if os.path.exists(tmp):
-                    os.unlink(tmp)
-                raise RuntimeError(f"nvcc failed with exit code {r.returncode}")
-            os.replace(tmp, LIB_PATH)
+            jobs = []
+            if force or _library_stale():
+                jobs.append((LIB_PATH, _library_command(verbose)))
+            if force or _binding_stale():
+                jobs.append((BINDING_PATH, _binding_command()))
+            running = []
+            for path, cmd in jobs:
+                tmp = f"{path}.{os.getpid()}.tmp"
+                cmd = cmd + ["-o", tmp]
+                if verbose:
+                    print(" ".join(cmd), file=sys.stderr)
+                running.append((path, tmp, cmd[0], subprocess.Popen(
+                    cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))
+            failed = []
+            for path, tmp, tool, proc in running:
+                out, _ = proc.communicate()
+                if verbose or proc.returncode != 0:
+                    sys.stderr.write(out)
+                if proc.returncode != 0:
+                    if os.path.exists(tmp):
+                        os.unlink(tmp)
+                    failed.append(f"{os.path.basename(tool)} failed with exit code "
+                                  f"{proc.returncode}")
+                else:
+                    os.replace(tmp, path)
+            if failed:
+                raise RuntimeError("; ".join(failed))
         finally:
             fcntl.flock(lock, fcntl.LOCK_UN)
     return LIB_PATH

@@ -1,12 +1,18 @@
 """What the rotary and paged operators refuse, without a GPU: the Python checks on
 CPU tensors (devices are checked last) and the C ABI's status codes."""
 
+import struct
+
 import pytest
 import torch
 
-from cs348k_fast_attention_grammar_b200 import _lib, paged, paged_attention, paged_kv_append, rotary
+from cs348k_fast_attention_grammar_b200 import _lib, paged_attention, paged_kv_append, rotary
 
 BF16 = torch.bfloat16
+# The argument structs of include/fa_b200.h: pointers, then 64-bit members.
+ROTARY = struct.Struct("=4Q24q")
+APPEND = struct.Struct("=11Q35q")
+ATTN = struct.Struct("=7Q22qd")
 P = 4096            # a stand-in for a device address: argument checks come before any CUDA call
 
 
@@ -113,7 +119,7 @@ def test_rotary_status_codes():
 
     def call(x=P, out=P, pos=P, freq=P, dtype=0, B=1, H=2, S=5, D=64, R=64, xs=(640, 320, 64),
              os=(640, 320, 64), axes=1, ends=(32, 0, 0, 0)):
-        return lib.fa_rotary(paged._ROTARY.pack(x, out, pos, freq, dtype, B, H, S, D, R, *xs, *os,
+        return lib.fa_rotary(ROTARY.pack(x, out, pos, freq, dtype, B, H, S, D, R, *xs, *os,
                                                 axes, *ends, 0, 0, 1, 0, 0, 0, 0), None)
 
     assert lib.fa_rotary(None, None) == code["FA_ERR_NULL"]
@@ -138,7 +144,7 @@ def test_append_status_codes():
     def call(ptrs=(P,) * 11, dtype=0, T=3, B=3, Hq=4, Hkv=2, D=64, R=64, pages=4, page=16, width=2,
              ts=2, st=(128, 64, 128, 64, 256, 64, 256, 64), cs=(2048, 128, 64) * 2, axes=1,
              ends=(32, 0, 0, 0)):
-        return lib.fa_paged_append(paged._APPEND.pack(
+        return lib.fa_paged_append(APPEND.pack(
             *ptrs, dtype, T, B, Hq, Hkv, D, R, pages, page, width, ts, *st, *cs, axes, *ends, 0, 1,
             0, 0, 0), None)
 
@@ -172,7 +178,7 @@ def test_attention_status_codes():
 
     def call(ptrs=(P,) * 7, dtype=0, T=3, B=3, Hq=4, Hkv=2, D=64, pages=4, page=16, width=2, ts=2,
              st=(256, 64, 256, 64), cs=(2048, 128, 64) * 2, longest=1, scale=0.125):
-        args = paged._ATTN.pack(*ptrs, dtype, T, B, Hq, Hkv, D, pages, page, width, ts, *st, *cs,
+        args = ATTN.pack(*ptrs, dtype, T, B, Hq, Hkv, D, pages, page, width, ts, *st, *cs,
                                 longest, 1, scale)
         rc = lib.fa_paged_attn(args, P, 1 << 40, None)
         assert lib.fa_paged_attn_workspace(args) == -rc
@@ -204,8 +210,8 @@ def test_argument_structs_match_the_header():
     from conftest import ROOT
     text = open(os.path.join(ROOT, "include", "fa_b200.h")).read()
     text = re.sub(r"/\*.*?\*/", "", text, flags=re.S)
-    for name, packed in (("fa_rotary_args", paged._ROTARY), ("fa_paged_append_args", paged._APPEND),
-                         ("fa_paged_attn_args", paged._ATTN)):
+    for name, packed in (("fa_rotary_args", ROTARY), ("fa_paged_append_args", APPEND),
+                         ("fa_paged_attn_args", ATTN)):
         body = re.search(r"typedef struct %s \{(.*?)\} %s;" % (name, name), text, re.S).group(1)
         n = 0
         for decl in body.split(";"):
