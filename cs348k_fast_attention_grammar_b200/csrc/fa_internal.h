@@ -52,4 +52,23 @@ int make_tmap_2d(CUtensorMap* map, const void* base, uint64_t rows, uint64_t col
 int make_tmap_bhsd(CUtensorMap* map, const void* base, int B, int H, int S, int D,
                    int64_t sb, int64_t sh, int64_t ss, uint32_t box_rows, bool f16 = false);
 
+// Launches a kernel as a programmatic dependent of the one before it in the
+// stream: it may start while that one ends, and calls grid_dependency_wait()
+// before it touches memory.
+template <typename... Args>
+inline int launch_after(void (*kern)(Args...), dim3 grid, int threads, int smem, cudaStream_t stream,
+                 const Args&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, args...) == cudaSuccess ? FA_OK : FA_ERR_LAUNCH;
+}
+
 }  // namespace fa

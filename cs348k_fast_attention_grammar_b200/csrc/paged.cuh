@@ -25,17 +25,21 @@ __host__ __device__ __forceinline__ SeqRows seq_rows(const int32_t* cu, int b, i
   return r;
 }
 
-// Sequence that row t belongs to (the last b with cu[b] <= t), or -1.
-__host__ __device__ __forceinline__ int seq_of_row(const int32_t* cu, int B, int t) {
+// Sequence that row t belongs to (the last b with cu[b] <= t), or -1.  A search by
+// 32 probes at a time: count(lo, step, hi) is the number of the probes lo + step,
+// lo + 2 step, ... (32 of them, those below hi) with cu[probe] <= t.
+template <typename Count>
+__host__ __device__ __forceinline__ int seq_of_row(const int32_t* cu, int B, int t, Count count) {
   if (cu == nullptr) return t < B ? t : -1;
-  if (t < cu[0] || t >= cu[B]) return -1;
+  const int below = cu[0], above = cu[B];
   int lo = 0, hi = B;                 // cu[lo] <= t < cu[hi]
   while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (cu[mid] <= t) lo = mid;
-    else hi = mid;
+    const int step = (hi - lo - 1 + 31) / 32;
+    const int n = count(lo, step, hi);
+    if (hi - lo > (n + 1) * static_cast<int64_t>(step)) hi = lo + (n + 1) * step;
+    lo += n * step;
   }
-  return lo;
+  return t < below || t >= above ? -1 : lo;
 }
 
 // Page of key `place` of a sequence with this table row: -1 where the place lies

@@ -190,6 +190,7 @@ __global__ void __launch_bounds__(kRowThreads)
   constexpr int CH = DT / 8;            // 16-byte chunks of a row
   constexpr int RPI = 32 / CH;          // rows one warp-wide copy covers
   extern __shared__ __align__(128) uint8_t smem[];
+  grid_dependency_wait();
   grid_dependents_launch();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t ring = smem_u32(smem) + warp * C::kWarp;
@@ -473,8 +474,11 @@ __global__ void __launch_bounds__(kRowThreads)
   using C = RowCfg<DT, MT>;
   const int lane = threadIdx.x & 31;
   const int r = blockIdx.y * kRowWarps + (threadIdx.x >> 5);
+  // The row kernel starts when all before it is done, so lengths and tables can
+  // be read ahead of the wait for its parts.
   const Range rg = find_range<true>(p, blockIdx.x, C::kRows);
-  grid_dependency_wait();               // the parts are complete
+  grid_dependency_wait();
+  grid_dependents_launch();
   if (rg.start >= rg.end) return;
   const RowWork w = row_work(p, rg.b, C::kRows);
   const int unit = static_cast<int>((rg.end - 1 - rg.base) / w.blocks);
@@ -539,22 +543,13 @@ int launch_rows(const PagedParams& p, cudaStream_t stream) {
   using C = RowCfg<DT, MT>;
   static KernelPrep prep;
   int dev = 0;
-  const int rc = prepare_kernel(
+  int rc = prepare_kernel(
       prep, reinterpret_cast<const void*>(paged_rows_kernel<DT, MT, F16>), C::kSmem, &dev);
   if (rc != FA_OK) return rc;
-  paged_rows_kernel<DT, MT, F16><<<p.ctas, kRowThreads, C::kSmem, stream>>>(p);
-  if (cudaGetLastError() != cudaSuccess) return FA_ERR_LAUNCH;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(p.ctas, C::kRows / kRowWarps);
-  cfg.blockDim = dim3(kRowThreads);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, paged_rows_join<DT, MT, F16>, p) == cudaSuccess ? FA_OK
-                                                                                  : FA_ERR_LAUNCH;
+  rc = launch_after(paged_rows_kernel<DT, MT, F16>, dim3(p.ctas), kRowThreads, C::kSmem, stream, p);
+  if (rc != FA_OK) return rc;
+  return launch_after(paged_rows_join<DT, MT, F16>, dim3(p.ctas, C::kRows / kRowWarps), kRowThreads,
+                      0, stream, p);
 }
 
 template <int DT, int MT>

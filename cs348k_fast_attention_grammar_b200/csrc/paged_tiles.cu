@@ -170,6 +170,7 @@ __global__ void __launch_bounds__(kPlanThreads)
   __shared__ int64_t red[32];
   __shared__ int64_t cells_before[kPlanThreads + 1];    // of (sequence, unit) pairs, one head
   __shared__ int count[kPlanThreads];
+  grid_dependency_wait();
   grid_dependents_launch();
   const int tid = threadIdx.x;
   int64_t pairs = 0;
@@ -785,6 +786,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps)
     paged_tiles_join(const TileParams p) {
   using C = Cfg<D>;
   grid_dependency_wait();
+  grid_dependents_launch();
   if (p.plan[kSplit] == 0) return;
   const int2 jn = p.join[blockIdx.x];
   if (jn.y == 0) return;
@@ -889,22 +891,6 @@ int make_map(CUtensorMap* map, const void* ptr, const int64_t (&dims)[4],
   return r == CUDA_SUCCESS ? FA_OK : FA_ERR_TMA;
 }
 
-template <typename... Args>
-int launch_after(void (*kern)(Args...), dim3 grid, int threads, int smem, cudaStream_t stream,
-                 const Args&... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kern, args...) == cudaSuccess ? FA_OK : FA_ERR_LAUNCH;
-}
-
 template <int D, bool F16>
 int launch_tiles(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
                  const TileParams& p, bool split, cudaStream_t stream) {
@@ -914,8 +900,8 @@ int launch_tiles(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap
   int rc = prepare_kernel(prep, reinterpret_cast<const void*>(paged_tiles_kernel<D, F16>),
                           C::kSmemBytes, &dev);
   if (rc != FA_OK) return rc;
-  paged_plan_kernel<<<1, kPlanThreads, 0, stream>>>(p);
-  if (cudaGetLastError() != cudaSuccess) return FA_ERR_LAUNCH;
+  rc = launch_after(paged_plan_kernel, dim3(1), kPlanThreads, 0, stream, p);
+  if (rc != FA_OK) return rc;
   rc = launch_after(paged_tiles_kernel<D, F16>, dim3(p.ctas), kThreads, C::kSmemBytes, stream, mq,
                     mk, mv, p);
   if (rc != FA_OK || !split) return rc;

@@ -3,12 +3,12 @@
 //     (a, b) -> (a cos t - b sin t, b cos t + a sin t),   t = position * inv_freq[i]
 //
 // Both are bound by HBM: each value is read once and written once.  A CTA of
-// 256 threads takes a few rows (tokens).  It loads its first vectors, computes
-// the rows' sines and cosines once into shared memory while those loads are in
-// flight, then rotates and stores; a thread's item is two 16-byte vectors R / 2
-// channels apart, so that the planes (i, i + R / 2) stay inside one thread and
-// the planes (2i, 2i + 1) inside one vector.  Every head of a row shares the
-// row's angles.
+// 256 threads takes a few rows (tokens).  It loads its first vectors, finds the
+// rows' places and computes their sines and cosines once into shared memory while
+// those loads are in flight, then rotates and stores; a thread's item is two
+// 16-byte vectors R / 2 channels apart, so that the planes (i, i + R / 2) stay
+// inside one thread and the planes (2i, 2i + 1) inside one vector.  Every head of
+// a row shares the row's angles.
 //
 // An angle of a far position needs more than fp32: position * inv_freq is
 // formed in fp64 in turns (inv_freq / 2 pi), the whole turns are dropped
@@ -43,7 +43,8 @@ struct Part {
   void* dst;
   int64_t src_sb, src_sh, src_ss;       // elements
   int64_t dst_sb, dst_sh, dst_ss;
-  int heads, rotate, items;             // items per head
+  int heads, rotate;
+  int items, count;                     // items of a head, of all heads
 };
 
 struct RotParams {
@@ -103,6 +104,25 @@ __device__ __forceinline__ uint4 pack(const float (&f)[16 / Elem<TYPE>::kSize]) 
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// N consecutive cosines or sines from shared memory.
+template <int N>
+__device__ __forceinline__ void load_angles(const float* at, float (&f)[N]) {
+  if constexpr (N >= 4) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      const float4 v = *reinterpret_cast<const float4*>(at + i);
+      f[i] = v.x;
+      f[i + 1] = v.y;
+      f[i + 2] = v.z;
+      f[i + 3] = v.w;
+    }
+  } else {
+    const float2 v = *reinterpret_cast<const float2*>(at);
+    f[0] = v.x;
+    f[1] = v.y;
+  }
+}
+
 __device__ __forceinline__ float2 cos_sin(const Angles& a, int64_t b, int64_t s, int i,
                                           bool own_pos, int place) {
   double pos;
@@ -127,10 +147,10 @@ __device__ __forceinline__ float2 cos_sin(const Angles& a, int64_t b, int64_t s,
 // An item: up to two vectors of one head.
 struct Item {
   const char* src;
-  char* dst;
-  int off0, off1;       // byte offsets of the vectors, -1: none
-  int row, chunk;
-  bool rotate;
+  char* dst;            // its tensor's start; the row's offset is added when it is known
+  int off0, off1;       // byte offsets of the vectors, -1: no second one
+  int row, angle;       // row of the CTA; first plane, -1: copied
+  int part;
 };
 
 // APPEND: rows are packed new tokens, keys and values go to their pages.
@@ -139,155 +159,167 @@ __global__ void __launch_bounds__(kRotThreads)
     rotary_kernel(const RotParams p) {
   constexpr int kSize = Elem<TYPE>::kSize;
   constexpr int V = 16 / kSize;
-  __shared__ float2 cs[kRotMaxAngles];
-  __shared__ int64_t s_kdst[kRotMaxRows], s_vdst[kRotMaxRows];   // element offsets, -1: no place
+  __shared__ __align__(16) float s_cos[kRotMaxAngles], s_sin[kRotMaxAngles];
+  __shared__ int64_t s_dst[3][kRotMaxRows];     // element offset of the row's place, -1: none
+  __shared__ int64_t s_batch[kRotMaxRows];
   __shared__ int s_place[kRotMaxRows];
-  __shared__ int s_live[kRotMaxRows];
+  grid_dependency_wait();
+  grid_dependents_launch();
 
   const int64_t row0 = static_cast<int64_t>(blockIdx.x) * p.rows_per_cta;
   const int rows = static_cast<int>(min(static_cast<int64_t>(p.rows_per_cta), p.rows - row0));
   const int half = p.ang.R / 2;
-  const int rot_items = half / V;
-  const int total = rows * p.items_per_row;
+  const unsigned rot_items = half / V;
+  const unsigned total = rows * p.items_per_row;
 
-  auto locate = [&](int it) {
+  if (!APPEND) {
+    if (threadIdx.x < rows) s_batch[threadIdx.x] = (row0 + threadIdx.x) / p.S;
+    __syncthreads();
+  }
+
+  auto locate = [&](unsigned it) {
     Item x;
-    x.row = it / p.items_per_row;
-    int r = it - x.row * p.items_per_row;
-    int part = 0;
+    x.row = it / static_cast<unsigned>(p.items_per_row);
+    unsigned r = it - x.row * p.items_per_row;
+    x.part = 0;
     if (APPEND) {
-      while (part + 1 < p.parts && r >= p.part[part].heads * p.part[part].items) {
-        r -= p.part[part].heads * p.part[part].items;
-        ++part;
+      while (x.part + 1 < p.parts && r >= static_cast<unsigned>(p.part[x.part].count)) {
+        r -= p.part[x.part].count;
+        ++x.part;
       }
     }
-    const Part& q = p.part[part];
-    const int head = r / q.items;
-    x.chunk = r - head * q.items;
-    x.rotate = q.rotate != 0;
-    const int64_t row = row0 + x.row;
-    const int64_t b = APPEND ? 0 : row / p.S;
-    const int64_t s = APPEND ? row : row - b * p.S;
-    x.src = static_cast<const char*>(q.src) + (b * q.src_sb + s * q.src_ss + head * q.src_sh) * kSize;
-    x.dst = static_cast<char*>(q.dst) + (b * q.dst_sb + head * q.dst_sh) * kSize;
-    if (!APPEND || part == 2) {
-      x.dst += s * q.dst_ss * kSize;
+    const Part& q = p.part[x.part];
+    const unsigned head = r / static_cast<unsigned>(q.items);
+    const unsigned chunk = r - head * q.items;
+    const int64_t b = APPEND ? 0 : s_batch[x.row];
+    const int64_t s = row0 + x.row - b * p.S;
+    x.src = static_cast<const char*>(q.src) +
+            (b * q.src_sb + s * q.src_ss + head * q.src_sh) * kSize;
+    x.dst = static_cast<char*>(q.dst) + head * q.dst_sh * kSize;
+    if (!APPEND) x.dst += (b * q.dst_sb + s * q.dst_ss) * kSize;
+    if (q.rotate && chunk < rot_items) {
+      x.off0 = chunk * 16;
+      x.off1 = (half + chunk * V) * kSize;
+      x.angle = x.row * half + chunk * (INTERLEAVED ? V / 2 : V);
     } else {
-      const int64_t at = part == 0 ? s_kdst[x.row] : s_vdst[x.row];
-      x.dst = at < 0 ? nullptr : x.dst + at * kSize;
-    }
-    if (APPEND && !s_live[x.row]) x.dst = nullptr;
-    if (x.rotate && x.chunk < rot_items) {
-      x.off0 = x.chunk * 16;
-      x.off1 = (half + x.chunk * V) * kSize;
-    } else {
-      const int c0 = x.rotate ? p.ang.R + 2 * (x.chunk - rot_items) * V : 2 * x.chunk * V;
+      const int c0 = q.rotate ? p.ang.R + 2 * (chunk - rot_items) * V : 2 * chunk * V;
       x.off0 = c0 * kSize;
       x.off1 = c0 + V < p.D ? (c0 + V) * kSize : -1;
-      x.rotate = false;
+      x.angle = -1;
     }
     return x;
   };
+  auto load = [&](const Item& x, uint4& u0, uint4& u1) {
+    u0 = *reinterpret_cast<const uint4*>(x.src + x.off0);
+    if (x.off1 >= 0) u1 = *reinterpret_cast<const uint4*>(x.src + x.off1);
+  };
 
+  // The first items' loads are in flight while places and angles are found.
+  uint4 a[kRotItems], c[kRotItems];
+  Item item[kRotItems];
+#pragma unroll
+  for (int u = 0; u < kRotItems; ++u) {
+    const unsigned it = threadIdx.x + u * kRotThreads;
+    if (it < total) {
+      item[u] = locate(it);
+      load(item[u], a[u], c[u]);
+    }
+  }
   if (APPEND) {
-    // Where each row goes.
-    if (threadIdx.x < rows) {
-      const int r = threadIdx.x;
+    // Where each row goes: one warp per row.
+    const int lane = threadIdx.x & 31;
+    for (int r = threadIdx.x >> 5; r < rows; r += kRotThreads / 32) {
       const int t = static_cast<int>(row0) + r;
-      const int b = seq_of_row(p.cu, p.B, t);
-      s_live[r] = b >= 0;
-      s_kdst[r] = s_vdst[r] = -1;
-      s_place[r] = 0;
-      if (b >= 0) {
-        const int end = p.cu == nullptr ? b + 1 : p.cu[b + 1];
-        const int place = p.kv_lens[b] - (end - t);
-        s_place[r] = place;
-        if (place >= 0) {
-          const int page = page_at(p.table + b * p.table_stride, place, p.page_shift, p.max_pages,
-                                   p.pages);
-          if (page >= 0) {
-            const int in = place & ((1 << p.page_shift) - 1);
-            s_kdst[r] = page * p.kc_page + in * p.part[0].dst_ss;
-            s_vdst[r] = page * p.vc_page + in * p.part[1].dst_ss;
-          } else {
-            atomicExch(p.status, kDevBadPage);
+      const int b = seq_of_row(p.cu, p.B, t, [&](int lo, int step, int hi) {
+        const int64_t at = lo + static_cast<int64_t>(lane + 1) * step;
+        return __popc(__ballot_sync(0xffffffffu, at < hi && p.cu[at < hi ? at : lo] <= t));
+      });
+      if (lane == 0) {
+        int64_t k = -1, v = -1;
+        int place = 0;
+        if (b >= 0) {
+          place = p.kv_lens[b] - ((p.cu == nullptr ? b + 1 : p.cu[b + 1]) - t);
+          if (place >= 0) {
+            const int page = page_at(p.table + b * p.table_stride, place, p.page_shift,
+                                     p.max_pages, p.pages);
+            if (page >= 0) {
+              const int in = place & ((1 << p.page_shift) - 1);
+              k = page * p.kc_page + in * p.part[0].dst_ss;
+              v = page * p.vc_page + in * p.part[1].dst_ss;
+            } else {
+              atomicExch(p.status, kDevBadPage);
+            }
           }
         }
+        s_dst[0][r] = k;
+        s_dst[1][r] = v;
+        s_dst[2][r] = b < 0 ? -1 : t * p.part[2].dst_ss;
+        s_place[r] = place;
       }
     }
     __syncthreads();
   }
-
-  // The first items' loads are in flight while the angles are computed.
-  uint4 a[kRotItems], c[kRotItems];
-#pragma unroll
-  for (int u = 0; u < kRotItems; ++u) {
-    const int it = threadIdx.x + u * kRotThreads;
-    if (it < total) {
-      const Item x = locate(it);
-      if (x.dst != nullptr) {
-        a[u] = *reinterpret_cast<const uint4*>(x.src + x.off0);
-        if (x.off1 >= 0) c[u] = *reinterpret_cast<const uint4*>(x.src + x.off1);
-      }
-    }
-  }
   for (int i = threadIdx.x; i < rows * half; i += kRotThreads) {
-    const int r = i / half;
-    const int64_t row = row0 + r;
-    const int64_t b = APPEND ? 0 : row / p.S;
-    if (!APPEND || s_live[r])
-      cs[i] = cos_sin(p.ang, b, row - b * p.S, i - r * half, p.ang.pos == nullptr,
-                      APPEND ? s_place[r] : 0);
+    const int r = static_cast<unsigned>(i) / static_cast<unsigned>(half);
+    const int64_t b = APPEND ? 0 : s_batch[r];
+    if (APPEND && s_dst[2][r] < 0) continue;           // (a row of no sequence has no position)
+    const float2 w = cos_sin(p.ang, b, row0 + r - b * p.S, i - r * half, p.ang.pos == nullptr,
+                             APPEND ? s_place[r] : 0);
+    s_cos[i] = w.x;
+    s_sin[i] = w.y;
   }
   __syncthreads();
 
   auto finish = [&](const Item& x, const uint4& u0, const uint4& u1) {
-    if (!x.rotate) {
-      *reinterpret_cast<uint4*>(x.dst + x.off0) = u0;
-      if (x.off1 >= 0) *reinterpret_cast<uint4*>(x.dst + x.off1) = u1;
+    char* dst = x.dst;
+    if (APPEND) {
+      const int64_t at = s_dst[x.part][x.row];
+      if (at < 0) return;
+      dst += at * kSize;
+    }
+    if (x.angle < 0) {
+      *reinterpret_cast<uint4*>(dst + x.off0) = u0;
+      if (x.off1 >= 0) *reinterpret_cast<uint4*>(dst + x.off1) = u1;
       return;
     }
     float f[V], g[V];
     unpack<TYPE>(u0, f);
     unpack<TYPE>(u1, g);
-    const float2* w = cs + x.row * half;
     if (INTERLEAVED) {
-      const int i0 = x.chunk * V / 2, i1 = half / 2 + x.chunk * V / 2;
+      float cf[V / 2], sf[V / 2], cg[V / 2], sg[V / 2];
+      load_angles(s_cos + x.angle, cf);
+      load_angles(s_sin + x.angle, sf);
+      load_angles(s_cos + x.angle + half / 2, cg);
+      load_angles(s_sin + x.angle + half / 2, sg);
 #pragma unroll
       for (int e = 0; e < V; e += 2) {
-        const float2 r = w[i0 + e / 2], q = w[i1 + e / 2];
         const float f0 = f[e], g0 = g[e];
-        f[e] = fmaf(f0, r.x, -f[e + 1] * r.y);
-        f[e + 1] = fmaf(f[e + 1], r.x, f0 * r.y);
-        g[e] = fmaf(g0, q.x, -g[e + 1] * q.y);
-        g[e + 1] = fmaf(g[e + 1], q.x, g0 * q.y);
+        f[e] = fmaf(f0, cf[e / 2], -f[e + 1] * sf[e / 2]);
+        f[e + 1] = fmaf(f[e + 1], cf[e / 2], f0 * sf[e / 2]);
+        g[e] = fmaf(g0, cg[e / 2], -g[e + 1] * sg[e / 2]);
+        g[e + 1] = fmaf(g[e + 1], cg[e / 2], g0 * sg[e / 2]);
       }
     } else {
+      float co[V], si[V];
+      load_angles(s_cos + x.angle, co);
+      load_angles(s_sin + x.angle, si);
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        const float2 r = w[x.chunk * V + e];
         const float f0 = f[e];
-        f[e] = fmaf(f0, r.x, -g[e] * r.y);
-        g[e] = fmaf(g[e], r.x, f0 * r.y);
+        f[e] = fmaf(f0, co[e], -g[e] * si[e]);
+        g[e] = fmaf(g[e], co[e], f0 * si[e]);
       }
     }
-    *reinterpret_cast<uint4*>(x.dst + x.off0) = pack<TYPE>(f);
-    *reinterpret_cast<uint4*>(x.dst + x.off1) = pack<TYPE>(g);
+    *reinterpret_cast<uint4*>(dst + x.off0) = pack<TYPE>(f);
+    *reinterpret_cast<uint4*>(dst + x.off1) = pack<TYPE>(g);
   };
 #pragma unroll
-  for (int u = 0; u < kRotItems; ++u) {
-    const int it = threadIdx.x + u * kRotThreads;
-    if (it < total) {
-      const Item x = locate(it);
-      if (x.dst != nullptr) finish(x, a[u], c[u]);
-    }
-  }
-  for (int it = threadIdx.x + kRotItems * kRotThreads; it < total; it += kRotThreads) {
+  for (int u = 0; u < kRotItems; ++u)
+    if (threadIdx.x + u * kRotThreads < total) finish(item[u], a[u], c[u]);
+  for (unsigned it = threadIdx.x + kRotItems * kRotThreads; it < total; it += kRotThreads) {
     const Item x = locate(it);
-    if (x.dst == nullptr) continue;
-    const uint4 u0 = *reinterpret_cast<const uint4*>(x.src + x.off0);
-    uint4 u1 = u0;
-    if (x.off1 >= 0) u1 = *reinterpret_cast<const uint4*>(x.src + x.off1);
+    uint4 u0, u1;
+    load(x, u0, u1);
     finish(x, u0, u1);
   }
 }
@@ -303,11 +335,15 @@ int launch_rotary(RotParams& p, int dtype, bool append, bool interleaved, cudaSt
     Part& q = p.part[i];
     const int rest = q.rotate ? p.D - p.ang.R : p.D;
     q.items = (q.rotate ? half / V : 0) + (rest / V + 1) / 2;
-    p.items_per_row += q.heads * q.items;
+    q.count = q.heads * q.items;
+    p.items_per_row += q.count;
   }
   // Rows per CTA: as many as its threads take in one go, within the shared
-  // memory for their angles.
+  // memory for their angles, and no more than leave every SM some.
   int rows = kRotThreads * kRotItems / p.items_per_row;
+  const int sms = sm_count(dev);
+  if (sms > 0 && p.rows < static_cast<int64_t>(rows) * sms)
+    rows = static_cast<int>((p.rows + sms - 1) / sms);
   if (half > 0) rows = rows < kRotMaxAngles / half ? rows : kRotMaxAngles / half;
   rows = rows < kRotMaxRows ? rows : kRotMaxRows;
   p.rows_per_cta = rows > 1 ? rows : 1;
@@ -318,19 +354,19 @@ int launch_rotary(RotParams& p, int dtype, bool append, bool interleaved, cudaSt
     p.status = device_status_ptr();
     if (p.status == nullptr) return FA_ERR_CUDA;
   }
-#define FA_ROT(T, A, I) rotary_kernel<T, A, I><<<g, kRotThreads, 0, stream>>>(p)
+  // (as a programmatic dependent: its CTAs come up while the kernel before ends)
+#define FA_ROT(T, A, I) launch_after(rotary_kernel<T, A, I>, dim3(g), kRotThreads, 0, stream, p)
   if (append) {
-    if (dtype == FA_BF16) interleaved ? FA_ROT(FA_BF16, true, true) : FA_ROT(FA_BF16, true, false);
-    else interleaved ? FA_ROT(FA_F16, true, true) : FA_ROT(FA_F16, true, false);
-  } else if (dtype == FA_BF16) {
-    interleaved ? FA_ROT(FA_BF16, false, true) : FA_ROT(FA_BF16, false, false);
-  } else if (dtype == FA_F16) {
-    interleaved ? FA_ROT(FA_F16, false, true) : FA_ROT(FA_F16, false, false);
-  } else {
-    interleaved ? FA_ROT(FA_F32, false, true) : FA_ROT(FA_F32, false, false);
+    if (dtype == FA_BF16)
+      return interleaved ? FA_ROT(FA_BF16, true, true) : FA_ROT(FA_BF16, true, false);
+    return interleaved ? FA_ROT(FA_F16, true, true) : FA_ROT(FA_F16, true, false);
   }
+  if (dtype == FA_BF16)
+    return interleaved ? FA_ROT(FA_BF16, false, true) : FA_ROT(FA_BF16, false, false);
+  if (dtype == FA_F16)
+    return interleaved ? FA_ROT(FA_F16, false, true) : FA_ROT(FA_F16, false, false);
+  return interleaved ? FA_ROT(FA_F32, false, true) : FA_ROT(FA_F32, false, false);
 #undef FA_ROT
-  return cudaGetLastError() == cudaSuccess ? FA_OK : FA_ERR_LAUNCH;
 }
 
 constexpr int64_t kMaxDim = 0x7fffffffLL;
@@ -395,7 +431,7 @@ extern "C" int fa_rotary(const fa_rotary_args* a, void* stream) {
   p.parts = 1;
   p.part[0] = {a->x, a->out, a->x_strides[0], a->x_strides[1], a->x_strides[2],
                a->out_strides[0], a->out_strides[1], a->out_strides[2],
-               static_cast<int>(a->H), 1, 0};
+               static_cast<int>(a->H), 1, 0, 0};
   p.D = static_cast<int>(a->D);
   p.rows = a->B * a->S;
   p.S = static_cast<int>(a->S);
@@ -441,13 +477,13 @@ extern "C" int fa_paged_append(const fa_paged_append_args* a, void* stream) {
   p.ang.pos_ss = a->pos_strides[1];
   const int rotate = a->R > 0;
   p.part[0] = {a->k, a->k_cache, 0, a->k_strides[1], a->k_strides[0], 0, a->k_cache_strides[2],
-               a->k_cache_strides[1], static_cast<int>(a->Hkv), rotate, 0};
+               a->k_cache_strides[1], static_cast<int>(a->Hkv), rotate, 0, 0};
   p.part[1] = {a->v, a->v_cache, 0, a->v_strides[1], a->v_strides[0], 0, a->v_cache_strides[2],
-               a->v_cache_strides[1], static_cast<int>(a->Hkv), 0, 0};
+               a->v_cache_strides[1], static_cast<int>(a->Hkv), 0, 0, 0};
   p.parts = 2;
   if (a->q) {
     p.part[2] = {a->q, a->q_out, 0, a->q_strides[1], a->q_strides[0], 0, a->q_out_strides[1],
-                 a->q_out_strides[0], static_cast<int>(a->Hq), rotate, 0};
+                 a->q_out_strides[0], static_cast<int>(a->Hq), rotate, 0, 0};
     p.parts = 3;
   }
   p.D = static_cast<int>(a->D);

@@ -231,7 +231,16 @@ _HARNESS = r"""
 #define __forceinline__ inline
 #include "paged.cuh"
 extern "C" {
-int seq_of_row(const int* cu, int B, int t) { return fa::seq_of_row(cu, B, t); }
+int seq_of_row(const int* cu, int B, int t) {
+  return fa::seq_of_row(cu, B, t, [&](int lo, int step, int hi) {
+    int n = 0;
+    for (int lane = 0; lane < 32; ++lane) {
+      const int64_t at = lo + static_cast<int64_t>(lane + 1) * step;
+      n += at < hi && cu[at] <= t;
+    }
+    return n;
+  });
+}
 void seq_rows(const int* cu, int b, int T, int* out) {
   const fa::SeqRows r = fa::seq_rows(cu, b, T);
   out[0] = r.begin;
@@ -271,6 +280,17 @@ def test_rows_of_sequences(index):
     for t in range(-1, 14):
         want = next((b for b in range(5) if cu[b] <= t < cu[b + 1]), -1)
         assert index.seq_of_row(a, 5, t) == want, t
+    for B in (1, 2, 31, 32, 33, 34, 63, 65, 1000, 1056, 1057, 40000):
+        cu = [0]
+        for b in range(B):
+            cu.append(cu[-1] + (b * 7 + B) % 3)
+        a = _array(cu)
+        owner = {}
+        for b in range(B):
+            for t in range(cu[b], cu[b + 1]):
+                owner[t] = b
+        for t in list(range(0, cu[-1], max(1, cu[-1] // 500))) + [cu[-1] - 1, cu[-1], cu[-1] + 1]:
+            assert index.seq_of_row(a, B, t) == owner.get(t, -1), (B, t)
     assert [index.seq_of_row(None, 3, t) for t in (0, 2, 3)] == [0, 2, -1]
     out = _array([0, 0])
     for borders, T in (([0, 1, 900], 4), ([-5, 1, 2], 4), ([3, 1, 2], 4), ([0, 2 ** 31 - 1, 1], 4),
