@@ -20,7 +20,6 @@
 // depend on timing.
 #include <cuda_bf16.h>
 
-#include <climits>
 #include <cmath>
 
 #include "paged_attn.h"
@@ -43,7 +42,7 @@ struct RowWork : SeqWork {
 __device__ __forceinline__ RowWork row_work(const PagedParams& p, int b, int tile_rows) {
   RowWork w;
   static_cast<SeqWork&>(w) = seq_work(p, b);
-  w.tiles = static_cast<int>((w.rows + tile_rows - 1) / tile_rows);
+  w.tiles = static_cast<int>((static_cast<int64_t>(w.q_len) * p.g + tile_rows - 1) / tile_rows);
   w.blocks = max(1, (w.kv_len + kRowKeys - 1) / kRowKeys);
   return w;
 }
@@ -593,37 +592,25 @@ int check_paged_attn(const fa_paged_attn_args* a) {
   return FA_OK;
 }
 
-// Which kernels run.  The row kernel takes sequences of up to kRowMax rows and
-// the tile kernel the others; only one of them runs where the longest sequence
-// is short, where all are alike (T = B * max_q_len) or there is only one, and it
-// then takes whatever it finds.
+// Which kernel runs: the row kernel where the longest sequence has few rows,
+// else the tile kernel, for short sequences of the batch too.  (Separate launches
+// for the two kinds took 176 us against 130 for 5 chunks and 4 single tokens,
+// 1787 tokens over 32k keys, 32/8 heads of 128: the second launch costs more than
+// a tile kernel's unit of a single token.)
 constexpr int kRowMax = 32;
 
-struct Choice {
-  bool rows, tiles;
-  int row_tiles;        // the row kernel's tiles: 16 rows where every sequence fits, else 32
-};
+enum class Kernel { kRows16, kRows32, kTiles };
 
-Choice choose(const fa_paged_attn_args* a) {
-  const int64_t g = a->Hq / a->Hkv;
-  const int64_t longest = a->max_q_len < a->T ? a->max_q_len : a->T;
-  Choice c = {true, true, 2};
+Kernel choose(const fa_paged_attn_args* a) {
+  const int64_t longest = (a->max_q_len < a->T ? a->max_q_len : a->T) * (a->Hq / a->Hkv);
   // The tile kernel's copies need real strides, its exponent a scale that keeps order.
   const bool flat = (a->q_strides[0] == 0 && a->T > 1) || (a->q_strides[1] == 0 && a->Hq > 1) ||
                     (a->k_cache_strides[0] == 0 && a->pages > 1) || a->k_cache_strides[1] == 0 ||
                     (a->k_cache_strides[2] == 0 && a->Hkv > 1) ||
                     (a->v_cache_strides[0] == 0 && a->pages > 1) || a->v_cache_strides[1] == 0 ||
                     (a->v_cache_strides[2] == 0 && a->Hkv > 1);
-  if (longest * g <= kRowMax || flat || a->scale < 0) c.tiles = false;
-  else if (a->B == 1 || a->T == a->B * longest) c.rows = false;
-  if (longest * g <= 16) c.row_tiles = 1;
-  return c;
-}
-
-int64_t rows_bytes(const fa_paged_attn_args* a, const Choice& c, int sms) {
-  if (!c.rows) return 0;
-  const int dt = a->D <= 64 ? 64 : 128;
-  return static_cast<int64_t>(2 * kRowCtasPerSm * sms) * 16 * c.row_tiles * (dt + 2) * 4;
+  if (longest > kRowMax && !flat && a->scale >= 0) return Kernel::kTiles;
+  return longest <= 16 ? Kernel::kRows16 : Kernel::kRows32;
 }
 
 }  // namespace
@@ -637,8 +624,10 @@ extern "C" int64_t fa_paged_attn_workspace(const fa_paged_attn_args* a) {
   if (cudaGetDevice(&dev) != cudaSuccess) return -FA_ERR_CUDA;
   const int sms = sm_count(dev);
   if (sms <= 0) return -FA_ERR_CUDA;
-  const Choice c = choose(a);
-  return rows_bytes(a, c, sms) + (c.tiles ? paged_tiles_bytes(a, sms) : 0);
+  const Kernel k = choose(a);
+  if (k == Kernel::kTiles) return paged_tiles_bytes(a, sms);
+  const int64_t slot = (k == Kernel::kRows16 ? 16 : 32) * ((a->D <= 64 ? 64 : 128) + 2);
+  return 2ll * kRowCtasPerSm * sms * slot * 4;
 }
 
 extern "C" int fa_paged_attn(const fa_paged_attn_args* a, void* workspace,
@@ -686,22 +675,15 @@ extern "C" int fa_paged_attn(const fa_paged_attn_args* a, void* workspace,
   const int sms = sm_count(dev);
   const bool f16 = a->dtype == FA_F16;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const Choice c = choose(a);
-  if (c.rows) {
-    p.part = static_cast<float*>(workspace);
-    p.ctas = kRowCtasPerSm * sms;
-    p.min_blocks = 4;
-    p.row_lo = 1;
-    p.row_hi = c.tiles ? kRowMax : INT_MAX;
-    if (c.row_tiles == 1)
-      rc = p.D <= 64 ? launch_rows_t<64, 1>(p, f16, s) : launch_rows_t<128, 1>(p, f16, s);
-    else
-      rc = p.D <= 64 ? launch_rows_t<64, 2>(p, f16, s) : launch_rows_t<128, 2>(p, f16, s);
-    if (rc != FA_OK) return rc;
+  const Kernel k = choose(a);
+  if (k == Kernel::kTiles) {
+    p.ctas = sms;
+    return launch_paged_tiles(a, p, workspace, s);
   }
-  if (!c.tiles) return FA_OK;
-  p.row_lo = c.rows ? kRowMax + 1 : 1;
-  p.row_hi = INT_MAX;
-  p.ctas = sms;
-  return launch_paged_tiles(a, p, static_cast<char*>(workspace) + rows_bytes(a, c, sms), s);
+  p.part = static_cast<float*>(workspace);
+  p.ctas = kRowCtasPerSm * sms;
+  p.min_blocks = 4;
+  if (k == Kernel::kRows16)
+    return p.D <= 64 ? launch_rows_t<64, 1>(p, f16, s) : launch_rows_t<128, 1>(p, f16, s);
+  return p.D <= 64 ? launch_rows_t<64, 2>(p, f16, s) : launch_rows_t<128, 2>(p, f16, s);
 }

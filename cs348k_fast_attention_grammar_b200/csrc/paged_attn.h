@@ -27,13 +27,11 @@ struct PagedParams {
   float* part;                          // partial results of split units
   int ctas;                             // ranges the key blocks are cut into
   int min_blocks;                       // least key blocks of a range
-  int row_lo, row_hi;                   // takes sequences of row_lo .. row_hi rows (q_len * g)
 };
 
-// A sequence's new tokens and keys; rows = 0 where a kernel leaves it to the other.
+// A sequence's new tokens and keys.
 struct SeqWork {
   int begin, q_len, kv_len;
-  int64_t rows;
 };
 
 __device__ __forceinline__ SeqWork seq_work(const PagedParams& p, int b) {
@@ -44,8 +42,6 @@ __device__ __forceinline__ SeqWork seq_work(const PagedParams& p, int b) {
   const int len = p.lens[b];
   w.kv_len = held_len(len, p.page_shift, p.max_pages);
   if (len > w.kv_len && len > 0) atomicExch(p.status, kDevBadPage);
-  w.rows = static_cast<int64_t>(w.q_len) * p.g;
-  if (w.rows < p.row_lo || w.rows > p.row_hi) w.rows = 0;
   return w;
 }
 

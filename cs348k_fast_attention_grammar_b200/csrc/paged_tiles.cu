@@ -8,8 +8,9 @@
 // so one tile's products run while the other's softmax does.  Warp roles (384
 // threads, one CTA per SM):
 //   warps 0-3, 4-7  softmax of tile 0 and 1 (a thread = a row = a TMEM lane)
-//   warp 8          loads: Q tiles once per unit, K and V by pages into a ring
+//   warp 8          loads: Q tiles once per unit, K by pages into a ring
 //   warp 9          TMEM allocation and the single thread that issues tcgen05.mma
+//   warp 10         loads V by pages into the ring
 // S_t lives in TMEM columns [128 t, 128 t + 128), P_t over its first half as 16-bit
 // pairs, O_t at 256 + D t.  The kernel is bound by the chain S -> softmax -> P of
 // each tile, about 2900 clocks per 128 keys for 2048 clocks of tensor work.
@@ -41,7 +42,7 @@ namespace {
 constexpr int kRows = 128;           // rows of a tile (TMEM lanes)
 constexpr int kKeys = 128;           // keys of a block
 constexpr int kThreads = 384;
-constexpr int kRegsCtrl = 56, kRegsSoftmax = 224;
+constexpr int kRegsCtrl = 72, kRegsSoftmax = 216;
 static_assert(128 * kRegsCtrl + 256 * kRegsSoftmax <= 384 * 168,
               "the register split exceeds the launch's pool");
 constexpr int kUnitsPerSm = 4;       // from here on units are not split
@@ -84,7 +85,7 @@ __host__ __device__ constexpr int64_t up128(int64_t n) { return (n + 127) / 128 
 // Work
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ int units_of(const TileParams& p, const SeqWork& w) {
-  return w.rows == 0 ? 0 : (w.q_len + 2 * p.tq - 1) / (2 * p.tq);
+  return (w.q_len + 2 * p.tq - 1) / (2 * p.tq);
 }
 // Key blocks that the tokens [tok0, tok0 + n) of the sequence see.
 __device__ __forceinline__ int blocks_of(const TileParams& p, const SeqWork& w, int tok0, int n) {
@@ -283,7 +284,9 @@ struct Cfg {
   static constexpr int kStages = D == 128 ? 4 : 8;       // K and V tiles in the ring
   static constexpr int kQOff = 0;
   static constexpr int kKVOff = 2 * kTileBytes;
-  static constexpr int kBarOff = kKVOff + kStages * kTileBytes;
+  static constexpr int kOutOff = kKVOff + kStages * kTileBytes;   // a warp's 32 x 32 outputs
+  static constexpr int kOutRow = 80;                              // bytes, 16 of them padding
+  static constexpr int kBarOff = kOutOff + 8 * 32 * kOutRow;
   // q, kv_full[], kv_empty[], s_full[2], p_full[2], o_full[2], drain, p_half[2],
   // q_empty, unit_full[2], unit_empty[2], v_raw
   static constexpr int kNumBars = 1 + 2 * kStages + 15;
@@ -348,7 +351,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(bar_p_half(t), kRows);
       mbar_init(bar_o_full(t), 1);
       mbar_init(bar_unit_full(t), 1);
-      mbar_init(bar_unit_empty(t), 1 + 8);
+      mbar_init(bar_unit_empty(t), 1 + 1 + 8);
     }
     mbar_init(bar_drain, 1);
     mbar_init(bar_q_empty, 1);
@@ -375,27 +378,85 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem = *tmem_slot;
   grid_dependency_wait();               // the plan is complete
 
+  int raws = 0;         // V tiles whose end was zeroed
+
   // Warp-uniform bounded wait: every lane waits, and the warp goes on only if
   // all saw the phase, so that giving up never splits a warp.
   auto wwait = [&](uint32_t bar, uint32_t parity) {
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, p.status));
   };
 
+  // K (kv = 0) or V (1) tiles of the n key blocks from blk0, by one warp: one
+  // lane per page.  Block i of the CTA goes to ring position 2 i + kv.
+  auto load_keys = [&](const CUtensorMap* map, int kv, int b, int h, int kv_len, int blk0, int n,
+                       int& blocks) {
+    const uint64_t policy = l2_policy_evict_last();
+    const int boxes = kKeys / p.box_rows;
+    const int in_page = (1 << p.page_shift) - p.box_rows;      // mask of a box's row in its page
+    const uint32_t box_bytes = static_cast<uint32_t>(p.box_rows) * 128u;
+    const int32_t* trow = p.table + b * p.table_stride;
+    // Page of this lane's box of block j; one outside the cache reads as zeros.
+    auto page_for = [&](int j) {
+      const int key = j * kKeys + lane * p.box_rows;
+      if (lane >= boxes || key >= kv_len) return p.pages;
+      const int pg = page_at(trow, key, p.page_shift, p.max_pages, p.pages);
+      if (pg < 0) atomicExch(p.status, kDevBadPage);
+      return pg < 0 ? p.pages : pg;
+    };
+    int page = page_for(blk0);
+    for (int j = blk0; j < blk0 + n; ++j, ++blocks) {
+      const int page_next = j + 1 < blk0 + n ? page_for(j + 1) : 0;
+      const int keys = min(kKeys, kv_len - j * kKeys);          // > 0
+      const int used = (keys + p.box_rows - 1) / p.box_rows;
+      const int pos = 2 * blocks + kv;
+      const int s = pos % C::kStages;
+      const uint32_t phase = (pos / C::kStages) & 1;
+      if (!wwait(bar_kv_empty(s), phase ^ 1u)) return false;
+      const uint32_t dst = sKV + s * C::kTileBytes;
+      // A V tile that ends inside is handed on after its end is zeroed.
+      const bool cut = kv == 1 && keys < kKeys;
+      const uint32_t bar = cut ? bar_v_raw : bar_kv_full(s);
+      if (lane == 0) mbar_arrive_expect_tx(bar, used * box_bytes * (D / 64));
+      __syncwarp();
+      if (lane < used) {
+#pragma unroll
+        for (int dk = 0; dk < D / 64; ++dk)
+          tma_load_4d(dst + dk * 16384 + lane * box_bytes, map, bar, dk * 64,
+                      (j * kKeys) & in_page, h, page, policy);
+      }
+      if (cut) {
+        if (!wwait(bar_v_raw, raws & 1)) return false;
+        ++raws;
+        uint8_t* v = gbase + C::kKVOff + s * C::kTileBytes;
+        for (int i = keys * 8 + lane; i < kKeys * 8; i += 32)
+#pragma unroll
+          for (int dk = 0; dk < D / 64; ++dk)
+            *reinterpret_cast<uint4*>(v + dk * 16384 + i * 16) = make_uint4(0, 0, 0, 0);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_kv_full(s));
+      }
+      page = page_next;
+    }
+    return true;
+  };
+  // On the way out: waits for a loader's last copies.
+  auto land = [&](int kv, int blocks) {
+    if (kv == 1) last_wait(bar_v_raw, raws & 1);
+    for (int i = max(0, blocks - C::kStages / 2); i < blocks; ++i)
+      last_wait(bar_kv_full((2 * i + kv) % C::kStages), ((2 * i + kv) / C::kStages) & 1);
+  };
+
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsCtrl) : "memory");
     if (warp == 8) {
-      // =================== loads ===================
-      const uint64_t pol_q = l2_policy_evict_first();
-      const uint64_t pol_kv = l2_policy_evict_last();
+      // =================== loads of Q and K ===================
       const bool split = p.plan[kSplit] != 0;
       int64_t next = split ? p.first[blockIdx.x] : static_cast<int>(blockIdx.x);
       const int64_t stop = split ? p.first[blockIdx.x + 1] : p.plan[kUnits];
-      const int boxes = kKeys / p.box_rows;
-      const int page_mask = (1 << p.page_shift) - 1;
-      const uint32_t box_bytes = static_cast<uint32_t>(p.box_rows) * 128u;
-      int issued = 0;       // K and V tiles, over all pieces (ring position)
+      const uint64_t pol_q = l2_policy_evict_first();
+      int blocks = 0;       // K tiles issued, over all pieces
       int uc = 0;           // pieces with keys
-      int raws = 0;         // V tiles whose end was zeroed
       for (int take = 0;; ++take) {
         const int us = take & 1;
         if (take >= 2 && !wwait(bar_unit_empty(us), ((take >> 1) - 1) & 1)) break;
@@ -433,63 +494,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                               x.q_begin + x.tok0 + t * p.tq, x.h, pol_q);
           }
           ++uc;
-          const int32_t* trow = p.table + x.b * p.table_stride;
-          // Page of this lane's box of block j; one outside the cache reads as zeros.
-          auto page_for = [&](int j) {
-            const int key = j * kKeys + lane * p.box_rows;
-            if (lane >= boxes || key >= x.kv_len) return p.pages;
-            const int pg = page_at(trow, key, p.page_shift, p.max_pages, p.pages);
-            if (pg < 0) atomicExch(p.status, kDevBadPage);
-            return pg < 0 ? p.pages : pg;
-          };
-          int page = page_for(x.blk0);
-          bool ok = true;
-          for (int j = x.blk0; ok && j < x.blk0 + n; ++j) {
-            const int page_next = j + 1 < x.blk0 + n ? page_for(j + 1) : 0;
-            const int keys = min(kKeys, x.kv_len - j * kKeys);          // > 0
-            const int used = (keys + p.box_rows - 1) / p.box_rows;
-            const int in = (j * kKeys) & page_mask & ~(p.box_rows - 1);
-#pragma unroll
-            for (int kv = 0; kv < 2; ++kv) {
-              const int s = issued % C::kStages;
-              if (!wwait(bar_kv_empty(s), ((issued / C::kStages) & 1) ^ 1u)) {
-                ok = false;
-                break;
-              }
-              const uint32_t dst = sKV + s * C::kTileBytes;
-              // A V tile that ends inside is handed on after its end is zeroed.
-              const bool cut = kv == 1 && keys < kKeys;
-              const uint32_t bar = cut ? bar_v_raw : bar_kv_full(s);
-              if (lane == 0) mbar_arrive_expect_tx(bar, used * box_bytes * (D / 64));
-              __syncwarp();
-              if (lane < used) {
-                const void* map = kv ? static_cast<const void*>(&tmV)
-                                     : static_cast<const void*>(&tmK);
-#pragma unroll
-                for (int dk = 0; dk < D / 64; ++dk)
-                  tma_load_4d(dst + dk * 16384 + lane * box_bytes, map, bar, dk * 64, in, x.h,
-                              page, pol_kv);
-              }
-              ++issued;
-              if (cut) {
-                if (!wwait(bar_v_raw, raws & 1)) {
-                  ok = false;
-                  break;
-                }
-                ++raws;
-                uint8_t* v = gbase + C::kKVOff + s * C::kTileBytes;
-                for (int i = keys * 8 + lane; i < kKeys * 8; i += 32)
-#pragma unroll
-                  for (int dk = 0; dk < D / 64; ++dk)
-                    *reinterpret_cast<uint4*>(v + dk * 16384 + i * 16) = make_uint4(0, 0, 0, 0);
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(bar_kv_full(s));
-              }
-            }
-            page = page_next;
-          }
-          if (!ok) break;
+          if (!load_keys(&tmK, 0, x.b, x.h, x.kv_len, x.blk0, n, blocks)) break;
         }
         if (split) {
           ++next;
@@ -502,10 +507,23 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (*abort_flag && lane == 0) {
         // Let the copies in flight land before the CTA exits.
         if (uc > 0) last_wait(bar_q, (uc - 1) & 1);
-        last_wait(bar_v_raw, raws & 1);
-        for (int i = max(0, issued - C::kStages); i < issued; ++i)
-          last_wait(bar_kv_full(i % C::kStages), (i / C::kStages) & 1);
+        land(0, blocks);
       }
+      __syncwarp();
+    } else if (warp == 10) {
+      // =================== loads of V ===================
+      int blocks = 0;
+      for (int uc = 0;; ++uc) {
+        const int us = uc & 1;
+        if (!wwait(bar_unit_full(us), (uc >> 1) & 1)) break;
+        const int b = ring[us].b, h = ring[us].h, kv_len = ring[us].kv_len;
+        const int blk0 = ring[us].blk0, n = max(ring[us].nt[0], ring[us].nt[1]);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_unit_empty(us));
+        if (h < 0) break;
+        if (n > 0 && !load_keys(&tmV, 1, b, h, kv_len, blk0, n, blocks)) break;
+      }
+      if (*abort_flag && lane == 0) land(1, blocks);
       __syncwarp();
     } else if (warp == 9) {
       // =================== MMA issuer ===================
@@ -610,24 +628,25 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t tO = tmem + lane_off + C::col_o(t);
     const float sl2 = p.scale_log2;
     const uint64_t sl2x2 = f2_pack(sl2, sl2);
-    const int row_tok = row / p.g, row_head = row - row_tok * p.g;
+    const int row_tok = row / p.g;
     bool ok = true;
     int sb = 0;   // key blocks of this tile in earlier pieces (S phases)
     int ou = 0;   // earlier pieces in which this tile had keys (O phases)
     for (int uc = 0; ok; ++uc) {
       const int us = uc & 1;
       if (!wwait(bar_unit_full(us), (uc >> 1) & 1)) break;
-      const int h = ring[us].h, q_begin = ring[us].q_begin, q_len = ring[us].q_len;
-      const int kv_len = ring[us].kv_len, blk0 = ring[us].blk0, slot = ring[us].slot;
-      const int tok_t = ring[us].tok0 + t * p.tq, nt = ring[us].nt[t];
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar_unit_empty(us));
-      if (h < 0) break;
-      const int tok = tok_t + row_tok;
-      const bool live = row_tok < p.tq && tok < q_len;
+      if (ring[us].h < 0) break;
+      const int kv_len = ring[us].kv_len, blk0 = ring[us].blk0, nt = ring[us].nt[t];
       // Keys [0, lim) are seen by this row; no row of the tile sees fewer than lim0.
-      const int lim0 = p.causal ? kv_len - q_len + tok_t + 1 : kv_len;
-      const int lim = p.causal && live ? lim0 + row_tok : kv_len;
+      int lim = kv_len, lim0 = kv_len;
+      bool any_live;
+      {
+        const int tok_t = ring[us].tok0 + t * p.tq, q_len = ring[us].q_len;
+        const bool live = row_tok < p.tq && tok_t + row_tok < q_len;
+        if (p.causal) lim0 = kv_len - q_len + tok_t + 1;
+        if (p.causal && live) lim = lim0 + row_tok;
+        any_live = __any_sync(0xffffffffu, live);
+      }
       float m_ref = -INFINITY;   // reference maximum (scaled, log2 domain)
       float l = 0.f;             // sum of exp2(s * sl2 - m_ref)
       for (int j = 0; j < nt; ++j) {
@@ -636,6 +655,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           break;
         }
         tc_fence_after();
+        if (!any_live) {         // rows of no token: whatever their P holds stays in their O
+          mbar_arrive(bar_p_half(t));
+          mbar_arrive(bar_p_full(t));
+          continue;
+        }
         uint32_t sr[128];
         tmem_ld128_wait(tS, sr);
         const int k0 = (blk0 + j) * kKeys;
@@ -720,9 +744,21 @@ __global__ void __launch_bounds__(kThreads, 1)
       // (l is NaN where the scores were, and stays so.)
       if (m_ref == -INFINITY && l == l) l = 0.f;
       const float inv = l == 0.f ? 0.f : 1.f / l;
+      const int h = ring[us].h, q_begin = ring[us].q_begin, slot = ring[us].slot;
+      const int tok = ring[us].tok0 + t * p.tq + row_tok;
+      const bool live = row_tok < p.tq && tok < ring[us].q_len;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar_unit_empty(us));
       if (slot < 0) {
-        uint16_t* dst = static_cast<uint16_t*>(p.o) + static_cast<int64_t>(q_begin + tok) * p.o_st +
-                        static_cast<int64_t>(h * p.g + row_head) * p.o_sh;
+        // 32 x 32 outputs at a time through shared memory, so that a store
+        // covers 64 bytes of each of 8 rows instead of 16 of 32.
+        uint8_t* stage = gbase + C::kOutOff + warp * 32 * C::kOutRow;
+        const int64_t off = live ? static_cast<int64_t>(q_begin + tok) * p.o_st +
+                                       static_cast<int64_t>(h * p.g + row - row_tok * p.g) * p.o_sh
+                                 : -1;
+        int64_t to[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) to[i] = __shfl_sync(0xffffffffu, off, i * 8 + lane / 4);
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) {
           uint32_t o[32];
@@ -732,38 +768,45 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int e = 0; e < 32; ++e) o[e] = 0u;
           }
-          if (live) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              if (c * 32 + e * 8 >= p.D) continue;
-              uint32_t w[4];
+          for (int e = 0; e < 4; ++e) {
+            uint32_t w[4];
 #pragma unroll
-              for (int i = 0; i < 4; ++i)
-                w[i] = pack_16x2<F16>(__uint_as_float(o[e * 8 + 2 * i]) * inv,
-                                      __uint_as_float(o[e * 8 + 2 * i + 1]) * inv);
-              *reinterpret_cast<uint4*>(dst + c * 32 + e * 8) = make_uint4(w[0], w[1], w[2], w[3]);
-            }
+            for (int i = 0; i < 4; ++i)
+              w[i] = pack_16x2<F16>(__uint_as_float(o[e * 8 + 2 * i]) * inv,
+                                    __uint_as_float(o[e * 8 + 2 * i + 1]) * inv);
+            *reinterpret_cast<uint4*>(stage + lane * C::kOutRow + e * 16) =
+                make_uint4(w[0], w[1], w[2], w[3]);
           }
+          __syncwarp();
+          const int d = c * 32 + (lane & 3) * 8;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint4 v = *reinterpret_cast<const uint4*>(
+                stage + (i * 8 + lane / 4) * C::kOutRow + (lane & 3) * 16);
+            if (to[i] >= 0 && d < p.D)
+              *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.o) + to[i] + d) = v;
+          }
+          __syncwarp();
         }
       } else {
+        // Four channels of 32 rows side by side: 512 bytes per store.
         float* part = p.part + static_cast<int64_t>(slot) * C::kSlot;
-        const int r = t * kRows + row;
         if (nt > 0) {
 #pragma unroll
           for (int c = 0; c < D / 32; ++c) {
             uint32_t o[32];
             tmem_ld32_wait(tO + c * 32, o);
-            if (live) {
-              uint4* dst = reinterpret_cast<uint4*>(part + r * D + c * 32);
+            uint4* dst = reinterpret_cast<uint4*>(part) + (t * (D / 4) + c * 8) * kRows + row;
 #pragma unroll
-              for (int e = 0; e < 8; ++e)
-                dst[e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
-            }
+            for (int e = 0; e < 8; ++e)
+              if (live)
+                dst[e * kRows] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
           }
         }
         if (live) {
-          part[2 * kRows * D + r] = m_ref;
-          part[2 * kRows * D + 2 * kRows + r] = l;
+          part[2 * kRows * D + t * kRows + row] = m_ref;
+          part[2 * kRows * D + 2 * kRows + t * kRows + row] = l;
         }
       }
       sb += nt;
@@ -779,68 +822,79 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // Adds up the parts of the unit that begins in CTA blockIdx.x's range and goes
-// on behind it; one warp per row.  Bound by HBM: each part is read once.
+// on behind it: a CTA takes 32 rows (a lane each), a warp D / 8 channels of them.
+// Bound by HBM: each part is read once.
 constexpr int kJoinWarps = 8;
 template <int D, bool F16>
 __global__ void __launch_bounds__(32 * kJoinWarps)
     paged_tiles_join(const TileParams p) {
   using C = Cfg<D>;
+  constexpr int E = D / 4 / kJoinWarps;               // groups of four channels of a warp
+  constexpr int kRowBytes = D * 2 + 16;
+  __shared__ __align__(16) uint8_t s_out[32 * kRowBytes];
+  __shared__ int64_t s_off[32];
   grid_dependency_wait();
   grid_dependents_launch();
   if (p.plan[kSplit] == 0) return;
   const int2 jn = p.join[blockIdx.x];
   if (jn.y == 0) return;
-  const int lane = threadIdx.x & 31;
-  const int r = blockIdx.y * kJoinWarps + (threadIdx.x >> 5);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const Piece& x = p.pieces[jn.x];
-  const int t = r / kRows, row_tok = (r - t * kRows) / p.g;
-  const int head = r - t * kRows - row_tok * p.g;
+  const int t = blockIdx.y / (kRows / 32);
+  const int row = (blockIdx.y % (kRows / 32)) * 32 + lane;    // of the tile
+  const int row_tok = row / p.g;
   const int tok = x.tok0 + t * p.tq + row_tok;
-  if (row_tok >= p.tq || tok >= x.q_len) return;
+  const bool live = row_tok < p.tq && tok < x.q_len;
+  if (!__any_sync(0xffffffffu, live)) return;                 // (the same in every warp)
   auto part = [&](int i) {
     return p.part + static_cast<int64_t>(2 * (blockIdx.x + i) + (i == 0 ? 1 : 0)) * C::kSlot;
   };
+  const int at_m = 2 * kRows * D + t * kRows + row, at_l = at_m + 2 * kRows;
   float top = -INFINITY;
-  for (int i = lane; i < jn.y; i += 32) top = fmaxf(top, part(i)[2 * kRows * D + r]);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  constexpr int E = D / 32;
-  float sum = 0.f, acc[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e) acc[e] = 0.f;
+  if (live)
 #pragma unroll 4
-  for (int i = 0; i < jn.y; ++i) {
-    const float* s = part(i);
-    const float mi = s[2 * kRows * D + r], li = s[2 * kRows * D + 2 * kRows + r];
-    if (mi == -INFINITY) {              // saw none of these keys: O was not written
-      sum += li;
-      continue;
+    for (int i = 0; i < jn.y; ++i) top = fmaxf(top, part(i)[at_m]);
+  float sum = 0.f;
+  float4 acc[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) acc[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (live)
+#pragma unroll 4
+    for (int i = 0; i < jn.y; ++i) {
+      const float* s = part(i);
+      const float mi = s[at_m], li = s[at_l];
+      if (mi == -INFINITY) {            // saw none of these keys: O was not written
+        sum += li;
+        continue;
+      }
+      const float al = ex2_approx(mi - top);
+      sum += li * al;
+      const float4* o = reinterpret_cast<const float4*>(s) + (t * (D / 4) + warp * E) * kRows + row;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const float4 v = o[e * kRows];
+        acc[e].x += v.x * al;
+        acc[e].y += v.y * al;
+        acc[e].z += v.z * al;
+        acc[e].w += v.w * al;
+      }
     }
-    const float al = ex2_approx(mi - top);
-    sum += li * al;
-    if constexpr (E == 4) {
-      const float4 v = *reinterpret_cast<const float4*>(s + r * D + lane * 4);
-      acc[0] += v.x * al;
-      acc[1] += v.y * al;
-      acc[2] += v.z * al;
-      acc[3] += v.w * al;
-    } else {
-      const float2 v = *reinterpret_cast<const float2*>(s + r * D + lane * 2);
-      acc[0] += v.x * al;
-      acc[1] += v.y * al;
-    }
-  }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  uint16_t* dst = static_cast<uint16_t*>(p.o) +
-                  static_cast<int64_t>(x.q_begin + tok) * p.o_st +
-                  static_cast<int64_t>(x.h * p.g + head) * p.o_sh;
-  if (lane * E < p.D) {
-    if constexpr (E == 4)
-      *reinterpret_cast<uint2*>(dst + lane * 4) =
-          make_uint2(pack_16x2<F16>(acc[0] * inv, acc[1] * inv),
-                     pack_16x2<F16>(acc[2] * inv, acc[3] * inv));
-    else
-      *reinterpret_cast<uint32_t*>(dst + lane * 2) = pack_16x2<F16>(acc[0] * inv, acc[1] * inv);
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+    *reinterpret_cast<uint2*>(s_out + lane * kRowBytes + (warp * E + e) * 8) =
+        make_uint2(pack_16x2<F16>(acc[e].x * inv, acc[e].y * inv),
+                   pack_16x2<F16>(acc[e].z * inv, acc[e].w * inv));
+  if (warp == 0)
+    s_off[lane] = live ? static_cast<int64_t>(x.q_begin + tok) * p.o_st +
+                             static_cast<int64_t>(x.h * p.g + row - row_tok * p.g) * p.o_sh
+                       : -1;
+  __syncthreads();
+  for (int i = threadIdx.x; i < 32 * (D / 8); i += 32 * kJoinWarps) {
+    const int r = i / (D / 8), d = (i - r * (D / 8)) * 8;
+    if (s_off[r] >= 0 && d < p.D)
+      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.o) + s_off[r] + d) =
+          *reinterpret_cast<const uint4*>(s_out + r * kRowBytes + d * 2);
   }
 }
 
@@ -905,7 +959,7 @@ int launch_tiles(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap
   rc = launch_after(paged_tiles_kernel<D, F16>, dim3(p.ctas), kThreads, C::kSmemBytes, stream, mq,
                     mk, mv, p);
   if (rc != FA_OK || !split) return rc;
-  return launch_after(paged_tiles_join<D, F16>, dim3(p.ctas, 2 * kRows / kJoinWarps),
+  return launch_after(paged_tiles_join<D, F16>, dim3(p.ctas, 2 * kRows / 32),
                       32 * kJoinWarps, 0, stream, p);
 }
 

@@ -23,8 +23,8 @@
 namespace fa {
 namespace {
 
-constexpr int kRotThreads = 256;
-constexpr int kRotItems = 2;            // items a thread loads ahead of the angles
+constexpr int kRotThreads = 192;
+constexpr int kRotBatches = 4;          // goes of a CTA over its items
 constexpr int kRotMaxRows = 64;         // rows of one CTA
 constexpr int kRotMaxAngles = 2048;     // angles of one CTA (16 KiB of shared memory)
 
@@ -155,7 +155,7 @@ struct Item {
 
 // APPEND: rows are packed new tokens, keys and values go to their pages.
 template <int TYPE, bool APPEND, bool INTERLEAVED>
-__global__ void __launch_bounds__(kRotThreads)
+__global__ void __launch_bounds__(kRotThreads, 8)
     rotary_kernel(const RotParams p) {
   constexpr int kSize = Elem<TYPE>::kSize;
   constexpr int V = 16 / kSize;
@@ -202,9 +202,10 @@ __global__ void __launch_bounds__(kRotThreads)
       x.off1 = (half + chunk * V) * kSize;
       x.angle = x.row * half + chunk * (INTERLEAVED ? V / 2 : V);
     } else {
-      const int c0 = q.rotate ? p.ang.R + 2 * (chunk - rot_items) * V : 2 * chunk * V;
+      const int c0 = q.rotate ? p.ang.R + (chunk - rot_items) * V : chunk * V;
+      const int c1 = c0 + (q.items - (q.rotate ? rot_items : 0)) * V;
       x.off0 = c0 * kSize;
-      x.off1 = c0 + V < p.D ? (c0 + V) * kSize : -1;
+      x.off1 = c1 < p.D ? c1 * kSize : -1;
       x.angle = -1;
     }
     return x;
@@ -214,16 +215,13 @@ __global__ void __launch_bounds__(kRotThreads)
     if (x.off1 >= 0) u1 = *reinterpret_cast<const uint4*>(x.src + x.off1);
   };
 
-  // The first items' loads are in flight while places and angles are found.
-  uint4 a[kRotItems], c[kRotItems];
-  Item item[kRotItems];
-#pragma unroll
-  for (int u = 0; u < kRotItems; ++u) {
-    const unsigned it = threadIdx.x + u * kRotThreads;
-    if (it < total) {
-      item[u] = locate(it);
-      load(item[u], a[u], c[u]);
-    }
+  // The first item's load is in flight while places and angles are found.
+  unsigned it = threadIdx.x;
+  uint4 a, c;
+  Item item;
+  if (it < total) {
+    item = locate(it);
+    load(item, a, c);
   }
   if (APPEND) {
     // Where each row goes: one warp per row.
@@ -313,14 +311,11 @@ __global__ void __launch_bounds__(kRotThreads)
     *reinterpret_cast<uint4*>(dst + x.off0) = pack<TYPE>(f);
     *reinterpret_cast<uint4*>(dst + x.off1) = pack<TYPE>(g);
   };
-#pragma unroll
-  for (int u = 0; u < kRotItems; ++u)
-    if (threadIdx.x + u * kRotThreads < total) finish(item[u], a[u], c[u]);
-  for (unsigned it = threadIdx.x + kRotItems * kRotThreads; it < total; it += kRotThreads) {
-    const Item x = locate(it);
-    uint4 u0, u1;
-    load(x, u0, u1);
-    finish(x, u0, u1);
+  if (it < total) finish(item, a, c);
+  for (it += kRotThreads; it < total; it += kRotThreads) {
+    item = locate(it);
+    load(item, a, c);
+    finish(item, a, c);
   }
 }
 
@@ -338,12 +333,13 @@ int launch_rotary(RotParams& p, int dtype, bool append, bool interleaved, cudaSt
     q.count = q.heads * q.items;
     p.items_per_row += q.count;
   }
-  // Rows per CTA: as many as its threads take in one go, within the shared
-  // memory for their angles, and no more than leave every SM some.
-  int rows = kRotThreads * kRotItems / p.items_per_row;
+  // Rows per CTA: what its threads take in kRotBatches goes (a row's place takes
+  // a chain of loads that the goes share), within the shared memory for their
+  // angles, and no more than leave every SM eight CTAs.
+  int rows = kRotBatches * kRotThreads / p.items_per_row;
   const int sms = sm_count(dev);
-  if (sms > 0 && p.rows < static_cast<int64_t>(rows) * sms)
-    rows = static_cast<int>((p.rows + sms - 1) / sms);
+  if (sms > 0 && p.rows < 8ll * rows * sms)
+    rows = static_cast<int>((p.rows + 8 * sms - 1) / (8 * sms));
   if (half > 0) rows = rows < kRotMaxAngles / half ? rows : kRotMaxAngles / half;
   rows = rows < kRotMaxRows ? rows : kRotMaxRows;
   p.rows_per_cta = rows > 1 ? rows : 1;
