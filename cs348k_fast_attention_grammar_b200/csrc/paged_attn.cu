@@ -8,16 +8,21 @@
 // paged_rows_kernel takes sequences of few rows (a generation step).  It is
 // bound by HBM: two passes' worth of arithmetic per key and row is far below
 // what even warp-level matrix instructions deliver, so the kernel is built
-// around its loads.  A CTA has four warps; per 64-key block each warp owns 16
-// keys, loads their K and V rows with 16-byte asynchronous copies into a ring
-// of its own (no barrier between warps), and keeps its own running maximum, sum
-// and output, joined over the warps when the CTA leaves a tile.
+// around its loads.  A CTA has four warps (more for short tables, below); per
+// 64-key block each warp owns 16 keys, loads their K and V rows with 16-byte
+// asynchronous copies into a ring of its own (no barrier between warps), and
+// keeps its own running maximum, sum and output, joined over the warps when the
+// CTA leaves a tile.
 //
-// The key blocks of all (sequence, key head, row tile) units, one after the
-// other, are cut into equal ranges, one per CTA, whatever the lengths: a unit
-// that crosses a range's border leaves (m, l, O) of its parts in the workspace
-// and paged_rows_join adds them up in the order of the keys, so results do not
-// depend on timing.
+// CTAs work in teams of up to 16 key heads, a head each, that walk the same keys
+// side by side: a cached token's heads lie next to each other, and DRAM is read
+// in longer runs than one head's row (64 sequences of up to 4096 keys, 8 heads of
+// 64: 4127 -> 5344 GB/s; D = 128: 6071 -> 6136).  The key blocks
+// of all (sequence, group of heads, row tile) units, one after the other, are cut
+// into equal ranges, one per team, whatever the lengths: a unit that crosses a
+// range's border leaves (m, l, O) of its parts in the workspace and
+// paged_rows_join adds them up in the order of the keys, so results do not depend
+// on timing.
 #include <cuda_bf16.h>
 
 #include <cmath>
@@ -47,7 +52,7 @@ __device__ __forceinline__ RowWork row_work(const PagedParams& p, int b, int til
   return w;
 }
 __device__ __forceinline__ int64_t weight(const PagedParams& p, const RowWork& w) {
-  return static_cast<int64_t>(w.tiles) * p.Hkv * w.blocks;
+  return static_cast<int64_t>(w.tiles) * (p.Hkv / p.team) * w.blocks;
 }
 
 // The sum of v over the CTA's threads below this one, and over all of them.
@@ -72,7 +77,7 @@ __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* red, int64_t* 
   return before + x - v;
 }
 
-// A CTA's range [start, end) of the key blocks and the sequence that `at`
+// A team's range [start, end) of the key blocks and the sequence that `at`
 // (start, or the range's last block) falls into.
 struct Range {
   int64_t start, end, per;
@@ -81,7 +86,7 @@ struct Range {
 };
 
 template <bool LAST>
-__device__ __forceinline__ Range find_range(const PagedParams& p, int cta, int tile_rows) {
+__device__ __forceinline__ Range find_range(const PagedParams& p, int team, int tile_rows) {
   __shared__ int64_t red[kRowWarps];
   __shared__ int64_t s_base;
   __shared__ int s_b;
@@ -100,7 +105,7 @@ __device__ __forceinline__ Range find_range(const PagedParams& p, int cta, int t
     total += sum;
   }
   r.per = max(static_cast<int64_t>(p.min_blocks), (total + p.ctas - 1) / p.ctas);
-  r.start = min(total, r.per * cta);
+  r.start = min(total, r.per * team);
   r.end = min(total, r.start + r.per);
   if (threadIdx.x == 0) s_b = p.B;
   __syncthreads();
@@ -169,23 +174,35 @@ __device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4],
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-template <int DT, int MT>
+// How a launch cuts its work: ranges of key blocks for teams of CTAs, joined
+// afterwards; a CTA per sequence, head and row tile; the same with more warps,
+// for fewer CTAs than SMs, where a warp's chain of 16-key steps (about 900 clocks
+// each with one warp per scheduler) is what a call waits for.
+enum Cut { kSplit, kWhole, kWholeWide };
+
+template <int DT, int MT, Cut CUT = kSplit>
 struct RowCfg {
   static constexpr int kRows = 16 * MT;
-  static constexpr int kStages = 3;
+  static constexpr int kWarps = CUT == kWholeWide ? (DT == 64 ? 16 : 8) : kRowWarps;
+  static constexpr int kThreads = 32 * kWarps;
+  static constexpr int kStep = 16 * kWarps;              // keys of the CTA's steps
+  // Ring steps by shared memory (CTAs per SM also by registers).
+  static constexpr int kStages = DT == 64 && MT == 2 ? 6 : 3;
+  static constexpr int kCtasPerSm = CUT == kWholeWide ? 1 : DT == 64 && MT == 1 ? 4 : 2;
   static constexpr int kTile = 16 * DT * 2;              // 16 keys of K or of V
   static constexpr int kStage = 2 * kTile;
   static constexpr int kWarp = kStages * kStage;
-  static constexpr int kRing = kRowWarps * kWarp;
-  static constexpr int kSmem = kRing + 2 * kRowWarps * kRows * 4;   // + m, l of each warp
+  static constexpr int kRing = kWarps * kWarp;
+  static constexpr int kSmem = kRing + 2 * kWarps * kRows * 4;   // + m, l of each warp
   static constexpr int kSlot = kRows * (DT + 2);         // floats of a partial result
-  static_assert(kRowWarps * kRows * DT * 4 <= kRing, "the joined output reuses the ring");
+  static_assert(kWarps * kRows * DT * 4 <= kRing, "the joined output reuses the ring");
 };
 
-template <int DT, int MT, bool F16>
-__global__ void __launch_bounds__(kRowThreads)
+template <int DT, int MT, bool F16, Cut CUT>
+__global__ void __launch_bounds__(RowCfg<DT, MT, CUT>::kThreads, RowCfg<DT, MT, CUT>::kCtasPerSm)
     paged_rows_kernel(const PagedParams p) {
-  using C = RowCfg<DT, MT>;
+  using C = RowCfg<DT, MT, CUT>;
+  constexpr bool WHOLE = CUT != kSplit;   // teams of all heads, a sequence each
   constexpr int CH = DT / 8;            // 16-byte chunks of a row
   constexpr int RPI = 32 / CH;          // rows one warp-wide copy covers
   extern __shared__ __align__(128) uint8_t smem[];
@@ -195,10 +212,17 @@ __global__ void __launch_bounds__(kRowThreads)
   const uint32_t ring = smem_u32(smem) + warp * C::kWarp;
   float* s_o = reinterpret_cast<float*>(smem);
   float* s_m = reinterpret_cast<float*>(smem + C::kRing);
-  float* s_l = s_m + kRowWarps * C::kRows;
+  float* s_l = s_m + C::kWarps * C::kRows;
 
-  const Range rg = find_range<false>(p, blockIdx.x, C::kRows);
-  if (rg.start >= rg.end) return;
+  Range rg = {};
+  int tile = 0;                         // whole units: this CTA's row tile
+  if (WHOLE) {
+    rg.b = blockIdx.x / p.team / p.tile_ctas;
+    tile = blockIdx.x / p.team % p.tile_ctas;
+  } else {
+    rg = find_range<false>(p, blockIdx.x / p.team, C::kRows);
+    if (rg.start >= rg.end) return;
+  }
   const int page_mask = (1 << p.page_shift) - 1;
   const int crow = lane / CH, cchunk = lane % CH;
   const bool cin = cchunk * 8 < p.D;
@@ -208,14 +232,81 @@ __global__ void __launch_bounds__(kRowThreads)
   int b = rg.b;
   int64_t base = rg.base, cur = rg.start;
   RowWork w = row_work(p, b, C::kRows);
+  if (WHOLE) {
+    if (tile >= w.tiles) return;
+    cur = static_cast<int64_t>(tile) * w.blocks;
+    rg.end = cur + w.blocks;
+  }
   while (true) {
     const int64_t in_seq = cur - base;
     const int unit = static_cast<int>(in_seq / w.blocks);
     const int blk0 = static_cast<int>(in_seq - static_cast<int64_t>(unit) * w.blocks);
     const int nblk = static_cast<int>(min(static_cast<int64_t>(w.blocks - blk0), rg.end - cur));
-    const int h = unit / w.tiles;
-    const int row0 = (unit - h * w.tiles) * C::kRows;
+    const int group = unit / w.tiles;
+    const int h = group * p.team + blockIdx.x % p.team;
+    const int row0 = (unit - group * w.tiles) * C::kRows;
     const int rows = min(C::kRows, w.q_len * p.g - row0);      // of this tile
+
+    const int tile_seen = min(w.kv_len, seen_keys(p, w, (row0 + rows - 1) / p.g));
+
+    // This warp's 16-key steps of the blocks: those that some row sees.
+    const int key00 = blk0 * kRowKeys + warp * 16;
+    const int key_end = min(tile_seen, (blk0 + nblk) * kRowKeys);
+    const int steps = key00 < key_end ? (key_end - key00 + C::kStep - 1) / C::kStep : 0;
+    const int32_t* trow = p.table + b * p.table_stride;
+    auto page_of = [&](int s) {
+      if (s >= steps) return 0;
+      const int pg = page_at(trow, key00 + s * C::kStep, p.page_shift, p.max_pages, p.pages);
+      if (pg < 0) atomicExch(p.status, kDevBadPage);
+      return pg;
+    };
+    int ids = page_of(lane), ids_next = page_of(32 + lane);
+    const int64_t kh = (h * p.kc_h + crow * p.kc_r + cchunk * 8) * 2;
+    const int64_t vh = (h * p.vc_h + crow * p.vc_r + cchunk * 8) * 2;
+    const int64_t kstep = p.kc_r * (2 * RPI), vstep = p.vc_r * (2 * RPI);
+    auto issue = [&](int s) {
+      if (s < steps) {
+        if (s > 0 && (s & 31) == 0) {
+          ids = ids_next;
+          ids_next = page_of(s + 32 + lane);
+        }
+        const int pg = __shfl_sync(0xffffffffu, ids, s & 31);
+        const int key0 = key00 + s * C::kStep;
+        const int in = key0 & page_mask;
+        const uint32_t st = ring + (s % C::kStages) * C::kStage;
+        if (pg >= 0 && key0 + 16 <= w.kv_len && p.D == DT) {
+          const char* ks = kc + kh + (pg * p.kc_p + in * p.kc_r) * 2;
+          const char* vs = vc + vh + (pg * p.vc_p + in * p.vc_r) * 2;
+#pragma unroll
+          for (int it = 0; it < 16 / RPI; ++it) {
+            const int r = it * RPI + crow;
+            const uint32_t at = st + r * (DT * 2) + ((cchunk ^ (r & 7)) * 16);
+            cp_async16(at, ks, 16);
+            cp_async16(at + C::kTile, vs, 16);
+            ks += kstep;
+            vs += vstep;
+          }
+        } else {
+          // The sequence's last keys, a page outside the cache, channels behind
+          // D: zeros where there is nothing to copy.
+          const int64_t pgc = pg < 0 ? 0 : pg;
+          const char* ks = kc + kh + (pgc * p.kc_p + in * p.kc_r) * 2;
+          const char* vs = vc + vh + (pgc * p.vc_p + in * p.vc_r) * 2;
+          const int left = pg < 0 || !cin ? 0 : w.kv_len - key0 - crow;
+#pragma unroll
+          for (int it = 0; it < 16 / RPI; ++it) {
+            const int r = it * RPI + crow;
+            const uint32_t at = st + r * (DT * 2) + ((cchunk ^ (r & 7)) * 16);
+            const bool in_seq = it * RPI < left;
+            cp_async16(at, in_seq ? ks + it * kstep : kc, in_seq ? 16 : 0);
+            cp_async16(at + C::kTile, in_seq ? vs + it * vstep : vc, in_seq ? 16 : 0);
+          }
+        }
+      }
+      cp_async_commit();
+    };
+#pragma unroll
+    for (int s = 0; s < C::kStages - 1; ++s) issue(s);
 
     // Q fragments and what each of this thread's rows sees.
     uint32_t qf[MT][DT / 16][4];
@@ -240,7 +331,6 @@ __global__ void __launch_bounds__(kRowThreads)
                 in && d < p.D ? *reinterpret_cast<const uint32_t*>(src + d) : 0u;
           }
       }
-    const int tile_seen = min(w.kv_len, seen_keys(p, w, (row0 + rows - 1) / p.g));
 
     float m[MT][2], l[MT][2], o[MT][DT / 8][4];
 #pragma unroll
@@ -253,55 +343,12 @@ __global__ void __launch_bounds__(kRowThreads)
         for (int e = 0; e < 4; ++e) o[mt][n][e] = 0.f;
     }
 
-    // This warp's 16-key steps of the blocks: those that some row sees.
-    const int key00 = blk0 * kRowKeys + warp * 16;
-    const int steps = key00 < tile_seen
-                          ? min(nblk, (tile_seen - key00 + kRowKeys - 1) / kRowKeys)
-                          : 0;
-    const int32_t* trow = p.table + b * p.table_stride;
-    auto page_of = [&](int s) {
-      if (s >= steps) return 0;
-      const int pg = page_at(trow, key00 + s * kRowKeys, p.page_shift, p.max_pages, p.pages);
-      if (pg < 0) atomicExch(p.status, kDevBadPage);
-      return pg;
-    };
-    int ids = page_of(lane), ids_next = page_of(32 + lane);
-    const int64_t kh = (h * p.kc_h + crow * p.kc_r + cchunk * 8) * 2;
-    const int64_t vh = (h * p.vc_h + crow * p.vc_r + cchunk * 8) * 2;
-    auto issue = [&](int s) {
-      if (s < steps) {
-        if (s > 0 && (s & 31) == 0) {
-          ids = ids_next;
-          ids_next = page_of(s + 32 + lane);
-        }
-        const int pg = __shfl_sync(0xffffffffu, ids, s & 31);
-        const int key0 = key00 + s * kRowKeys;
-        const int in = key0 & page_mask;
-        const int64_t pgc = pg < 0 ? 0 : pg;
-        const char* ks = kc + kh + (pgc * p.kc_p + in * p.kc_r) * 2;
-        const char* vs = vc + vh + (pgc * p.vc_p + in * p.vc_r) * 2;
-        const int left = pg < 0 || !cin ? 0 : w.kv_len - key0 - crow;   // rows it - RPI < left
-        const uint32_t st = ring + (s % C::kStages) * C::kStage;
-#pragma unroll
-        for (int it = 0; it < 16 / RPI; ++it) {
-          const int r = it * RPI + crow;
-          const uint32_t at = st + r * (DT * 2) + ((cchunk ^ (r & 7)) * 16);
-          const int n = it * RPI < left ? 16 : 0;
-          cp_async16(at, ks + (n ? it * RPI * p.kc_r * 2 : 0), n);
-          cp_async16(at + C::kTile, vs + (n ? it * RPI * p.vc_r * 2 : 0), n);
-        }
-      }
-      cp_async_commit();
-    };
-#pragma unroll
-    for (int s = 0; s < C::kStages - 1; ++s) issue(s);
-
     for (int s = 0; s < steps; ++s) {
       cp_async_wait<C::kStages - 2>();
       __syncwarp();
       issue(s + C::kStages - 1);
       const uint32_t st = ring + (s % C::kStages) * C::kStage;
-      const int key0 = key00 + s * kRowKeys;
+      const int key0 = key00 + s * C::kStep;
       // S = Q K^T for 16 keys: two 8-key column tiles.
       float sc[MT][2][4];
 #pragma unroll
@@ -319,6 +366,7 @@ __global__ void __launch_bounds__(kRowThreads)
           ldsm4(row + (((kk * 2 + ((lane >> 3) & 1)) ^ (r & 7)) * 16), kf);
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt) {
+            if (mt * 16 >= rows) continue;
             mma_16816<F16>(sc[mt][0], qf[mt][kk], kf[0], kf[1]);
             mma_16816<F16>(sc[mt][1], qf[mt][kk], kf[2], kf[3]);
           }
@@ -330,6 +378,7 @@ __global__ void __launch_bounds__(kRowThreads)
       uint32_t pf[MT][4];
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
+        if (mt * 16 >= rows) continue;
         float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
         for (int n = 0; n < 2; ++n)
@@ -381,6 +430,7 @@ __global__ void __launch_bounds__(kRowThreads)
           ldsm4_t(row + (((nn * 2 + (lane >> 4)) ^ (r & 7)) * 16), vf);
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt) {
+            if (mt * 16 >= rows) continue;
             mma_16816<F16>(o[mt][2 * nn], pf[mt], vf[0], vf[1]);
             mma_16816<F16>(o[mt][2 * nn + 1], pf[mt], vf[2], vf[3]);
           }
@@ -410,7 +460,7 @@ __global__ void __launch_bounds__(kRowThreads)
         const int r = mt * 16 + hf * 8 + lane / 4;
         float top = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < kRowWarps; ++i) top = fmaxf(top, s_m[i * C::kRows + r]);
+        for (int i = 0; i < C::kWarps; ++i) top = fmaxf(top, s_m[i * C::kRows + r]);
         const float al = m[mt][hf] == -INFINITY ? 0.f : ex2_approx(m[mt][hf] - top);
 #pragma unroll
         for (int n = 0; n < DT / 8; ++n)
@@ -420,14 +470,14 @@ __global__ void __launch_bounds__(kRowThreads)
     __syncthreads();
     const bool first = blk0 == 0, last = blk0 + nblk == w.blocks;
     float* slot = p.part + static_cast<int64_t>(2 * blockIdx.x + (first ? 1 : 0)) * C::kSlot;
-    for (int i = threadIdx.x; i < rows * (DT / 4); i += kRowThreads) {
+    for (int i = threadIdx.x; i < rows * (DT / 4); i += C::kThreads) {
       const int r = i / (DT / 4), d = (i - r * (DT / 4)) * 4;
       float top = -INFINITY, sum = 0.f;
 #pragma unroll
-      for (int k = 0; k < kRowWarps; ++k) top = fmaxf(top, s_m[k * C::kRows + r]);
+      for (int k = 0; k < C::kWarps; ++k) top = fmaxf(top, s_m[k * C::kRows + r]);
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-      for (int k = 0; k < kRowWarps; ++k) {
+      for (int k = 0; k < C::kWarps; ++k) {
         const float mk = s_m[k * C::kRows + r];
         sum += mk == -INFINITY ? 0.f : s_l[k * C::kRows + r] * ex2_approx(mk - top);
         const float4 x = *reinterpret_cast<const float4*>(s_o + (k * C::kRows + r) * DT + d);
@@ -454,9 +504,16 @@ __global__ void __launch_bounds__(kRowThreads)
       }
     }
     cur += nblk;
-    if (cur >= rg.end) break;
+    if (WHOLE) {
+      tile += p.tile_ctas;
+      if (tile >= w.tiles) break;
+      cur = static_cast<int64_t>(tile) * w.blocks;
+      rg.end = cur + w.blocks;
+    } else if (cur >= rg.end) {
+      break;
+    }
     __syncthreads();        // the ring is free again
-    if (last && unit + 1 == w.tiles * p.Hkv) {
+    if (!WHOLE && last && unit + 1 == w.tiles * (p.Hkv / p.team)) {
       base += weight(p, w);
       do {
         w = row_work(p, ++b, C::kRows);
@@ -465,17 +522,16 @@ __global__ void __launch_bounds__(kRowThreads)
   }
 }
 
-// Adds up the parts of the unit that CTA blockIdx.x's range ends in, when the
-// unit begins in that range and goes on behind it.  One warp per row.
+// Adds up the parts of the unit that the range of CTA blockIdx.x's team ends in,
+// when the unit begins in that range and goes on behind it.  One warp per row.
 template <int DT, int MT, bool F16>
 __global__ void __launch_bounds__(kRowThreads)
     paged_rows_join(const PagedParams p) {
   using C = RowCfg<DT, MT>;
   const int lane = threadIdx.x & 31;
-  const int r = blockIdx.y * kRowWarps + (threadIdx.x >> 5);
   // The row kernel starts when all before it is done, so lengths and tables can
   // be read ahead of the wait for its parts.
-  const Range rg = find_range<true>(p, blockIdx.x, C::kRows);
+  const Range rg = find_range<true>(p, blockIdx.x / p.team, C::kRows);
   grid_dependency_wait();
   grid_dependents_launch();
   if (rg.start >= rg.end) return;
@@ -483,77 +539,89 @@ __global__ void __launch_bounds__(kRowThreads)
   const int unit = static_cast<int>((rg.end - 1 - rg.base) / w.blocks);
   const int64_t us = rg.base + static_cast<int64_t>(unit) * w.blocks, ue = us + w.blocks;
   if (us < rg.start || ue <= rg.end) return;
-  const int h = unit / w.tiles;
-  const int row0 = (unit - h * w.tiles) * C::kRows;
-  if (row0 + r >= w.q_len * p.g) return;
+  const int group = unit / w.tiles;
+  const int h = group * p.team + blockIdx.x % p.team;
+  const int row0 = (unit - group * w.tiles) * C::kRows;
+  const int rows = min(C::kRows, w.q_len * p.g - row0);
   const int parts = 1 + static_cast<int>((ue - rg.end + rg.per - 1) / rg.per);
-  // Part 0 is slot 1 of this CTA, part i slot 0 of the i-th CTA behind it.
+  // Part 0 is slot 1 of this CTA, part i slot 0 of its head's in the i-th team behind.
   auto slot = [&](int i) {
-    return p.part + static_cast<int64_t>(2 * (blockIdx.x + i) + (i == 0 ? 1 : 0)) * C::kSlot;
+    return p.part +
+           static_cast<int64_t>(2 * (blockIdx.x + i * p.team) + (i == 0 ? 1 : 0)) * C::kSlot;
   };
-  float top = -INFINITY;
-  for (int i = lane; i < parts; i += 32) top = fmaxf(top, slot(i)[C::kRows * DT + r]);
+  for (int r = blockIdx.y * kRowWarps + (threadIdx.x >> 5); r < rows; r += gridDim.y * kRowWarps) {
+    float top = -INFINITY;
+    for (int i = lane; i < parts; i += 32) top = fmaxf(top, slot(i)[C::kRows * DT + r]);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  float sum = 0.f;
-  float acc[DT / 32];
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    float sum = 0.f;
+    float acc[DT / 32];
 #pragma unroll
-  for (int e = 0; e < DT / 32; ++e) acc[e] = 0.f;
-#pragma unroll 4
-  for (int i = 0; i < parts; ++i) {
-    const float* s = slot(i);
-    const float mi = s[C::kRows * DT + r];
-    const float al = mi == -INFINITY ? 0.f : ex2_approx(mi - top);
-    sum += s[C::kRows * DT + C::kRows + r] * al;
-    if constexpr (DT == 128) {
-      const float4 x = *reinterpret_cast<const float4*>(s + r * DT + lane * 4);
-      acc[0] += x.x * al;
-      acc[1] += x.y * al;
-      acc[2] += x.z * al;
-      acc[3] += x.w * al;
-    } else {
-      const float2 x = *reinterpret_cast<const float2*>(s + r * DT + lane * 2);
-      acc[0] += x.x * al;
-      acc[1] += x.y * al;
+    for (int e = 0; e < DT / 32; ++e) acc[e] = 0.f;
+#pragma unroll 8
+    for (int i = 0; i < parts; ++i) {
+      const float* s = slot(i);
+      const float mi = s[C::kRows * DT + r];
+      const float al = mi == -INFINITY ? 0.f : ex2_approx(mi - top);
+      sum += s[C::kRows * DT + C::kRows + r] * al;
+      if constexpr (DT == 128) {
+        const float4 x = *reinterpret_cast<const float4*>(s + r * DT + lane * 4);
+        acc[0] += x.x * al;
+        acc[1] += x.y * al;
+        acc[2] += x.z * al;
+        acc[3] += x.w * al;
+      } else {
+        const float2 x = *reinterpret_cast<const float2*>(s + r * DT + lane * 2);
+        acc[0] += x.x * al;
+        acc[1] += x.y * al;
+      }
     }
-  }
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  const int tok = (row0 + r) / p.g, hd = (row0 + r) - tok * p.g;
-  uint16_t* dst = static_cast<uint16_t*>(p.o) + static_cast<int64_t>(w.begin + tok) * p.o_st +
-                  static_cast<int64_t>(h * p.g + hd) * p.o_sh;
-  if constexpr (DT == 128) {
-    if (lane * 4 < p.D)
-      *reinterpret_cast<uint2*>(dst + lane * 4) =
-          make_uint2(pack_16x2<F16>(acc[0] * inv, acc[1] * inv),
-                     pack_16x2<F16>(acc[2] * inv, acc[3] * inv));
-  } else {
-    if (lane * 2 < p.D)
-      *reinterpret_cast<uint32_t*>(dst + lane * 2) = pack_16x2<F16>(acc[0] * inv, acc[1] * inv);
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const int tok = (row0 + r) / p.g, hd = (row0 + r) - tok * p.g;
+    uint16_t* dst = static_cast<uint16_t*>(p.o) + static_cast<int64_t>(w.begin + tok) * p.o_st +
+                    static_cast<int64_t>(h * p.g + hd) * p.o_sh;
+    if constexpr (DT == 128) {
+      if (lane * 4 < p.D)
+        *reinterpret_cast<uint2*>(dst + lane * 4) =
+            make_uint2(pack_16x2<F16>(acc[0] * inv, acc[1] * inv),
+                       pack_16x2<F16>(acc[2] * inv, acc[3] * inv));
+    } else {
+      if (lane * 2 < p.D)
+        *reinterpret_cast<uint32_t*>(dst + lane * 2) = pack_16x2<F16>(acc[0] * inv, acc[1] * inv);
+    }
   }
 }
 
 // ---------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------
-constexpr int kRowCtasPerSm = 2;
-
-template <int DT, int MT, bool F16>
-int launch_rows(const PagedParams& p, cudaStream_t stream) {
-  using C = RowCfg<DT, MT>;
+template <int DT, int MT, bool F16, Cut CUT>
+int launch_rows_kernel(const PagedParams& p, cudaStream_t stream) {
+  using C = RowCfg<DT, MT, CUT>;
   static KernelPrep prep;
   int dev = 0;
-  int rc = prepare_kernel(
-      prep, reinterpret_cast<const void*>(paged_rows_kernel<DT, MT, F16>), C::kSmem, &dev);
+  const int rc = prepare_kernel(
+      prep, reinterpret_cast<const void*>(paged_rows_kernel<DT, MT, F16, CUT>), C::kSmem, &dev);
   if (rc != FA_OK) return rc;
-  rc = launch_after(paged_rows_kernel<DT, MT, F16>, dim3(p.ctas), kRowThreads, C::kSmem, stream, p);
+  return launch_after(paged_rows_kernel<DT, MT, F16, CUT>, dim3(p.ctas * p.team), C::kThreads,
+                      C::kSmem, stream, p);
+}
+
+template <int DT, int MT, bool F16>
+int launch_rows(const PagedParams& p, Cut cut, int rows, cudaStream_t stream) {
+  if (cut == kWhole) return launch_rows_kernel<DT, MT, F16, kWhole>(p, stream);
+  if (MT == 1 && cut == kWholeWide) return launch_rows_kernel<DT, 1, F16, kWholeWide>(p, stream);
+  const int rc = launch_rows_kernel<DT, MT, F16, kSplit>(p, stream);
   if (rc != FA_OK) return rc;
-  return launch_after(paged_rows_join<DT, MT, F16>, dim3(p.ctas, C::kRows / kRowWarps), kRowThreads,
-                      0, stream, p);
+  return launch_after(paged_rows_join<DT, MT, F16>,
+                      dim3(p.ctas * p.team, (rows + kRowWarps - 1) / kRowWarps), kRowThreads, 0,
+                      stream, p);
 }
 
 template <int DT, int MT>
-int launch_rows_t(const PagedParams& p, bool f16, cudaStream_t stream) {
-  return f16 ? launch_rows<DT, MT, true>(p, stream) : launch_rows<DT, MT, false>(p, stream);
+int launch_rows_t(const PagedParams& p, bool f16, Cut cut, int rows, cudaStream_t stream) {
+  return f16 ? launch_rows<DT, MT, true>(p, cut, rows, stream)
+             : launch_rows<DT, MT, false>(p, cut, rows, stream);
 }
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
@@ -592,25 +660,62 @@ int check_paged_attn(const fa_paged_attn_args* a) {
   return FA_OK;
 }
 
-// Which kernel runs: the row kernel where the longest sequence has few rows,
-// else the tile kernel, for short sequences of the batch too.  (Separate launches
-// for the two kinds took 176 us against 130 for 5 chunks and 4 single tokens,
-// 1787 tokens over 32k keys, 32/8 heads of 128: the second launch costs more than
-// a tile kernel's unit of a single token.)
+// Which kernel runs, by sizes that the host knows.
+//  * Few rows over a short table: the row kernel with a CTA per sequence, head and
+//    16 rows, of 16 warps (8 with D > 64), up to 8 steps of each and a CTA per SM.
+//    37 tokens over 1061 keys, 16 heads of 64: 10.4 us, 16.5 split and joined, 21 by
+//    the tile kernel.
+//  * The row kernel takes the other sequences of up to kRowMax rows (single
+//    tokens), and chunks whose products over the whole table are at most kRowWork
+//    operations; over up to 1024 keys again without a join (256 sequences of 512
+//    keys, 8 heads of 64: 36 us against 51).
+//  * The tile kernel takes chunks, and then the batch's short sequences too: a
+//    second launch for those costs more than a tile kernel's unit of one token.
 constexpr int kRowMax = 32;
+constexpr double kRowWork = 1e9;
 
-enum class Kernel { kRows16, kRows32, kTiles };
+struct Choice {
+  bool tiles;
+  bool rows32;          // row tiles of 32 rows, else 16
+  Cut cut;
+  int tile_ctas;        // whole units: CTAs over a head's row tiles
+};
 
-Kernel choose(const fa_paged_attn_args* a) {
+Choice choose(const fa_paged_attn_args* a, int sms) {
   const int64_t longest = (a->max_q_len < a->T ? a->max_q_len : a->T) * (a->Hq / a->Hkv);
+  const int64_t keys = a->max_pages * a->page_size, units = a->B * a->Hkv;
+  const int64_t tiles16 = (longest + 15) / 16;
+  const int wide_keys = 8 * (a->D <= 64 ? RowCfg<64, 1, kWholeWide>::kStep
+                                        : RowCfg<128, 1, kWholeWide>::kStep);
+  if (units <= sms && units * tiles16 <= sms && keys <= wide_keys)
+    return {false, false, kWholeWide, static_cast<int>(tiles16)};
+  if (longest <= kRowMax && keys <= 1024 && units <= 0x7fffffffLL)
+    return {false, longest > 16, kWhole, 1};
   // The tile kernel's copies need real strides, its exponent a scale that keeps order.
   const bool flat = (a->q_strides[0] == 0 && a->T > 1) || (a->q_strides[1] == 0 && a->Hq > 1) ||
                     (a->k_cache_strides[0] == 0 && a->pages > 1) || a->k_cache_strides[1] == 0 ||
                     (a->k_cache_strides[2] == 0 && a->Hkv > 1) ||
                     (a->v_cache_strides[0] == 0 && a->pages > 1) || a->v_cache_strides[1] == 0 ||
                     (a->v_cache_strides[2] == 0 && a->Hkv > 1);
-  if (longest > kRowMax && !flat && a->scale >= 0) return Kernel::kTiles;
-  return longest <= 16 ? Kernel::kRows16 : Kernel::kRows32;
+  const double most = 4.0 * a->T * a->Hq * a->D * keys;
+  return {longest > kRowMax && most > kRowWork && !flat && a->scale >= 0, longest > 16, kSplit, 1};
+}
+
+// Teams of the row kernel: of the size, up to 16 heads, that fills the device
+// best, and as many as it holds at once.
+struct Teams {
+  int heads, count;
+};
+Teams row_teams(const fa_paged_attn_args* a, const Choice& c, int sms) {
+  if (c.cut != kSplit) return {static_cast<int>(a->Hkv), static_cast<int>(a->B) * c.tile_ctas};
+  const int ctas = sms * (c.rows32 ? (a->D <= 64 ? RowCfg<64, 2>::kCtasPerSm
+                                                 : RowCfg<128, 2>::kCtasPerSm)
+                                   : (a->D <= 64 ? RowCfg<64, 1>::kCtasPerSm
+                                                 : RowCfg<128, 1>::kCtasPerSm));
+  Teams best = {1, ctas};
+  for (int n = 2; n <= 16; ++n)
+    if (a->Hkv % n == 0 && ctas / n * n >= best.heads * best.count * 0.97) best = {n, ctas / n};
+  return best;
 }
 
 }  // namespace
@@ -618,16 +723,18 @@ Kernel choose(const fa_paged_attn_args* a) {
 
 extern "C" int64_t fa_paged_attn_workspace(const fa_paged_attn_args* a) {
   using namespace fa;
-  int rc = check_paged_attn(a);
+  const int rc = check_paged_attn(a);
   if (rc != FA_OK) return -rc;
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return -FA_ERR_CUDA;
   const int sms = sm_count(dev);
   if (sms <= 0) return -FA_ERR_CUDA;
-  const Kernel k = choose(a);
-  if (k == Kernel::kTiles) return paged_tiles_bytes(a, sms);
-  const int64_t slot = (k == Kernel::kRows16 ? 16 : 32) * ((a->D <= 64 ? 64 : 128) + 2);
-  return 2ll * kRowCtasPerSm * sms * slot * 4;
+  const Choice c = choose(a, sms);
+  if (c.tiles) return paged_tiles_bytes(a, sms);
+  if (c.cut != kSplit) return 0;
+  const Teams t = row_teams(a, c, sms);
+  return 2ll * t.heads * t.count * (c.rows32 ? 32 : 16) *
+         ((a->D <= 64 ? 64 : 128) + 2) * 4;
 }
 
 extern "C" int fa_paged_attn(const fa_paged_attn_args* a, void* workspace,
@@ -639,7 +746,7 @@ extern "C" int fa_paged_attn(const fa_paged_attn_args* a, void* workspace,
   if ((rc = prepare_device(nullptr, 0, &dev)) != FA_OK) return rc;
   const int64_t need = fa_paged_attn_workspace(a);
   if (need < 0) return static_cast<int>(-need);
-  if (!workspace || workspace_bytes < need) return FA_ERR_WORKSPACE;
+  if (need > 0 && (!workspace || workspace_bytes < need)) return FA_ERR_WORKSPACE;
   if (!aligned16(workspace)) return FA_ERR_ALIGN;
   PagedParams p = {};
   p.q = a->q;
@@ -675,15 +782,23 @@ extern "C" int fa_paged_attn(const fa_paged_attn_args* a, void* workspace,
   const int sms = sm_count(dev);
   const bool f16 = a->dtype == FA_F16;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const Kernel k = choose(a);
-  if (k == Kernel::kTiles) {
+  const Choice c = choose(a, sms);
+  if (c.tiles) {
     p.ctas = sms;
     return launch_paged_tiles(a, p, workspace, s);
   }
+  const Teams t = row_teams(a, c, sms);
+  p.ctas = t.count;
+  p.team = t.heads;
+  p.tile_ctas = c.tile_ctas;
   p.part = static_cast<float*>(workspace);
-  p.ctas = kRowCtasPerSm * sms;
   p.min_blocks = 4;
-  if (k == Kernel::kRows16)
-    return p.D <= 64 ? launch_rows_t<64, 1>(p, f16, s) : launch_rows_t<128, 1>(p, f16, s);
-  return p.D <= 64 ? launch_rows_t<64, 2>(p, f16, s) : launch_rows_t<128, 2>(p, f16, s);
+  // (the join's CTAs go over more rows than these where max_q_len was too small)
+  const int64_t longest = (a->max_q_len < a->T ? a->max_q_len : a->T) * p.g;
+  const int rows = static_cast<int>(longest < 32 ? longest : 32);
+  if (c.rows32)
+    return p.D <= 64 ? launch_rows_t<64, 2>(p, f16, c.cut, rows, s)
+                     : launch_rows_t<128, 2>(p, f16, c.cut, rows, s);
+  return p.D <= 64 ? launch_rows_t<64, 1>(p, f16, c.cut, rows, s)
+                   : launch_rows_t<128, 1>(p, f16, c.cut, rows, s);
 }

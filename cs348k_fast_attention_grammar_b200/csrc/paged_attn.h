@@ -27,6 +27,8 @@ struct PagedParams {
   float* part;                          // partial results of split units
   int ctas;                             // ranges the key blocks are cut into
   int min_blocks;                       // least key blocks of a range
+  int team;                             // row kernel: heads that stream side by side
+  int tile_ctas;                        // row kernel, whole units: CTAs over a head's row tiles
 };
 
 // A sequence's new tokens and keys.

@@ -437,8 +437,9 @@ PyObject* paged_attention(PyObject* const* in) {
     if (size < 0) check(static_cast<int>(-size), "fa_paged_attn");
     // The workspace is this call's own: on one stream the allocator hands it
     // out again in order, and a captured graph keeps its own.
-    const at::Tensor ws = make({size}, at::kByte, q->device());
-    check(lib.paged_attn(&a, ws.data_ptr(), size, c10::cuda::getCurrentCUDAStream().stream()),
+    at::Tensor ws;
+    if (size > 0) ws = make({size}, at::kByte, q->device());
+    check(lib.paged_attn(&a, size > 0 ? ws.data_ptr() : nullptr, size, c10::cuda::getCurrentCUDAStream().stream()),
           "fa_paged_attn");
   }
   return out.obj ? given(out.obj) : THPVariable_Wrap(std::move(made));
