@@ -24,10 +24,14 @@
 // Work (decided on the device by paged_plan_kernel, from the lengths):
 //  * many units (4 per SM or more): CTAs take whole units from a counter, heads
 //    in groups whose K and V fit half the L2, longest units first;
-//  * few units: the key blocks of all units, laid end to end, are cut into one
-//    equal range per CTA.  A unit that crosses a border leaves (m, l, O) of its
-//    parts in the workspace and paged_tiles_join adds them in the order of the
-//    keys.  A unit counts one block more than it has, for its start and end.
+//  * few units: every CTA gets the same number of key blocks, L.  A unit of more
+//    than L is cut at L, 2 L, ... and each such part is one CTA's work; what is
+//    left of it, and shorter units, are laid end to end and cut into equal ranges
+//    for the other CTAs.  The parts of one head's units begin at the same keys, so
+//    the CTAs that read them run side by side in the L2: with plain equal ranges
+//    512 tokens over 32768 keys (8 key heads of 128) read the cache from DRAM once
+//    for each of a head's 8 units.  A unit's parts leave (m, l, O) in the workspace
+//    and paged_tiles_join adds them in the order of the keys.
 // Results depend on the lengths alone, never on timing.
 #include <cuda_bf16.h>
 
@@ -46,7 +50,8 @@ constexpr int kRegsCtrl = 72, kRegsSoftmax = 216;
 static_assert(128 * kRegsCtrl + 256 * kRegsSoftmax <= 384 * 168,
               "the register split exceeds the launch's pool");
 constexpr int kUnitsPerSm = 4;       // from here on units are not split
-constexpr int kPlanThreads = 1024;
+constexpr int kPlanThreads = 640;       // at least the units that may be split
+constexpr int kStartCells = 2;          // what a part's start and end cost, in key blocks
 constexpr int64_t kGroupBytes = 32ll << 20;   // K and V of the heads worked on at once
 
 // A unit, or the part of one that a CTA computes.
@@ -62,7 +67,7 @@ struct Piece {
 static_assert(sizeof(Piece) == 48, "pieces are copied as three 16-byte words");
 
 // The plan, at the workspace's start.
-enum : int { kSplit = 0, kUnits = 1, kNext = 2, kHeader = 4 };
+enum : int { kSplit = 0, kUnits = 1, kNext = 2, kJoins = 3, kHeader = 4 };
 struct TileParams : PagedParams {
   int tq;                // tokens of a tile
   int box_rows;          // rows of a load box
@@ -71,7 +76,7 @@ struct TileParams : PagedParams {
   int* plan;             // header
   int* prefix;           // [B + 1]: units (per head) of the sequences before
   int* first;            // [ctas + 1]: first piece of each CTA
-  int2* join;            // [ctas]: first piece and number of parts of the unit to add up
+  int4* join;            // [ctas]: a unit in parts: a piece of it, its first slot, how many
   Piece* pieces;
 };
 
@@ -138,8 +143,9 @@ __device__ __forceinline__ Piece whole_unit(const TileParams& p, int64_t i) {
   return make_piece(p, w, b, g * hg + in % here, u, 0, INT_MAX, -1);
 }
 
-// Exclusive prefix sum over the CTA's 1024 threads; *total: the sum.
+// Exclusive prefix sum over the CTA's threads; *total: the sum.
 __device__ __forceinline__ int64_t plan_scan(int64_t v, int64_t* red, int64_t* total) {
+  constexpr int kWarps = kPlanThreads / 32;
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   int64_t x = v;
 #pragma unroll
@@ -150,37 +156,62 @@ __device__ __forceinline__ int64_t plan_scan(int64_t v, int64_t* red, int64_t* t
   __syncthreads();
   if (lane == 31) red[w] = x;
   __syncthreads();
-  if (w == 0) {
-    int64_t y = red[lane];
+  int64_t y = lane < kWarps ? red[lane] : 0;      // every warp scans the warps' sums
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t z = __shfl_up_sync(0xffffffffu, y, o);
-      if (lane >= o) y += z;
-    }
-    red[lane] = y;
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t z = __shfl_up_sync(0xffffffffu, y, o);
+    if (lane >= o) y += z;
   }
-  __syncthreads();
-  *total = red[31];
-  return (w > 0 ? red[w - 1] : 0) + x - v;
+  *total = __shfl_sync(0xffffffffu, y, 31);
+  const int64_t before = __shfl_sync(0xffffffffu, y, w > 0 ? w - 1 : 0);
+  return (w > 0 ? before : 0) + x - v;
+}
+
+// A unit of nb key blocks in parts of L: whole parts and what is left.
+struct Parts {
+  int whole, left;
+};
+__device__ __forceinline__ Parts cut_unit(int nb, int L) {
+  Parts c = {0, nb};
+  if (nb > L) {
+    c.whole = static_cast<int>(static_cast<unsigned>(nb) / static_cast<unsigned>(L));
+    c.left = nb - c.whole * L;
+  }
+  return c;
+}
+// Cells that the rest of a unit takes in the laid-out row of such rests.
+__device__ __forceinline__ int rest_cells(const Parts& c) {
+  return c.left > 0 || c.whole == 0 ? c.left + kStartCells : 0;
 }
 
 // One CTA.  Counts every sequence's units; where they are few, cuts their key
-// blocks into the CTAs' ranges.
+// blocks into the CTAs' shares.  Everything waits for it, so what it looks up
+// again (lengths, prefix sums) stays in shared memory.
+constexpr int kPlanWarps = kPlanThreads / 32;
 __global__ void __launch_bounds__(kPlanThreads)
     paged_plan_kernel(const TileParams p) {
   __shared__ int64_t red[32];
-  __shared__ int64_t cells_before[kPlanThreads + 1];    // of (sequence, unit) pairs, one head
+  __shared__ int s_blocks[kPlanThreads];                // of (sequence, unit) pairs, one head
   __shared__ int count[kPlanThreads];
+  __shared__ int s_prefix[kPlanThreads + 1];
+  __shared__ SeqWork s_work[kPlanThreads];
+  __shared__ int s_fits[kPlanWarps];
   grid_dependency_wait();
   grid_dependents_launch();
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   int64_t pairs = 0;
   for (int b0 = 0; b0 < p.B; b0 += kPlanThreads) {
     const int b = b0 + tid;
-    const int n = b < p.B ? units_of(p, seq_work(p, b)) : 0;
+    SeqWork w = {};
+    if (b < p.B) w = seq_work(p, b);
+    const int n = units_of(p, w);
     int64_t sum;
     const int64_t before = pairs + plan_scan(n, red, &sum);
     if (b < p.B) p.prefix[b] = static_cast<int>(before);
+    if (b0 == 0) {
+      s_prefix[tid] = static_cast<int>(before);
+      s_work[tid] = w;
+    }
     pairs += sum;
   }
   const int64_t units = pairs * p.Hkv;
@@ -190,57 +221,100 @@ __global__ void __launch_bounds__(kPlanThreads)
     p.plan[kSplit] = split;
     p.plan[kUnits] = static_cast<int>(units);
     p.plan[kNext] = 0;
+    if (p.B <= kPlanThreads) s_prefix[p.B] = static_cast<int>(pairs);
   }
   if (!split) return;
-  __syncthreads();
-
-  // Cells: a unit's key blocks and one more.
-  int64_t cells = 0;
-  if (tid < pairs) {
-    const int b = seq_of_unit(p.prefix, p.B, 1, tid);
-    const SeqWork w = seq_work(p, b);
-    cells = 1 + blocks_of(p, w, (tid - p.prefix[b]) * 2 * p.tq, 2 * p.tq);
-  }
-  int64_t per_head;
-  const int64_t before = plan_scan(cells, red, &per_head);
-  cells_before[tid] = before;
-  if (tid == kPlanThreads - 1) cells_before[kPlanThreads] = per_head;
   count[tid] = 0;
   __syncthreads();
-  const int64_t per = max(static_cast<int64_t>(p.min_cells),
-                          (per_head * p.Hkv + p.ctas - 1) / p.ctas);
+  const bool held = p.B <= kPlanThreads;
+  const int* prefix = held ? s_prefix : p.prefix;
+  auto work = [&](int b) { return held ? s_work[b] : seq_work(p, b); };
 
-  // Units in the order (sequence, head, unit): where each begins, the CTAs it spans.
-  int b = 0, h = 0, u = 0, c0 = 0, parts = 0;
-  int64_t at = 0, end = 0;
+  // The least cells (key blocks and kStartCells per part) of a CTA, of 20 tried,
+  // with which the work fits the CTAs: a warp tries one.
+  int nb = 0;
+  if (tid < pairs) {
+    const int b = seq_of_unit(prefix, p.B, 1, tid);
+    nb = blocks_of(p, work(b), (tid - prefix[b]) * 2 * p.tq, 2 * p.tq);
+  }
+  s_blocks[tid] = nb;
+  int64_t all;
+  plan_scan(tid < pairs ? nb + kStartCells : 0, red, &all);
+  const int least = max(p.min_cells + kStartCells,
+                        static_cast<int>((all * p.Hkv + p.ctas - 1) / p.ctas));
+  auto tried = [&](int j) {
+    return least + static_cast<int>((static_cast<int64_t>(least) * j + 39) / 40);
+  };
+  {
+    const int cells = tried(warp);
+    int64_t whole = 0, rest = 0;
+    for (int i = lane; i < pairs; i += 32) {
+      const Parts c = cut_unit(s_blocks[i], cells - kStartCells);
+      whole += c.whole;
+      rest += rest_cells(c);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      whole += __shfl_xor_sync(0xffffffffu, whole, o);
+      rest += __shfl_xor_sync(0xffffffffu, rest, o);
+    }
+    if (lane == 0) s_fits[warp] = (whole * p.Hkv + (rest * p.Hkv + cells - 1) / cells) <= p.ctas;
+  }
+  __syncthreads();
+  int cells = 2 * least;        // (always fits: a part's start is a third of it at most)
+  for (int j = kPlanWarps - 1; j >= 0; --j)
+    if (s_fits[j]) cells = tried(j);
+  const int L = cells - kStartCells;
+
+  // Units in the order (sequence, head, unit).
+  int b = 0, h = 0, u = 0;
   SeqWork w = {};
+  Parts cut = {0, 0};
+  int rest = 0;
   if (tid < units) {
-    b = seq_of_unit(p.prefix, p.B, p.Hkv, tid);
-    w = seq_work(p, b);
-    const int nu = p.prefix[b + 1] - p.prefix[b];
-    const int r = tid - p.prefix[b] * p.Hkv;
+    b = seq_of_unit(prefix, p.B, p.Hkv, tid);
+    w = work(b);
+    const int nu = prefix[b + 1] - prefix[b];
+    const int r = tid - prefix[b] * p.Hkv;
     h = r / nu;
     u = r - h * nu;
-    const int64_t s0 = cells_before[p.prefix[b]], s1 = cells_before[p.prefix[b + 1]];
-    const int64_t me = cells_before[p.prefix[b] + u], next = cells_before[p.prefix[b] + u + 1];
-    at = s0 * p.Hkv + (s1 - s0) * h + (me - s0);
-    end = at + (next - me);
-    // the first cell stands for the unit's start: its blocks begin behind it
-    c0 = static_cast<int>((end - at > 1 ? at + 1 : at) / per);
-    parts = static_cast<int>((end - 1) / per) - c0 + 1;
+    cut = cut_unit(s_blocks[prefix[b] + u], L);
+    rest = rest_cells(cut);
   }
+  // CTAs of the whole parts before this unit's, cells of the rests before it.
+  constexpr int64_t kHigh = 1ll << 40;
   int64_t total;
-  const int at_piece = static_cast<int>(plan_scan(parts, red, &total));
-  if (tid < p.ctas) p.join[tid] = make_int2(0, 0);
-  __syncthreads();
-  for (int i = 0; i < parts; ++i) {
-    const int64_t lo = max(at + 1, (c0 + i) * per), hi = min(end, (c0 + i + 1) * per);
-    const int blk0 = static_cast<int>(min(lo, hi) - at - 1), blk1 = static_cast<int>(hi - at - 1);
-    const int slot = parts == 1 ? -1 : 2 * (c0 + i) + (i == 0 ? 1 : 0);
-    p.pieces[at_piece + i] = make_piece(p, w, b, h, u, max(0, blk0), max(0, blk1), slot);
-    atomicAdd(&count[c0 + i], 1);
+  int64_t before = plan_scan(cut.whole * kHigh + rest, red, &total);
+  const int cta0 = static_cast<int>(before / kHigh), ctas_whole = static_cast<int>(total / kHigh);
+  const int64_t at = before % kHigh + kStartCells, end = at + cut.left;   // the rest's key blocks
+  int c0 = 0, n = 0;                                    // CTAs of the rest (a unit without keys:
+  if (rest > 0) {                                       // where its start lies)
+    c0 = static_cast<int>((end > at ? at : at - 1) / cells);
+    n = end > at ? static_cast<int>((end - 1) / cells) - c0 + 1 : 1;
   }
-  if (parts > 1) p.join[c0] = make_int2(at_piece, parts);
+  const int parts = cut.whole + n;
+  const bool alone = parts <= 1;
+  // Pieces of the rests before this unit's, slots, units in parts.
+  before = plan_scan(n + (alone ? 0 : parts) * (kHigh >> 20) + (alone ? 0 : kHigh), red, &total);
+  const int piece0 = ctas_whole + static_cast<int>(before % (kHigh >> 20));
+  const int slot0 = static_cast<int>(before / (kHigh >> 20) % (1 << 20));
+  for (int i = 0; i < cut.whole; ++i) {
+    p.pieces[cta0 + i] = make_piece(p, w, b, h, u, i * L, (i + 1) * L, alone ? -1 : slot0 + i);
+    count[cta0 + i] = 1;
+  }
+  for (int i = 0; i < n; ++i) {
+    const int64_t lo = max(at, static_cast<int64_t>(c0 + i) * cells);
+    const int64_t hi = min(end, static_cast<int64_t>(c0 + i + 1) * cells);
+    const int blk = cut.whole * L;
+    p.pieces[piece0 + i] =
+        make_piece(p, w, b, h, u, end > at ? blk + static_cast<int>(lo - at) : 0,
+                   end > at ? blk + static_cast<int>(hi - at) : 0,
+                   alone ? -1 : slot0 + cut.whole + i);
+    atomicAdd(&count[ctas_whole + c0 + i], 1);
+  }
+  if (!alone)
+    p.join[before / kHigh] = make_int4(cut.whole > 0 ? cta0 : piece0, slot0, parts, 0);
+  if (tid == 0) p.plan[kJoins] = static_cast<int>(total / kHigh);
   __syncthreads();
   const int64_t first = plan_scan(tid < p.ctas ? count[tid] : 0, red, &total);
   if (tid <= p.ctas) p.first[tid] = static_cast<int>(first);
@@ -821,8 +895,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// Adds up the parts of the unit that begins in CTA blockIdx.x's range and goes
-// on behind it: a CTA takes 32 rows (a lane each), a warp D / 8 channels of them.
+// Adds up the parts of a unit: a CTA takes 32 rows (a lane each), a warp D / 8
+// channels of them.
 // Bound by HBM: each part is read once.
 constexpr int kJoinWarps = 8;
 template <int D, bool F16>
@@ -835,9 +909,8 @@ __global__ void __launch_bounds__(32 * kJoinWarps)
   __shared__ int64_t s_off[32];
   grid_dependency_wait();
   grid_dependents_launch();
-  if (p.plan[kSplit] == 0) return;
-  const int2 jn = p.join[blockIdx.x];
-  if (jn.y == 0) return;
+  if (p.plan[kSplit] == 0 || static_cast<int>(blockIdx.x) >= p.plan[kJoins]) return;
+  const int4 jn = p.join[blockIdx.x];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const Piece& x = p.pieces[jn.x];
   const int t = blockIdx.y / (kRows / 32);
@@ -846,21 +919,19 @@ __global__ void __launch_bounds__(32 * kJoinWarps)
   const int tok = x.tok0 + t * p.tq + row_tok;
   const bool live = row_tok < p.tq && tok < x.q_len;
   if (!__any_sync(0xffffffffu, live)) return;                 // (the same in every warp)
-  auto part = [&](int i) {
-    return p.part + static_cast<int64_t>(2 * (blockIdx.x + i) + (i == 0 ? 1 : 0)) * C::kSlot;
-  };
+  auto part = [&](int i) { return p.part + static_cast<int64_t>(jn.y + i) * C::kSlot; };
   const int at_m = 2 * kRows * D + t * kRows + row, at_l = at_m + 2 * kRows;
   float top = -INFINITY;
   if (live)
 #pragma unroll 4
-    for (int i = 0; i < jn.y; ++i) top = fmaxf(top, part(i)[at_m]);
+    for (int i = 0; i < jn.z; ++i) top = fmaxf(top, part(i)[at_m]);
   float sum = 0.f;
   float4 acc[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) acc[e] = make_float4(0.f, 0.f, 0.f, 0.f);
   if (live)
 #pragma unroll 4
-    for (int i = 0; i < jn.y; ++i) {
+    for (int i = 0; i < jn.z; ++i) {
       const float* s = part(i);
       const float mi = s[at_m], li = s[at_l];
       if (mi == -INFINITY) {            // saw none of these keys: O was not written
@@ -918,7 +989,7 @@ PlanOffsets plan_offsets(const fa_paged_attn_args* a, int sms) {
   o.prefix = up128(kHeader * 4);
   o.first = o.prefix + up128((a->B + 1) * 4);
   o.join = o.first + up128((sms + 1) * 4);
-  o.pieces = o.join + up128(sms * 8);
+  o.pieces = o.join + up128(sms * 16);
   const bool split = may_split(a, sms);
   const int64_t most = split ? kUnitsPerSm * sms + sms : 0;
   o.parts = o.pieces + up128(most * static_cast<int64_t>(sizeof(Piece)));
@@ -983,7 +1054,7 @@ int launch_paged_tiles(const fa_paged_attn_args* a, const PagedParams& q, void* 
   p.plan = reinterpret_cast<int*>(ws);
   p.prefix = reinterpret_cast<int*>(ws + o.prefix);
   p.first = reinterpret_cast<int*>(ws + o.first);
-  p.join = reinterpret_cast<int2*>(ws + o.join);
+  p.join = reinterpret_cast<int4*>(ws + o.join);
   p.pieces = reinterpret_cast<Piece*>(ws + o.pieces);
   p.part = reinterpret_cast<float*>(ws + o.parts);
   p.min_cells = 4;
