@@ -66,6 +66,14 @@ struct Piece {
 };
 static_assert(sizeof(Piece) == 48, "pieces are copied as three 16-byte words");
 
+// A unit in parts, for the join.
+struct JoinUnit {
+  int slot0, parts;
+  int tok0, q_begin, q_len, h;
+  int pad[2];
+};
+static_assert(sizeof(JoinUnit) == 32, "read as two 16-byte words");
+
 // The plan, at the workspace's start.
 enum : int { kSplit = 0, kUnits = 1, kNext = 2, kJoins = 3, kHeader = 4 };
 struct TileParams : PagedParams {
@@ -76,7 +84,7 @@ struct TileParams : PagedParams {
   int* plan;             // header
   int* prefix;           // [B + 1]: units (per head) of the sequences before
   int* first;            // [ctas + 1]: first piece of each CTA
-  int4* join;            // [ctas]: a unit in parts: a piece of it, its first slot, how many
+  JoinUnit* join;        // [ctas]
   Piece* pieces;
 };
 
@@ -115,8 +123,15 @@ __device__ __forceinline__ Piece make_piece(const TileParams& p, const SeqWork& 
   x.pad[0] = x.pad[1] = 0;
   return x;
 }
+__device__ __forceinline__ void put_piece(Piece* to, const Piece& x) {
+  int4* d = reinterpret_cast<int4*>(to);
+  d[0] = make_int4(x.b, x.h, x.tok0, x.q_begin);
+  d[1] = make_int4(x.q_len, x.kv_len, x.blk0, x.nt[0]);
+  d[2] = make_int4(x.nt[1], x.slot, 0, 0);
+}
 // The sequence whose units (times heads) hold unit i.
-__device__ __forceinline__ int seq_of_unit(const int* prefix, int B, int64_t heads, int64_t i) {
+template <typename I>
+__device__ __forceinline__ int seq_of_unit(const int* prefix, int B, I heads, I i) {
   int lo = 0, hi = B;                   // prefix[lo] * heads <= i < prefix[hi] * heads
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
@@ -128,7 +143,7 @@ __device__ __forceinline__ int seq_of_unit(const int* prefix, int B, int64_t hea
 // Unit i of the whole list: sequences in order, a sequence's heads in groups
 // that stay in the L2, in a group the longest units (the last tokens) first.
 __device__ __forceinline__ Piece whole_unit(const TileParams& p, int64_t i) {
-  const int b = seq_of_unit(p.prefix, p.B, p.Hkv, i);
+  const int b = seq_of_unit<int64_t>(p.prefix, p.B, p.Hkv, i);
   const SeqWork w = seq_work(p, b);
   const int nu = p.prefix[b + 1] - p.prefix[b];
   const int r = static_cast<int>(i - static_cast<int64_t>(p.prefix[b]) * p.Hkv);
@@ -144,26 +159,26 @@ __device__ __forceinline__ Piece whole_unit(const TileParams& p, int64_t i) {
 }
 
 // Exclusive prefix sum over the CTA's threads; *total: the sum.
-__device__ __forceinline__ int64_t plan_scan(int64_t v, int64_t* red, int64_t* total) {
+__device__ __forceinline__ unsigned plan_scan(unsigned v, unsigned* red, unsigned* total) {
   constexpr int kWarps = kPlanThreads / 32;
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  int64_t x = v;
+  unsigned x = v;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+    const unsigned y = __shfl_up_sync(0xffffffffu, x, o);
     if (lane >= o) x += y;
   }
   __syncthreads();
   if (lane == 31) red[w] = x;
   __syncthreads();
-  int64_t y = lane < kWarps ? red[lane] : 0;      // every warp scans the warps' sums
+  unsigned y = lane < kWarps ? red[lane] : 0;     // every warp scans the warps' sums
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int64_t z = __shfl_up_sync(0xffffffffu, y, o);
+    const unsigned z = __shfl_up_sync(0xffffffffu, y, o);
     if (lane >= o) y += z;
   }
   *total = __shfl_sync(0xffffffffu, y, 31);
-  const int64_t before = __shfl_sync(0xffffffffu, y, w > 0 ? w - 1 : 0);
+  const unsigned before = __shfl_sync(0xffffffffu, y, w > 0 ? w - 1 : 0);
   return (w > 0 ? before : 0) + x - v;
 }
 
@@ -185,28 +200,33 @@ __device__ __forceinline__ int rest_cells(const Parts& c) {
 }
 
 // One CTA.  Counts every sequence's units; where they are few, cuts their key
-// blocks into the CTAs' shares.  Everything waits for it, so what it looks up
-// again (lengths, prefix sums) stays in shared memory.
+// blocks into the CTAs' shares.  Everything waits for it (6000 clocks, of which
+// each of its prefix sums takes 400), so what it looks up again stays in shared
+// memory and its numbers are packed into 32 bits.
 constexpr int kPlanWarps = kPlanThreads / 32;
+constexpr int kMaxSplitCells = 1 << 23;       // of a batch that is cut up
+constexpr int kMaxSplitCtas = 255;
 __global__ void __launch_bounds__(kPlanThreads)
     paged_plan_kernel(const TileParams p) {
-  __shared__ int64_t red[32];
+  __shared__ unsigned red[32];
   __shared__ int s_blocks[kPlanThreads];                // of (sequence, unit) pairs, one head
-  __shared__ int count[kPlanThreads];
   __shared__ int s_prefix[kPlanThreads + 1];
   __shared__ SeqWork s_work[kPlanThreads];
-  __shared__ int s_fits[kPlanWarps];
+  __shared__ unsigned s_all, s_fits;
   grid_dependency_wait();
   grid_dependents_launch();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  int64_t pairs = 0;
+  if (tid == 0) {
+    s_all = 0;
+    s_fits = 0;
+  }
+  unsigned pairs = 0;                   // (T and B are below 2^31, and so are units)
   for (int b0 = 0; b0 < p.B; b0 += kPlanThreads) {
     const int b = b0 + tid;
     SeqWork w = {};
     if (b < p.B) w = seq_work(p, b);
-    const int n = units_of(p, w);
-    int64_t sum;
-    const int64_t before = pairs + plan_scan(n, red, &sum);
+    unsigned sum;
+    const unsigned before = pairs + plan_scan(units_of(p, w), red, &sum);
     if (b < p.B) p.prefix[b] = static_cast<int>(before);
     if (b0 == 0) {
       s_prefix[tid] = static_cast<int>(before);
@@ -214,56 +234,55 @@ __global__ void __launch_bounds__(kPlanThreads)
     }
     pairs += sum;
   }
-  const int64_t units = pairs * p.Hkv;
-  const bool split = units < p.split_units;             // then units <= kPlanThreads
   if (tid == 0) {
     p.prefix[p.B] = static_cast<int>(pairs);
-    p.plan[kSplit] = split;
-    p.plan[kUnits] = static_cast<int>(units);
+    p.plan[kUnits] = static_cast<int>(pairs * p.Hkv);
     p.plan[kNext] = 0;
     if (p.B <= kPlanThreads) s_prefix[p.B] = static_cast<int>(pairs);
   }
-  if (!split) return;
-  count[tid] = 0;
-  __syncthreads();
+  bool split = static_cast<uint64_t>(pairs) * p.Hkv < static_cast<uint64_t>(p.split_units);
+  int nb = 0;                           // (split_units <= kPlanThreads)
   const bool held = p.B <= kPlanThreads;
   const int* prefix = held ? s_prefix : p.prefix;
   auto work = [&](int b) { return held ? s_work[b] : seq_work(p, b); };
+  __syncthreads();
+  if (split && tid < pairs) {
+    const int b = seq_of_unit(prefix, p.B, 1, tid);
+    nb = blocks_of(p, work(b), (tid - prefix[b]) * 2 * p.tq, 2 * p.tq);
+    s_blocks[tid] = nb;
+  }
+  if (split) {                          // (held to the limit, so that no sum overflows)
+    unsigned sum = tid < pairs ? min(nb + kStartCells, kMaxSplitCells) : 0;
+    sum = __reduce_add_sync(0xffffffffu, sum);
+    if (lane == 0) atomicAdd(&s_all, min(sum, static_cast<unsigned>(kMaxSplitCells)));
+  }
+  __syncthreads();
+  split = split && static_cast<uint64_t>(s_all) * p.Hkv < kMaxSplitCells;
+  if (tid == 0) p.plan[kSplit] = split;
+  if (!split) return;
+  const int units = static_cast<int>(pairs) * p.Hkv;
 
   // The least cells (key blocks and kStartCells per part) of a CTA, of 20 tried,
   // with which the work fits the CTAs: a warp tries one.
-  int nb = 0;
-  if (tid < pairs) {
-    const int b = seq_of_unit(prefix, p.B, 1, tid);
-    nb = blocks_of(p, work(b), (tid - prefix[b]) * 2 * p.tq, 2 * p.tq);
-  }
-  s_blocks[tid] = nb;
-  int64_t all;
-  plan_scan(tid < pairs ? nb + kStartCells : 0, red, &all);
-  const int least = max(p.min_cells + kStartCells,
-                        static_cast<int>((all * p.Hkv + p.ctas - 1) / p.ctas));
-  auto tried = [&](int j) {
-    return least + static_cast<int>((static_cast<int64_t>(least) * j + 39) / 40);
-  };
+  const unsigned all = s_all * p.Hkv;
+  const int least = max(p.min_cells + kStartCells, static_cast<int>((all + p.ctas - 1) / p.ctas));
+  auto tried = [&](int j) { return least + (least * j + 39) / 40; };
   {
     const int cells = tried(warp);
-    int64_t whole = 0, rest = 0;
-    for (int i = lane; i < pairs; i += 32) {
+    unsigned whole = 0, rest = 0;
+    for (int i = lane; i < static_cast<int>(pairs); i += 32) {
       const Parts c = cut_unit(s_blocks[i], cells - kStartCells);
       whole += c.whole;
       rest += rest_cells(c);
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      whole += __shfl_xor_sync(0xffffffffu, whole, o);
-      rest += __shfl_xor_sync(0xffffffffu, rest, o);
-    }
-    if (lane == 0) s_fits[warp] = (whole * p.Hkv + (rest * p.Hkv + cells - 1) / cells) <= p.ctas;
+    whole = __reduce_add_sync(0xffffffffu, whole);
+    rest = __reduce_add_sync(0xffffffffu, rest);
+    if (lane == 0 && whole * p.Hkv + (rest * p.Hkv + cells - 1) / cells <= p.ctas)
+      atomicOr(&s_fits, 1u << warp);
   }
   __syncthreads();
-  int cells = 2 * least;        // (always fits: a part's start is a third of it at most)
-  for (int j = kPlanWarps - 1; j >= 0; --j)
-    if (s_fits[j]) cells = tried(j);
+  // (2 * least always fits: a part's start is a third of it at most)
+  const int cells = s_fits ? tried(__ffs(s_fits) - 1) : 2 * least;
   const int L = cells - kStartCells;
 
   // Units in the order (sequence, head, unit).
@@ -274,50 +293,56 @@ __global__ void __launch_bounds__(kPlanThreads)
   if (tid < units) {
     b = seq_of_unit(prefix, p.B, p.Hkv, tid);
     w = work(b);
-    const int nu = prefix[b + 1] - prefix[b];
-    const int r = tid - prefix[b] * p.Hkv;
+    const unsigned nu = prefix[b + 1] - prefix[b];
+    const unsigned r = tid - prefix[b] * p.Hkv;
     h = r / nu;
     u = r - h * nu;
     cut = cut_unit(s_blocks[prefix[b] + u], L);
     rest = rest_cells(cut);
   }
   // CTAs of the whole parts before this unit's, cells of the rests before it.
-  constexpr int64_t kHigh = 1ll << 40;
-  int64_t total;
-  int64_t before = plan_scan(cut.whole * kHigh + rest, red, &total);
-  const int cta0 = static_cast<int>(before / kHigh), ctas_whole = static_cast<int>(total / kHigh);
-  const int64_t at = before % kHigh + kStartCells, end = at + cut.left;   // the rest's key blocks
+  unsigned total;
+  unsigned before = plan_scan(static_cast<unsigned>(cut.whole) * kMaxSplitCells + rest, red, &total);
+  const int cta0 = before / kMaxSplitCells, ctas_whole = total / kMaxSplitCells;
+  const int ctas_rest = (total % kMaxSplitCells + cells - 1) / cells;
+  const int at = before % kMaxSplitCells + kStartCells, end = at + cut.left;   // the rest's blocks
   int c0 = 0, n = 0;                                    // CTAs of the rest (a unit without keys:
   if (rest > 0) {                                       // where its start lies)
-    c0 = static_cast<int>((end > at ? at : at - 1) / cells);
-    n = end > at ? static_cast<int>((end - 1) / cells) - c0 + 1 : 1;
+    c0 = static_cast<unsigned>(end > at ? at : at - 1) / static_cast<unsigned>(cells);
+    n = end > at ? static_cast<unsigned>(end - 1) / static_cast<unsigned>(cells) - c0 + 1 : 1;
   }
   const int parts = cut.whole + n;
   const bool alone = parts <= 1;
-  // Pieces of the rests before this unit's, slots, units in parts.
-  before = plan_scan(n + (alone ? 0 : parts) * (kHigh >> 20) + (alone ? 0 : kHigh), red, &total);
-  const int piece0 = ctas_whole + static_cast<int>(before % (kHigh >> 20));
-  const int slot0 = static_cast<int>(before / (kHigh >> 20) % (1 << 20));
+  // Pieces of the rests before this unit's, slots, units in parts (1024, 2048, 1024 at most).
+  before = plan_scan(n + (alone ? 0u : parts << 10 | 1u << 21), red, &total);
+  const int piece0 = ctas_whole + (before & 1023), slot0 = before >> 10 & 2047;
+  const int pieces = ctas_whole + (total & 1023);
   for (int i = 0; i < cut.whole; ++i) {
-    p.pieces[cta0 + i] = make_piece(p, w, b, h, u, i * L, (i + 1) * L, alone ? -1 : slot0 + i);
-    count[cta0 + i] = 1;
+    put_piece(p.pieces + cta0 + i,
+              make_piece(p, w, b, h, u, i * L, (i + 1) * L, alone ? -1 : slot0 + i));
+    p.first[cta0 + i] = cta0 + i;
   }
   for (int i = 0; i < n; ++i) {
-    const int64_t lo = max(at, static_cast<int64_t>(c0 + i) * cells);
-    const int64_t hi = min(end, static_cast<int64_t>(c0 + i + 1) * cells);
-    const int blk = cut.whole * L;
-    p.pieces[piece0 + i] =
-        make_piece(p, w, b, h, u, end > at ? blk + static_cast<int>(lo - at) : 0,
-                   end > at ? blk + static_cast<int>(hi - at) : 0,
-                   alone ? -1 : slot0 + cut.whole + i);
-    atomicAdd(&count[ctas_whole + c0 + i], 1);
+    const int lo = max(at, (c0 + i) * cells), hi = min(end, (c0 + i + 1) * cells);
+    const int blk = cut.whole * L - at;
+    put_piece(p.pieces + piece0 + i,
+              make_piece(p, w, b, h, u, end > at ? blk + lo : 0, end > at ? blk + hi : 0,
+                         alone ? -1 : slot0 + cut.whole + i));
+    // The first piece of a CTA: one that goes on from the CTA before, or whose
+    // unit is the first to have a key block (or its end) among the CTA's cells.
+    const int unit_at = at - kStartCells;
+    if (i > 0 || unit_at == 0 ||
+        static_cast<unsigned>(unit_at - 1) / static_cast<unsigned>(cells) <
+            static_cast<unsigned>(c0))
+      p.first[ctas_whole + c0 + i] = piece0 + i;
   }
-  if (!alone)
-    p.join[before / kHigh] = make_int4(cut.whole > 0 ? cta0 : piece0, slot0, parts, 0);
-  if (tid == 0) p.plan[kJoins] = static_cast<int>(total / kHigh);
-  __syncthreads();
-  const int64_t first = plan_scan(tid < p.ctas ? count[tid] : 0, red, &total);
-  if (tid <= p.ctas) p.first[tid] = static_cast<int>(first);
+  if (!alone) {
+    int4* d = reinterpret_cast<int4*>(p.join + (before >> 21));
+    d[0] = make_int4(slot0, parts, u * 2 * p.tq, w.begin);
+    d[1] = make_int4(w.q_len, h, 0, 0);
+  }
+  if (tid == 0) p.plan[kJoins] = total >> 21;
+  if (tid <= p.ctas && tid >= ctas_whole + ctas_rest) p.first[tid] = pieces;
 }
 
 // ---------------------------------------------------------------------------
@@ -909,47 +934,71 @@ __global__ void __launch_bounds__(32 * kJoinWarps)
   __shared__ int64_t s_off[32];
   grid_dependency_wait();
   grid_dependents_launch();
-  if (p.plan[kSplit] == 0 || static_cast<int>(blockIdx.x) >= p.plan[kJoins]) return;
-  const int4 jn = p.join[blockIdx.x];
+  // (the unit is loaded along with the count that says whether there is one)
+  const int4 head = *reinterpret_cast<const int4*>(p.plan);
+  const int4 j0 = reinterpret_cast<const int4*>(p.join + blockIdx.x)[0];
+  const int4 j1 = reinterpret_cast<const int4*>(p.join + blockIdx.x)[1];
+  static_assert(kSplit == 0 && kJoins == 3, "order of the header's words");
+  if (head.x == 0 || static_cast<int>(blockIdx.x) >= head.w) return;
+  const int slot0 = j0.x, parts = j0.y, tok0 = j0.z, q_begin = j0.w, q_len = j1.x, h = j1.y;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const Piece& x = p.pieces[jn.x];
   const int t = blockIdx.y / (kRows / 32);
   const int row = (blockIdx.y % (kRows / 32)) * 32 + lane;    // of the tile
   const int row_tok = row / p.g;
-  const int tok = x.tok0 + t * p.tq + row_tok;
-  const bool live = row_tok < p.tq && tok < x.q_len;
+  const int tok = tok0 + t * p.tq + row_tok;
+  const bool live = row_tok < p.tq && tok < q_len;
   if (!__any_sync(0xffffffffu, live)) return;                 // (the same in every warp)
-  auto part = [&](int i) { return p.part + static_cast<int64_t>(jn.y + i) * C::kSlot; };
+  const float* part = p.part + static_cast<int64_t>(slot0) * C::kSlot;
   const int at_m = 2 * kRows * D + t * kRows + row, at_l = at_m + 2 * kRows;
-  float top = -INFINITY;
-  if (live)
-#pragma unroll 4
-    for (int i = 0; i < jn.z; ++i) top = fmaxf(top, part(i)[at_m]);
-  float sum = 0.f;
+  const int at_o = (t * (D / 4) + warp * E) * kRows + row;
+  float top = -INFINITY, sum = 0.f;
   float4 acc[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) acc[e] = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (live)
-#pragma unroll 4
-    for (int i = 0; i < jn.z; ++i) {
-      const float* s = part(i);
-      const float mi = s[at_m], li = s[at_l];
-      if (mi == -INFINITY) {            // saw none of these keys: O was not written
-        sum += li;
+  // kAhead parts at a time, all of their loads in flight together.
+  constexpr int kAhead = 4;
+  for (int i0 = 0; live && i0 < parts; i0 += kAhead) {
+    float m[kAhead], l[kAhead];
+    float4 o[kAhead][E];
+    float now = top;
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const bool in = i0 + k < parts;
+      const float* s = part + static_cast<int64_t>(in ? i0 + k : i0) * C::kSlot;
+      m[k] = in ? s[at_m] : -INFINITY;
+      l[k] = in ? s[at_l] : 0.f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[k][e] = reinterpret_cast<const float4*>(s)[at_o + e * kRows];
+    }
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) now = fmaxf(now, m[k]);
+    const float keep = top == -INFINITY ? 0.f : ex2_approx(top - now);
+    sum *= keep;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      acc[e].x *= keep;
+      acc[e].y *= keep;
+      acc[e].z *= keep;
+      acc[e].w *= keep;
+    }
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      if (m[k] == -INFINITY) {          // saw none of these keys: O was not written
+        sum += l[k];
         continue;
       }
-      const float al = ex2_approx(mi - top);
-      sum += li * al;
-      const float4* o = reinterpret_cast<const float4*>(s) + (t * (D / 4) + warp * E) * kRows + row;
+      const float al = ex2_approx(m[k] - now);
+      sum += l[k] * al;
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        const float4 v = o[e * kRows];
-        acc[e].x += v.x * al;
-        acc[e].y += v.y * al;
-        acc[e].z += v.z * al;
-        acc[e].w += v.w * al;
+        acc[e].x += o[k][e].x * al;
+        acc[e].y += o[k][e].y * al;
+        acc[e].z += o[k][e].z * al;
+        acc[e].w += o[k][e].w * al;
       }
     }
+    top = now;
+  }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
   for (int e = 0; e < E; ++e)
@@ -957,8 +1006,8 @@ __global__ void __launch_bounds__(32 * kJoinWarps)
         make_uint2(pack_16x2<F16>(acc[e].x * inv, acc[e].y * inv),
                    pack_16x2<F16>(acc[e].z * inv, acc[e].w * inv));
   if (warp == 0)
-    s_off[lane] = live ? static_cast<int64_t>(x.q_begin + tok) * p.o_st +
-                             static_cast<int64_t>(x.h * p.g + row - row_tok * p.g) * p.o_sh
+    s_off[lane] = live ? static_cast<int64_t>(q_begin + tok) * p.o_st +
+                             static_cast<int64_t>(h * p.g + row - row_tok * p.g) * p.o_sh
                        : -1;
   __syncthreads();
   for (int i = threadIdx.x; i < 32 * (D / 8); i += 32 * kJoinWarps) {
@@ -989,7 +1038,7 @@ PlanOffsets plan_offsets(const fa_paged_attn_args* a, int sms) {
   o.prefix = up128(kHeader * 4);
   o.first = o.prefix + up128((a->B + 1) * 4);
   o.join = o.first + up128((sms + 1) * 4);
-  o.pieces = o.join + up128(sms * 16);
+  o.pieces = o.join + up128(sms * static_cast<int64_t>(sizeof(JoinUnit)));
   const bool split = may_split(a, sms);
   const int64_t most = split ? kUnitsPerSm * sms + sms : 0;
   o.parts = o.pieces + up128(most * static_cast<int64_t>(sizeof(Piece)));
@@ -1054,12 +1103,13 @@ int launch_paged_tiles(const fa_paged_attn_args* a, const PagedParams& q, void* 
   p.plan = reinterpret_cast<int*>(ws);
   p.prefix = reinterpret_cast<int*>(ws + o.prefix);
   p.first = reinterpret_cast<int*>(ws + o.first);
-  p.join = reinterpret_cast<int4*>(ws + o.join);
+  p.join = reinterpret_cast<JoinUnit*>(ws + o.join);
   p.pieces = reinterpret_cast<Piece*>(ws + o.pieces);
   p.part = reinterpret_cast<float*>(ws + o.parts);
   p.min_cells = 4;
   p.split_units = split ? kUnitsPerSm * p.ctas : 0;
   if (p.split_units > kPlanThreads) p.split_units = kPlanThreads;
+  if (p.ctas > kMaxSplitCtas) p.split_units = 0;
   CUtensorMap mq, mk, mv;
   const bool f16 = a->dtype == FA_F16;
   const int64_t g = a->Hq / a->Hkv;
