@@ -22,16 +22,19 @@
 // was never written would reach the output.
 //
 // Work (decided on the device by paged_plan_kernel, from the lengths):
-//  * many units (4 per SM or more): CTAs take whole units from a counter, heads
-//    in groups whose K and V fit half the L2, longest units first;
-//  * few units: every CTA gets the same number of key blocks, L.  A unit of more
-//    than L is cut at L, 2 L, ... and each such part is one CTA's work; what is
-//    left of it, and shorter units, are laid end to end and cut into equal ranges
-//    for the other CTAs.  The parts of one head's units begin at the same keys, so
-//    the CTAs that read them run side by side in the L2: with plain equal ranges
-//    512 tokens over 32768 keys (8 key heads of 128) read the cache from DRAM once
-//    for each of a head's 8 units.  A unit's parts leave (m, l, O) in the workspace
-//    and paged_tiles_join adds them in the order of the keys.
+//  * whole units: CTAs take them from a counter, heads in groups whose K and V
+//    fit half the L2, longest units first.  Of more than 4 units per SM, one that
+//    is longer than a CTA's even share is cut into parts that go first.
+//  * cut units, where there are up to 4 per SM and whole ones would leave CTAs
+//    idle for longer than the parts cost: every CTA gets the same number of key
+//    blocks, L.  A unit of more than L is cut at L, 2 L, ... and each such part is
+//    one CTA's work; what is left of it, and shorter units, are laid end to end and
+//    cut into equal ranges for the other CTAs.  The parts of one head's units begin
+//    at the same keys, so the CTAs that read them run side by side in the L2: with
+//    plain equal ranges 512 tokens over 32768 keys (8 key heads of 128) read the
+//    cache from DRAM once for each of a head's 8 units (244 us, now 221).
+// A unit's parts leave (m, l, O) in the workspace and paged_tiles_join adds them
+// in the order of the keys.
 // Results depend on the lengths alone, never on timing.
 #include <cuda_bf16.h>
 
@@ -49,9 +52,10 @@ constexpr int kThreads = 384;
 constexpr int kRegsCtrl = 72, kRegsSoftmax = 216;
 static_assert(128 * kRegsCtrl + 256 * kRegsSoftmax <= 384 * 168,
               "the register split exceeds the launch's pool");
-constexpr int kUnitsPerSm = 4;       // from here on units are not split
+constexpr int kUnitsPerSm = 4;       // from here on only outliers are cut
 constexpr int kPlanThreads = 640;       // at least the units that may be split
 constexpr int kStartCells = 2;          // what a part's start and end cost, in key blocks
+constexpr int kJoinCells = 8;           // what cutting costs the whole, in key blocks
 constexpr int64_t kGroupBytes = 32ll << 20;   // K and V of the heads worked on at once
 
 // A unit, or the part of one that a CTA computes.
@@ -75,12 +79,12 @@ struct JoinUnit {
 static_assert(sizeof(JoinUnit) == 32, "read as two 16-byte words");
 
 // The plan, at the workspace's start.
-enum : int { kSplit = 0, kUnits = 1, kNext = 2, kJoins = 3, kHeader = 4 };
+enum : int { kSplit = 0, kJoins = 1, kNext = 2, kUnits = 3, kPieces = 4, kLongest = 5, kHeader = 8 };
 struct TileParams : PagedParams {
   int tq;                // tokens of a tile
   int box_rows;          // rows of a load box
   int min_cells;         // least key blocks of a CTA's range
-  int split_units;       // units from which on none is split
+  int split_units;       // units from which on only outliers are cut
   int* plan;             // header
   int* prefix;           // [B + 1]: units (per head) of the sequences before
   int* first;            // [ctas + 1]: first piece of each CTA
@@ -128,6 +132,12 @@ __device__ __forceinline__ void put_piece(Piece* to, const Piece& x) {
   d[0] = make_int4(x.b, x.h, x.tok0, x.q_begin);
   d[1] = make_int4(x.q_len, x.kv_len, x.blk0, x.nt[0]);
   d[2] = make_int4(x.nt[1], x.slot, 0, 0);
+}
+__device__ __forceinline__ void put_join(JoinUnit* to, int slot0, int parts, int tok0,
+                                         const SeqWork& w, int h) {
+  int4* d = reinterpret_cast<int4*>(to);
+  d[0] = make_int4(slot0, parts, tok0, w.begin);
+  d[1] = make_int4(w.q_len, h, 0, 0);
 }
 // The sequence whose units (times heads) hold unit i.
 template <typename I>
@@ -212,13 +222,16 @@ __global__ void __launch_bounds__(kPlanThreads)
   __shared__ int s_blocks[kPlanThreads];                // of (sequence, unit) pairs, one head
   __shared__ int s_prefix[kPlanThreads + 1];
   __shared__ SeqWork s_work[kPlanThreads];
-  __shared__ unsigned s_all, s_fits;
+  __shared__ unsigned long long s_all;
+  __shared__ unsigned s_fits;
+  __shared__ int s_longest, s_joins, s_pieces;
   grid_dependency_wait();
   grid_dependents_launch();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (tid == 0) {
     s_all = 0;
     s_fits = 0;
+    s_longest = s_joins = s_pieces = 0;
   }
   unsigned pairs = 0;                   // (T and B are below 2^31, and so are units)
   for (int b0 = 0; b0 < p.B; b0 += kPlanThreads) {
@@ -240,34 +253,47 @@ __global__ void __launch_bounds__(kPlanThreads)
     p.plan[kNext] = 0;
     if (p.B <= kPlanThreads) s_prefix[p.B] = static_cast<int>(pairs);
   }
-  bool split = static_cast<uint64_t>(pairs) * p.Hkv < static_cast<uint64_t>(p.split_units);
-  int nb = 0;                           // (split_units <= kPlanThreads)
+  const uint64_t units64 = static_cast<uint64_t>(pairs) * p.Hkv;
+  const bool few = units64 < static_cast<uint64_t>(p.split_units);   // (at most kPlanThreads)
   const bool held = p.B <= kPlanThreads;
   const int* prefix = held ? s_prefix : p.prefix;
   auto work = [&](int b) { return held ? s_work[b] : seq_work(p, b); };
+  auto blocks_of_pair = [&](int i) {
+    const int b = seq_of_unit(prefix, p.B, 1, i);
+    return blocks_of(p, work(b), (i - prefix[b]) * 2 * p.tq, 2 * p.tq);
+  };
   __syncthreads();
-  if (split && tid < pairs) {
-    const int b = seq_of_unit(prefix, p.B, 1, tid);
-    nb = blocks_of(p, work(b), (tid - prefix[b]) * 2 * p.tq, 2 * p.tq);
-    s_blocks[tid] = nb;
-  }
-  if (split) {                          // (held to the limit, so that no sum overflows)
-    unsigned sum = tid < pairs ? min(nb + kStartCells, kMaxSplitCells) : 0;
-    sum = __reduce_add_sync(0xffffffffu, sum);
-    if (lane == 0) atomicAdd(&s_all, min(sum, static_cast<unsigned>(kMaxSplitCells)));
-  }
-  __syncthreads();
-  split = split && static_cast<uint64_t>(s_all) * p.Hkv < kMaxSplitCells;
-  if (tid == 0) p.plan[kSplit] = split;
-  if (!split) return;
-  const int units = static_cast<int>(pairs) * p.Hkv;
-
-  // The least cells (key blocks and kStartCells per part) of a CTA, of 20 tried,
-  // with which the work fits the CTAs: a warp tries one.
-  const unsigned all = s_all * p.Hkv;
-  const int least = max(p.min_cells + kStartCells, static_cast<int>((all + p.ctas - 1) / p.ctas));
-  auto tried = [&](int j) { return least + (least * j + 39) / 40; };
+  // All units' cells (key blocks and kStartCells) and the longest unit.
   {
+    uint64_t sum = 0;
+    int longest = 0;
+    for (int i = tid; i < static_cast<int>(pairs); i += kPlanThreads) {
+      const int nb = blocks_of_pair(i);
+      if (i < kPlanThreads) s_blocks[i] = nb;
+      sum += nb + kStartCells;
+      longest = max(longest, nb);
+    }
+    longest = __reduce_max_sync(0xffffffffu, longest);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) {
+      atomicAdd(&s_all, static_cast<unsigned long long>(sum));
+      atomicMax(&s_longest, longest);
+    }
+  }
+  __syncthreads();
+  const uint64_t all64 = s_all * static_cast<uint64_t>(p.Hkv);
+  const int longest = s_longest;
+  const int units = static_cast<int>(units64);
+
+  // The least cells of a CTA, of 20 tried, with which cut units fit the CTAs: a
+  // warp tries one.
+  const bool can_cut = few && all64 < kMaxSplitCells;
+  const unsigned all = static_cast<unsigned>(all64);
+  const int least =
+      can_cut ? max(p.min_cells + kStartCells, static_cast<int>((all + p.ctas - 1) / p.ctas)) : 0;
+  auto tried = [&](int j) { return least + (least * j + 39) / 40; };
+  if (can_cut) {
     const int cells = tried(warp);
     unsigned whole = 0, rest = 0;
     for (int i = lane; i < static_cast<int>(pairs); i += 32) {
@@ -284,6 +310,42 @@ __global__ void __launch_bounds__(kPlanThreads)
   // (2 * least always fits: a part's start is a third of it at most)
   const int cells = s_fits ? tried(__ffs(s_fits) - 1) : 2 * least;
   const int L = cells - kStartCells;
+  // Whole units end about a sixth of the longest after their even share, and not
+  // before the longest; cut ones after their share and the join.
+  const int end_whole =
+      max(longest + kStartCells, units <= p.ctas ? 0 : least + longest / 6);
+  const bool split = can_cut && cells + kJoinCells < end_whole;
+  if (!split) {
+    // A share's length for outliers; none is cut among few units.
+    const uint64_t share = few ? static_cast<uint64_t>(INT_MAX)
+                               : max(static_cast<uint64_t>(p.min_cells), all64 / p.ctas);
+    const int most = p.split_units > 0 && share < INT_MAX ? static_cast<int>(share) : INT_MAX;
+    if (longest > most) {
+      for (int i = tid; i < static_cast<int>(pairs); i += kPlanThreads) {
+        const int nb = blocks_of_pair(i);
+        if (nb <= most) continue;
+        const int b = seq_of_unit(prefix, p.B, 1, i);
+        const SeqWork w = work(b);
+        const int parts = (nb + most - 1) / most, len = (nb + parts - 1) / parts;
+        const int join0 = atomicAdd(&s_joins, p.Hkv), piece0 = atomicAdd(&s_pieces, parts * p.Hkv);
+        for (int h = 0; h < p.Hkv; ++h) {
+          put_join(p.join + join0 + h, piece0 + h * parts, parts, (i - prefix[b]) * 2 * p.tq, w, h);
+          for (int k = 0; k < parts; ++k)
+            put_piece(p.pieces + piece0 + h * parts + k,
+                      make_piece(p, w, b, h, i - prefix[b], k * len, min(nb, (k + 1) * len),
+                                 piece0 + h * parts + k));
+        }
+      }
+      __syncthreads();
+    }
+    if (tid == 0) {
+      p.plan[kSplit] = 0;
+      p.plan[kJoins] = s_joins;
+      p.plan[kPieces] = s_pieces;
+      p.plan[kLongest] = most;
+    }
+    return;
+  }
 
   // Units in the order (sequence, head, unit).
   int b = 0, h = 0, u = 0;
@@ -336,12 +398,11 @@ __global__ void __launch_bounds__(kPlanThreads)
             static_cast<unsigned>(c0))
       p.first[ctas_whole + c0 + i] = piece0 + i;
   }
-  if (!alone) {
-    int4* d = reinterpret_cast<int4*>(p.join + (before >> 21));
-    d[0] = make_int4(slot0, parts, u * 2 * p.tq, w.begin);
-    d[1] = make_int4(w.q_len, h, 0, 0);
+  if (!alone) put_join(p.join + (before >> 21), slot0, parts, u * 2 * p.tq, w, h);
+  if (tid == 0) {
+    p.plan[kSplit] = 1;
+    p.plan[kJoins] = total >> 21;
   }
-  if (tid == 0) p.plan[kJoins] = total >> 21;
   if (tid <= p.ctas && tid >= ctas_whole + ctas_rest) p.first[tid] = pieces;
 }
 
@@ -550,9 +611,21 @@ __global__ void __launch_bounds__(kThreads, 1)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsCtrl) : "memory");
     if (warp == 8) {
       // =================== loads of Q and K ===================
-      const bool split = p.plan[kSplit] != 0;
-      int64_t next = split ? p.first[blockIdx.x] : static_cast<int>(blockIdx.x);
-      const int64_t stop = split ? p.first[blockIdx.x + 1] : p.plan[kUnits];
+      // (all loaded at once, whichever of them are used)
+      const int4 plan0 = reinterpret_cast<const int4*>(p.plan)[0];
+      const int4 plan1 = reinterpret_cast<const int4*>(p.plan)[1];
+      const int first = p.first[blockIdx.x], behind = p.first[blockIdx.x + 1];
+      static_assert(kSplit == 0 && kUnits == 3 && kPieces == 4 && kLongest == 5, "header words");
+      const bool split = plan0.x != 0;
+      const int pieces = split ? 0 : plan1.x, longest = plan1.y;
+      int64_t next = split ? first : static_cast<int>(blockIdx.x);
+      const int64_t stop = split ? behind : static_cast<int64_t>(pieces) + plan0.w;
+      auto take_next = [&] {
+        if (split) return next + 1;
+        int got = 0;
+        if (lane == 0) got = atomicAdd(p.plan + kNext, 1);
+        return static_cast<int64_t>(gridDim.x) + __shfl_sync(0xffffffffu, got, 0);
+      };
       const uint64_t pol_q = l2_policy_evict_first();
       int blocks = 0;       // K tiles issued, over all pieces
       int uc = 0;           // pieces with keys
@@ -560,8 +633,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int us = take & 1;
         if (take >= 2 && !wwait(bar_unit_empty(us), ((take >> 1) - 1) & 1)) break;
         Piece x;
-        if (next < stop) x = split ? p.pieces[next] : whole_unit(p, next);
-        else x.h = -1;
+        x.h = -1;
+        for (; next < stop; next = take_next()) {
+          x = split || next < pieces ? p.pieces[next] : whole_unit(p, next - pieces);
+          // (a unit whose parts are pieces is not taken whole)
+          if (split || next < pieces || max(x.nt[0], x.nt[1]) <= longest) break;
+          x.h = -1;
+        }
         if (lane == 0) {
           volatile Piece* d = ring + us;
           d->b = x.b;
@@ -595,13 +673,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           ++uc;
           if (!load_keys(&tmK, 0, x.b, x.h, x.kv_len, x.blk0, n, blocks)) break;
         }
-        if (split) {
-          ++next;
-        } else {
-          int got = 0;
-          if (lane == 0) got = atomicAdd(p.plan + kNext, 1);
-          next = static_cast<int64_t>(gridDim.x) + __shfl_sync(0xffffffffu, got, 0);
-        }
+        next = take_next();
       }
       if (*abort_flag && lane == 0) {
         // Let the copies in flight land before the CTA exits.
@@ -924,6 +996,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 // channels of them.
 // Bound by HBM: each part is read once.
 constexpr int kJoinWarps = 8;
+constexpr int kJoinGroups = 2 * kRows / 32;             // groups of 32 rows of a unit
 template <int D, bool F16>
 __global__ void __launch_bounds__(32 * kJoinWarps)
     paged_tiles_join(const TileParams p) {
@@ -934,87 +1007,87 @@ __global__ void __launch_bounds__(32 * kJoinWarps)
   __shared__ int64_t s_off[32];
   grid_dependency_wait();
   grid_dependents_launch();
-  // (the unit is loaded along with the count that says whether there is one)
-  const int4 head = *reinterpret_cast<const int4*>(p.plan);
-  const int4 j0 = reinterpret_cast<const int4*>(p.join + blockIdx.x)[0];
-  const int4 j1 = reinterpret_cast<const int4*>(p.join + blockIdx.x)[1];
-  static_assert(kSplit == 0 && kJoins == 3, "order of the header's words");
-  if (head.x == 0 || static_cast<int>(blockIdx.x) >= head.w) return;
-  const int slot0 = j0.x, parts = j0.y, tok0 = j0.z, q_begin = j0.w, q_len = j1.x, h = j1.y;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int t = blockIdx.y / (kRows / 32);
-  const int row = (blockIdx.y % (kRows / 32)) * 32 + lane;    // of the tile
-  const int row_tok = row / p.g;
-  const int tok = tok0 + t * p.tq + row_tok;
-  const bool live = row_tok < p.tq && tok < q_len;
-  if (!__any_sync(0xffffffffu, live)) return;                 // (the same in every warp)
-  const float* part = p.part + static_cast<int64_t>(slot0) * C::kSlot;
-  const int at_m = 2 * kRows * D + t * kRows + row, at_l = at_m + 2 * kRows;
-  const int at_o = (t * (D / 4) + warp * E) * kRows + row;
-  float top = -INFINITY, sum = 0.f;
-  float4 acc[E];
+  const int items = p.plan[kJoins] * kJoinGroups;
+  for (int item = blockIdx.x; item < items; item += gridDim.x) {
+    const int4 j0 = reinterpret_cast<const int4*>(p.join + item / kJoinGroups)[0];
+    const int4 j1 = reinterpret_cast<const int4*>(p.join + item / kJoinGroups)[1];
+    const int slot0 = j0.x, parts = j0.y, tok0 = j0.z, q_begin = j0.w, q_len = j1.x, h = j1.y;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int t = item % kJoinGroups / (kRows / 32);
+    const int row = item % (kRows / 32) * 32 + lane;            // of the tile
+    const int row_tok = row / p.g;
+    const int tok = tok0 + t * p.tq + row_tok;
+    const bool live = row_tok < p.tq && tok < q_len;
+    if (!__any_sync(0xffffffffu, live)) continue;               // (the same in every warp)
+    const float* part = p.part + static_cast<int64_t>(slot0) * C::kSlot;
+    const int at_m = 2 * kRows * D + t * kRows + row, at_l = at_m + 2 * kRows;
+    const int at_o = (t * (D / 4) + warp * E) * kRows + row;
+    float top = -INFINITY, sum = 0.f;
+    float4 acc[E];
 #pragma unroll
-  for (int e = 0; e < E; ++e) acc[e] = make_float4(0.f, 0.f, 0.f, 0.f);
-  // kAhead parts at a time, all of their loads in flight together.
-  constexpr int kAhead = 4;
-  for (int i0 = 0; live && i0 < parts; i0 += kAhead) {
-    float m[kAhead], l[kAhead];
-    float4 o[kAhead][E];
-    float now = top;
+    for (int e = 0; e < E; ++e) acc[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+    // kAhead parts at a time, all of their loads in flight together.
+    constexpr int kAhead = 4;
+    for (int i0 = 0; live && i0 < parts; i0 += kAhead) {
+      float m[kAhead], l[kAhead];
+      float4 o[kAhead][E];
+      float now = top;
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      const bool in = i0 + k < parts;
-      const float* s = part + static_cast<int64_t>(in ? i0 + k : i0) * C::kSlot;
-      m[k] = in ? s[at_m] : -INFINITY;
-      l[k] = in ? s[at_l] : 0.f;
+      for (int k = 0; k < kAhead; ++k) {
+        const bool in = i0 + k < parts;
+        const float* s = part + static_cast<int64_t>(in ? i0 + k : i0) * C::kSlot;
+        m[k] = in ? s[at_m] : -INFINITY;
+        l[k] = in ? s[at_l] : 0.f;
 #pragma unroll
-      for (int e = 0; e < E; ++e) o[k][e] = reinterpret_cast<const float4*>(s)[at_o + e * kRows];
-    }
-#pragma unroll
-    for (int k = 0; k < kAhead; ++k) now = fmaxf(now, m[k]);
-    const float keep = top == -INFINITY ? 0.f : ex2_approx(top - now);
-    sum *= keep;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      acc[e].x *= keep;
-      acc[e].y *= keep;
-      acc[e].z *= keep;
-      acc[e].w *= keep;
-    }
-#pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      if (m[k] == -INFINITY) {          // saw none of these keys: O was not written
-        sum += l[k];
-        continue;
+        for (int e = 0; e < E; ++e) o[k][e] = reinterpret_cast<const float4*>(s)[at_o + e * kRows];
       }
-      const float al = ex2_approx(m[k] - now);
-      sum += l[k] * al;
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) now = fmaxf(now, m[k]);
+      const float keep = top == -INFINITY ? 0.f : ex2_approx(top - now);
+      sum *= keep;
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        acc[e].x += o[k][e].x * al;
-        acc[e].y += o[k][e].y * al;
-        acc[e].z += o[k][e].z * al;
-        acc[e].w += o[k][e].w * al;
+        acc[e].x *= keep;
+        acc[e].y *= keep;
+        acc[e].z *= keep;
+        acc[e].w *= keep;
       }
-    }
-    top = now;
-  }
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
-  for (int e = 0; e < E; ++e)
-    *reinterpret_cast<uint2*>(s_out + lane * kRowBytes + (warp * E + e) * 8) =
-        make_uint2(pack_16x2<F16>(acc[e].x * inv, acc[e].y * inv),
-                   pack_16x2<F16>(acc[e].z * inv, acc[e].w * inv));
-  if (warp == 0)
-    s_off[lane] = live ? static_cast<int64_t>(q_begin + tok) * p.o_st +
-                             static_cast<int64_t>(h * p.g + row - row_tok * p.g) * p.o_sh
-                       : -1;
-  __syncthreads();
-  for (int i = threadIdx.x; i < 32 * (D / 8); i += 32 * kJoinWarps) {
-    const int r = i / (D / 8), d = (i - r * (D / 8)) * 8;
-    if (s_off[r] >= 0 && d < p.D)
-      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.o) + s_off[r] + d) =
-          *reinterpret_cast<const uint4*>(s_out + r * kRowBytes + d * 2);
+      for (int k = 0; k < kAhead; ++k) {
+        if (m[k] == -INFINITY) {          // saw none of these keys: O was not written
+          sum += l[k];
+          continue;
+        }
+        const float al = ex2_approx(m[k] - now);
+        sum += l[k] * al;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          acc[e].x += o[k][e].x * al;
+          acc[e].y += o[k][e].y * al;
+          acc[e].z += o[k][e].z * al;
+          acc[e].w += o[k][e].w * al;
+        }
+      }
+      top = now;
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      *reinterpret_cast<uint2*>(s_out + lane * kRowBytes + (warp * E + e) * 8) =
+          make_uint2(pack_16x2<F16>(acc[e].x * inv, acc[e].y * inv),
+                     pack_16x2<F16>(acc[e].z * inv, acc[e].w * inv));
+    if (warp == 0)
+      s_off[lane] = live ? static_cast<int64_t>(q_begin + tok) * p.o_st +
+                               static_cast<int64_t>(h * p.g + row - row_tok * p.g) * p.o_sh
+                         : -1;
+    __syncthreads();
+    for (int i = threadIdx.x; i < 32 * (D / 8); i += 32 * kJoinWarps) {
+      const int r = i / (D / 8), d = (i - r * (D / 8)) * 8;
+      if (s_off[r] >= 0 && d < p.D)
+        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.o) + s_off[r] + d) =
+            *reinterpret_cast<const uint4*>(s_out + r * kRowBytes + d * 2);
+    }
+    __syncthreads();
   }
 }
 
@@ -1025,25 +1098,15 @@ int tile_tokens(const fa_paged_attn_args* a) {
   return static_cast<int>(kRows / (a->Hq / a->Hkv));
 }
 
-// Whether the device may find few enough units to split some: rows outside
-// every sequence and short sequences make units fewer than T gives, so only a
-// T of twice the limit rules it out.
-bool may_split(const fa_paged_attn_args* a, int sms) {
-  const int64_t least = a->T / (2 * tile_tokens(a)) * a->Hkv;
-  return least < 2ll * kUnitsPerSm * sms;
-}
-
 PlanOffsets plan_offsets(const fa_paged_attn_args* a, int sms) {
   PlanOffsets o;
   o.prefix = up128(kHeader * 4);
   o.first = o.prefix + up128((a->B + 1) * 4);
   o.join = o.first + up128((sms + 1) * 4);
   o.pieces = o.join + up128(sms * static_cast<int64_t>(sizeof(JoinUnit)));
-  const bool split = may_split(a, sms);
-  const int64_t most = split ? kUnitsPerSm * sms + sms : 0;
-  o.parts = o.pieces + up128(most * static_cast<int64_t>(sizeof(Piece)));
+  o.parts = o.pieces + up128((kUnitsPerSm + 1) * sms * static_cast<int64_t>(sizeof(Piece)));
   const int d = a->D <= 64 ? 64 : 128;
-  o.bytes = o.parts + (split ? 2ll * sms * 2 * kRows * (d + 2) * 4 : 0);
+  o.bytes = o.parts + 2ll * sms * 2 * kRows * (d + 2) * 4;   // a CTA ends and begins a part
   return o;
 }
 
@@ -1067,7 +1130,7 @@ int make_map(CUtensorMap* map, const void* ptr, const int64_t (&dims)[4],
 
 template <int D, bool F16>
 int launch_tiles(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
-                 const TileParams& p, bool split, cudaStream_t stream) {
+                 const TileParams& p, cudaStream_t stream) {
   using C = Cfg<D>;
   static KernelPrep prep;
   int dev = 0;
@@ -1078,8 +1141,8 @@ int launch_tiles(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap
   if (rc != FA_OK) return rc;
   rc = launch_after(paged_tiles_kernel<D, F16>, dim3(p.ctas), kThreads, C::kSmemBytes, stream, mq,
                     mk, mv, p);
-  if (rc != FA_OK || !split) return rc;
-  return launch_after(paged_tiles_join<D, F16>, dim3(p.ctas, 2 * kRows / 32),
+  if (rc != FA_OK) return rc;
+  return launch_after(paged_tiles_join<D, F16>, dim3(2 * p.ctas),
                       32 * kJoinWarps, 0, stream, p);
 }
 
@@ -1097,7 +1160,6 @@ int launch_paged_tiles(const fa_paged_attn_args* a, const PagedParams& q, void* 
   p.box_rows = a->page_size < kKeys ? static_cast<int>(a->page_size) : kKeys;
   // (the exponent's scale is kept off zero: -inf * 0 of a masked score is no number)
   if (p.scale_log2 < 1e-30f) p.scale_log2 = 1e-30f;
-  const bool split = may_split(a, p.ctas);
   const PlanOffsets o = plan_offsets(a, p.ctas);
   char* ws = static_cast<char*>(workspace);
   p.plan = reinterpret_cast<int*>(ws);
@@ -1107,7 +1169,7 @@ int launch_paged_tiles(const fa_paged_attn_args* a, const PagedParams& q, void* 
   p.pieces = reinterpret_cast<Piece*>(ws + o.pieces);
   p.part = reinterpret_cast<float*>(ws + o.parts);
   p.min_cells = 4;
-  p.split_units = split ? kUnitsPerSm * p.ctas : 0;
+  p.split_units = kUnitsPerSm * p.ctas;
   if (p.split_units > kPlanThreads) p.split_units = kPlanThreads;
   if (p.ctas > kMaxSplitCtas) p.split_units = 0;
   CUtensorMap mq, mk, mv;
@@ -1128,10 +1190,10 @@ int launch_paged_tiles(const fa_paged_attn_args* a, const PagedParams& q, void* 
                 {rows, 1, 1}, f16);
   if (rc != FA_OK) return rc;
   if (a->D <= 64)
-    return f16 ? launch_tiles<64, true>(mq, mk, mv, p, split, stream)
-               : launch_tiles<64, false>(mq, mk, mv, p, split, stream);
-  return f16 ? launch_tiles<128, true>(mq, mk, mv, p, split, stream)
-             : launch_tiles<128, false>(mq, mk, mv, p, split, stream);
+    return f16 ? launch_tiles<64, true>(mq, mk, mv, p, stream)
+               : launch_tiles<64, false>(mq, mk, mv, p, stream);
+  return f16 ? launch_tiles<128, true>(mq, mk, mv, p, stream)
+             : launch_tiles<128, false>(mq, mk, mv, p, stream);
 }
 
 }  // namespace fa

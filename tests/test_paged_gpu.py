@@ -101,6 +101,21 @@ def test_units_that_fill_the_device(causal):
     _check([300, 1100], [300, 1300], 128, 64, 128, 64, F16, causal=causal)
 
 
+def test_long_units_among_many():
+    """720 and more units, the longest of them beyond a CTA's even share of the key blocks: those
+    are cut, the others are not."""
+    _check([40] + [1] * 89, [6000] + [100 - i for i in range(89)], 8, 8, 64, 16)
+    _check([3, 200, 9] + [1] * 250, [900, 7000, 5000] + [50] * 250, 8, 4, 128, 16, F16)
+    _check([40] * 100, [4000] + [40] * 98 + [9000], 8, 8, 64, 32, causal=False)
+
+
+@pytest.mark.parametrize("q_lens,kv_lens", [([520], [9000]), ([64, 700], [20000, 6000]),
+                                            ([300] * 3, [4100, 4096, 300]), ([33], [33000])])
+def test_units_cut_over_the_device(q_lens, kv_lens):
+    _check(q_lens, kv_lens, 8, 2, 128, 64)
+    _check(q_lens, kv_lens, 2, 1, 64, 32, F16, causal=False)
+
+
 def test_rows_that_see_nothing():
     """kv_lens below the number of new tokens (0 among them): the tokens before the start see
     no key under the causal mask and get zeros."""
