@@ -83,6 +83,7 @@ struct Range {
   int64_t start, end, per;
   int64_t base;          // first key block of sequence b
   int b;
+  RowWork work;          // of sequence b
 };
 
 template <bool LAST>
@@ -90,16 +91,19 @@ __device__ __forceinline__ Range find_range(const PagedParams& p, int team, int 
   __shared__ int64_t red[kRowWarps];
   __shared__ int64_t s_base;
   __shared__ int s_b;
+  __shared__ RowWork s_work;
   Range r;
   int64_t total = 0;
-  int64_t first_w = 0, first_before = 0;      // the scan of the first kRowThreads sequences
+  RowWork first = {};                         // the first kRowThreads sequences': kept
+  int64_t first_before = 0;
   for (int b0 = 0; b0 < p.B; b0 += kRowThreads) {
     const int b = b0 + threadIdx.x;
-    const int64_t w = b < p.B ? weight(p, row_work(p, b, tile_rows)) : 0;
+    RowWork w = {};
+    if (b < p.B) w = row_work(p, b, tile_rows);
     int64_t sum;
-    const int64_t before = block_scan(w, red, &sum);
+    const int64_t before = block_scan(weight(p, w), red, &sum);
     if (b0 == 0) {
-      first_w = w;
+      first = w;
       first_before = before;
     }
     total += sum;
@@ -114,21 +118,25 @@ __device__ __forceinline__ Range find_range(const PagedParams& p, int team, int 
     int64_t base = 0;
     for (int b0 = 0; b0 < p.B; b0 += kRowThreads) {
       const int b = b0 + threadIdx.x;
-      int64_t w = first_w, before = first_before, sum = 0;
+      RowWork w = first;
+      int64_t before = first_before, sum = 0;
       if (p.B > kRowThreads) {
-        w = b < p.B ? weight(p, row_work(p, b, tile_rows)) : 0;
-        before = block_scan(w, red, &sum);
+        w = {};
+        if (b < p.B) w = row_work(p, b, tile_rows);
+        before = block_scan(weight(p, w), red, &sum);
       }
-      if (w > 0 && base + before <= at && at < base + before + w) {
+      if (base + before <= at && at < base + before + weight(p, w)) {
         s_b = b;
         s_base = base + before;
+        s_work = w;
       }
       base += sum;
     }
   }
   __syncthreads();
   r.b = s_b;
-  r.base = r.b < p.B ? s_base : 0;
+  r.base = s_base;
+  r.work = s_work;
   return r;
 }
 
@@ -216,9 +224,13 @@ __global__ void __launch_bounds__(RowCfg<DT, MT, CUT>::kThreads, RowCfg<DT, MT, 
 
   Range rg = {};
   int tile = 0;                         // whole units: this CTA's row tile
+  int ahead = 0;                        // and a page, loaded along with the lengths
   if (WHOLE) {
     rg.b = blockIdx.x / p.team / p.tile_ctas;
     tile = blockIdx.x / p.team % p.tile_ctas;
+    const int at = (warp * 16 + lane * C::kStep) >> p.page_shift;
+    if (at < p.max_pages) ahead = p.table[rg.b * p.table_stride + at];
+    rg.work = row_work(p, rg.b, C::kRows);
   } else {
     rg = find_range<false>(p, blockIdx.x / p.team, C::kRows);
     if (rg.start >= rg.end) return;
@@ -231,7 +243,7 @@ __global__ void __launch_bounds__(RowCfg<DT, MT, CUT>::kThreads, RowCfg<DT, MT, 
 
   int b = rg.b;
   int64_t base = rg.base, cur = rg.start;
-  RowWork w = row_work(p, b, C::kRows);
+  RowWork w = rg.work;
   if (WHOLE) {
     if (tile >= w.tiles) return;
     cur = static_cast<int64_t>(tile) * w.blocks;
@@ -256,7 +268,10 @@ __global__ void __launch_bounds__(RowCfg<DT, MT, CUT>::kThreads, RowCfg<DT, MT, 
     const int32_t* trow = p.table + b * p.table_stride;
     auto page_of = [&](int s) {
       if (s >= steps) return 0;
-      const int pg = page_at(trow, key00 + s * C::kStep, p.page_shift, p.max_pages, p.pages);
+      // (a whole unit's first 32 pages are at hand: its blocks begin at key 0)
+      const int pg = WHOLE && s < 32 ? (ahead >= 0 && ahead < p.pages ? ahead : -1)
+                                     : page_at(trow, key00 + s * C::kStep, p.page_shift,
+                                               p.max_pages, p.pages);
       if (pg < 0) atomicExch(p.status, kDevBadPage);
       return pg;
     };
@@ -535,7 +550,7 @@ __global__ void __launch_bounds__(kRowThreads)
   grid_dependency_wait();
   grid_dependents_launch();
   if (rg.start >= rg.end) return;
-  const RowWork w = row_work(p, rg.b, C::kRows);
+  const RowWork w = rg.work;
   const int unit = static_cast<int>((rg.end - 1 - rg.base) / w.blocks);
   const int64_t us = rg.base + static_cast<int64_t>(unit) * w.blocks, ue = us + w.blocks;
   if (us < rg.start || ue <= rg.end) return;
