@@ -86,7 +86,7 @@ def _binding_command() -> list:
              "-I" + sysconfig.get_paths()["include"], "-I" + os.path.join(root, "include"),
              "-I" + os.path.join(root, "include", "torch", "csrc", "api", "include"),
              "-I" + cuda, BINDING_SOURCE, "-L" + os.path.join(root, "lib"), "-ltorch_python",
-             "-ltorch_cpu", "-ltorch", "-lc10", "-lc10_cuda"])
+             "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-lc10", "-lc10_cuda"])
 
 
 def build(force: bool = False, verbose: bool = False) -> str:

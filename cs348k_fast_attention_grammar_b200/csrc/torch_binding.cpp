@@ -8,6 +8,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -157,7 +158,7 @@ void check(int rc, const char* where) {
 }
 
 at::Tensor make(at::IntArrayRef sizes, at::ScalarType type, const c10::Device& device) {
-  return at::empty(sizes, at::TensorOptions().dtype(type).device(device));
+  return at::detail::empty_cuda(sizes, type, device, c10::nullopt);
 }
 
 PyObject* given(PyObject* o) {
