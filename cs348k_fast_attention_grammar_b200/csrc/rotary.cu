@@ -23,7 +23,8 @@
 namespace fa {
 namespace {
 
-constexpr int kRotThreads = 192;
+constexpr int kRotThreads = 192;        // 192 x 4 items: 2 rows of 384, 3 of 256, 6 of 128
+constexpr int kRotCtasPerSm = 8;        // by registers
 constexpr int kRotBatches = 4;          // goes of a CTA over its items
 constexpr int kRotMaxRows = 64;         // rows of one CTA
 constexpr int kRotMaxAngles = 2048;     // angles of one CTA (16 KiB of shared memory)
@@ -155,7 +156,7 @@ struct Item {
 
 // APPEND: rows are packed new tokens, keys and values go to their pages.
 template <int TYPE, bool APPEND, bool INTERLEAVED>
-__global__ void __launch_bounds__(kRotThreads, 8)
+__global__ void __launch_bounds__(kRotThreads, kRotCtasPerSm)
     rotary_kernel(const RotParams p) {
   constexpr int kSize = Elem<TYPE>::kSize;
   constexpr int V = 16 / kSize;
@@ -333,16 +334,18 @@ int launch_rotary(RotParams& p, int dtype, bool append, bool interleaved, cudaSt
     q.count = q.heads * q.items;
     p.items_per_row += q.count;
   }
-  // Rows per CTA: what its threads take in kRotBatches goes (a row's place takes
-  // a chain of loads that the goes share), within the shared memory for their
-  // angles, and no more than leave every SM eight CTAs.
+  // Rows per CTA: at most what its threads take in kRotBatches goes (a row's place
+  // takes a chain of loads that the goes share), within the shared memory for
+  // their angles, and so many that the CTAs fill whole waves of the device: 16
+  // heads, 64 of 128 channels turned, 4636 tokens: 26.3 us in 1.3 waves, 23.7 in
+  // two.
   int rows = kRotBatches * kRotThreads / p.items_per_row;
-  const int sms = sm_count(dev);
-  if (sms > 0 && p.rows < 8ll * rows * sms)
-    rows = static_cast<int>((p.rows + 8 * sms - 1) / (8 * sms));
   if (half > 0) rows = rows < kRotMaxAngles / half ? rows : kRotMaxAngles / half;
   rows = rows < kRotMaxRows ? rows : kRotMaxRows;
-  p.rows_per_cta = rows > 1 ? rows : 1;
+  if (rows < 1) rows = 1;
+  const int64_t wave = static_cast<int64_t>(kRotCtasPerSm) * (sm_count(dev) > 0 ? sm_count(dev) : 1);
+  const int64_t waves = (p.rows + rows * wave - 1) / (rows * wave);
+  p.rows_per_cta = static_cast<int>((p.rows + waves * wave - 1) / (waves * wave));
   const int64_t grid = (p.rows + p.rows_per_cta - 1) / p.rows_per_cta;
   if (grid > 0x7fffffffLL) return FA_ERR_SHAPE;
   const unsigned g = static_cast<unsigned>(grid);
