@@ -54,21 +54,27 @@ int make_tmap_bhsd(CUtensorMap* map, const void* base, int B, int H, int S, int 
 
 // Launches a kernel as a programmatic dependent of the one before it in the
 // stream: it may start while that one ends, and calls grid_dependency_wait()
-// before it touches memory.
+// before it touches memory.  `cluster`: CTAs of a thread-block cluster.
 template <typename... Args>
-inline int launch_after(void (*kern)(Args...), dim3 grid, int threads, int smem, cudaStream_t stream,
-                 const Args&... args) {
+inline int launch_after(void (*kern)(Args...), dim3 grid, int threads, int smem, int cluster,
+                        cudaStream_t stream, const Args&... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kern, args...) == cudaSuccess ? FA_OK : FA_ERR_LAUNCH;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  if (cudaLaunchKernelEx(&cfg, kern, args...) == cudaSuccess) return FA_OK;
+  (void)cudaGetLastError();
+  return FA_ERR_LAUNCH;
 }
 
 }  // namespace fa

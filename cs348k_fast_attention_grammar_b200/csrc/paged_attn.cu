@@ -25,9 +25,11 @@
 // on timing.
 #include <cuda_bf16.h>
 
+#include <atomic>
 #include <cmath>
 
 #include "paged_attn.h"
+#include "sm100_2sm.cuh"
 
 namespace fa {
 namespace {
@@ -182,10 +184,31 @@ __device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4],
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// A value from the shared memory of CTA `cta` of the cluster, at this CTA's address.
+__device__ __forceinline__ float cluster_load(uint32_t addr, int cta) {
+  uint32_t a;
+  float v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(cta));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 cluster_load4(uint32_t addr, int cta) {
+  uint32_t a;
+  float4 v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(cta));
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(a)
+               : "memory");
+  return v;
+}
+
 // How a launch cuts its work: ranges of key blocks for teams of CTAs, joined
 // afterwards; a CTA per sequence, head and row tile; the same with more warps,
-// for fewer CTAs than SMs, where a warp's chain of 16-key steps (about 900 clocks
-// each with one warp per scheduler) is what a call waits for.
+// and a cluster of up to 8 CTAs instead of one, for fewer CTAs than SMs, where a
+// warp's chain of 16-key steps (about 900 clocks each with one warp per scheduler)
+// is what a call waits for.  The cluster's CTAs take turns at the steps and add
+// their results up through each other's shared memory.
 enum Cut { kSplit, kWhole, kWholeWide };
 
 template <int DT, int MT, Cut CUT = kSplit>
@@ -194,6 +217,8 @@ struct RowCfg {
   static constexpr int kWarps = CUT == kWholeWide ? (DT == 64 ? 16 : 8) : kRowWarps;
   static constexpr int kThreads = 32 * kWarps;
   static constexpr int kStep = 16 * kWarps;              // keys of the CTA's steps
+  static constexpr int kStepLog2 = kWarps == 16 ? 8 : kWarps == 8 ? 7 : 6;
+  static_assert(1 << kStepLog2 == kStep, "steps are powers of two");
   // Ring steps by shared memory (CTAs per SM also by registers).
   static constexpr int kStages = DT == 64 && MT == 2 ? 6 : 3;
   static constexpr int kCtasPerSm = CUT == kWholeWide ? 1 : DT == 64 && MT == 1 ? 4 : 2;
@@ -201,8 +226,9 @@ struct RowCfg {
   static constexpr int kStage = 2 * kTile;
   static constexpr int kWarp = kStages * kStage;
   static constexpr int kRing = kWarps * kWarp;
-  static constexpr int kSmem = kRing + 2 * kWarps * kRows * 4;   // + m, l of each warp
   static constexpr int kSlot = kRows * (DT + 2);         // floats of a partial result
+  static constexpr int kSumOff = kRing + 2 * kWarps * kRows * 4;   // m, l of each warp before it
+  static constexpr int kSmem = kSumOff + (CUT == kWholeWide ? kSlot * 4 : 0);
   static_assert(kWarps * kRows * DT * 4 <= kRing, "the joined output reuses the ring");
 };
 
@@ -225,14 +251,21 @@ __global__ void __launch_bounds__(RowCfg<DT, MT, CUT>::kThreads, RowCfg<DT, MT, 
   Range rg = {};
   int tile = 0;                         // whole units: this CTA's row tile
   int ahead = 0;                        // and a page, loaded along with the lengths
+  // This warp's first key of a block or unit, and how far its steps are apart.
+  const int cshift = CUT == kWholeWide ? p.cluster_shift : 0;
+  const int cluster = 1 << cshift;
+  const unsigned rank = blockIdx.x & (cluster - 1), cta = blockIdx.x >> cshift;
+  const int warp_key = (rank * C::kWarps + warp) * 16;
+  const int step_keys = C::kStep << cshift;
   if (WHOLE) {
-    rg.b = blockIdx.x / p.team / p.tile_ctas;
-    tile = blockIdx.x / p.team % p.tile_ctas;
-    const int at = (warp * 16 + lane * C::kStep) >> p.page_shift;
+    const unsigned team = cta / static_cast<unsigned>(p.team);
+    rg.b = team / static_cast<unsigned>(p.tile_ctas);
+    tile = team - rg.b * p.tile_ctas;
+    const int at = (warp_key + lane * step_keys) >> p.page_shift;
     if (at < p.max_pages) ahead = p.table[rg.b * p.table_stride + at];
     rg.work = row_work(p, rg.b, C::kRows);
   } else {
-    rg = find_range<false>(p, blockIdx.x / p.team, C::kRows);
+    rg = find_range<false>(p, cta / p.team, C::kRows);
     if (rg.start >= rg.end) return;
   }
   const int page_mask = (1 << p.page_shift) - 1;
@@ -255,22 +288,22 @@ __global__ void __launch_bounds__(RowCfg<DT, MT, CUT>::kThreads, RowCfg<DT, MT, 
     const int blk0 = static_cast<int>(in_seq - static_cast<int64_t>(unit) * w.blocks);
     const int nblk = static_cast<int>(min(static_cast<int64_t>(w.blocks - blk0), rg.end - cur));
     const int group = unit / w.tiles;
-    const int h = group * p.team + blockIdx.x % p.team;
+    const int h = group * p.team + cta % p.team;
     const int row0 = (unit - group * w.tiles) * C::kRows;
     const int rows = min(C::kRows, w.q_len * p.g - row0);      // of this tile
 
     const int tile_seen = min(w.kv_len, seen_keys(p, w, (row0 + rows - 1) / p.g));
 
     // This warp's 16-key steps of the blocks: those that some row sees.
-    const int key00 = blk0 * kRowKeys + warp * 16;
+    const int key00 = blk0 * kRowKeys + warp_key;
     const int key_end = min(tile_seen, (blk0 + nblk) * kRowKeys);
-    const int steps = key00 < key_end ? (key_end - key00 + C::kStep - 1) / C::kStep : 0;
+    const int steps = key00 < key_end ? (key_end - key00 + step_keys - 1) >> (C::kStepLog2 + cshift) : 0;
     const int32_t* trow = p.table + b * p.table_stride;
     auto page_of = [&](int s) {
       if (s >= steps) return 0;
       // (a whole unit's first 32 pages are at hand: its blocks begin at key 0)
       const int pg = WHOLE && s < 32 ? (ahead >= 0 && ahead < p.pages ? ahead : -1)
-                                     : page_at(trow, key00 + s * C::kStep, p.page_shift,
+                                     : page_at(trow, key00 + s * step_keys, p.page_shift,
                                                p.max_pages, p.pages);
       if (pg < 0) atomicExch(p.status, kDevBadPage);
       return pg;
@@ -286,7 +319,7 @@ __global__ void __launch_bounds__(RowCfg<DT, MT, CUT>::kThreads, RowCfg<DT, MT, 
           ids_next = page_of(s + 32 + lane);
         }
         const int pg = __shfl_sync(0xffffffffu, ids, s & 31);
-        const int key0 = key00 + s * C::kStep;
+        const int key0 = key00 + s * step_keys;
         const int in = key0 & page_mask;
         const uint32_t st = ring + (s % C::kStages) * C::kStage;
         if (pg >= 0 && key0 + 16 <= w.kv_len && p.D == DT) {
@@ -363,7 +396,7 @@ __global__ void __launch_bounds__(RowCfg<DT, MT, CUT>::kThreads, RowCfg<DT, MT, 
       __syncwarp();
       issue(s + C::kStages - 1);
       const uint32_t st = ring + (s % C::kStages) * C::kStage;
-      const int key0 = key00 + s * C::kStep;
+      const int key0 = key00 + s * step_keys;
       // S = Q K^T for 16 keys: two 8-key column tiles.
       float sc[MT][2][4];
 #pragma unroll
@@ -484,7 +517,18 @@ __global__ void __launch_bounds__(RowCfg<DT, MT, CUT>::kThreads, RowCfg<DT, MT, 
       }
     __syncthreads();
     const bool first = blk0 == 0, last = blk0 + nblk == w.blocks;
-    float* slot = p.part + static_cast<int64_t>(2 * blockIdx.x + (first ? 1 : 0)) * C::kSlot;
+    const bool shared = CUT == kWholeWide && cluster > 1;    // to add up in the cluster
+    float* slot = shared ? reinterpret_cast<float*>(smem + C::kSumOff)
+                         : p.part + static_cast<int64_t>(2 * cta + (first ? 1 : 0)) * C::kSlot;
+    auto put = [&](int r, int d, const float4& acc, float sum) {
+      if (d >= p.D) return;
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      const int tok = (row0 + r) / p.g, hd = (row0 + r) - tok * p.g;
+      uint16_t* dst = static_cast<uint16_t*>(p.o) + static_cast<int64_t>(w.begin + tok) * p.o_st +
+                      static_cast<int64_t>(h * p.g + hd) * p.o_sh + d;
+      *reinterpret_cast<uint2*>(dst) = make_uint2(pack_16x2<F16>(acc.x * inv, acc.y * inv),
+                                                  pack_16x2<F16>(acc.z * inv, acc.w * inv));
+    };
     for (int i = threadIdx.x; i < rows * (DT / 4); i += C::kThreads) {
       const int r = i / (DT / 4), d = (i - r * (DT / 4)) * 4;
       float top = -INFINITY, sum = 0.f;
@@ -501,15 +545,8 @@ __global__ void __launch_bounds__(RowCfg<DT, MT, CUT>::kThreads, RowCfg<DT, MT, 
         acc.z += x.z;
         acc.w += x.w;
       }
-      if (first && last) {
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
-        const int tok = (row0 + r) / p.g, hd = (row0 + r) - tok * p.g;
-        uint16_t* dst = static_cast<uint16_t*>(p.o) +
-                        static_cast<int64_t>(w.begin + tok) * p.o_st +
-                        static_cast<int64_t>(h * p.g + hd) * p.o_sh + d;
-        if (d < p.D)
-          *reinterpret_cast<uint2*>(dst) = make_uint2(pack_16x2<F16>(acc.x * inv, acc.y * inv),
-                                                      pack_16x2<F16>(acc.z * inv, acc.w * inv));
+      if (first && last && !shared) {
+        put(r, d, acc, sum);
       } else {
         *reinterpret_cast<float4*>(slot + r * DT + d) = acc;
         if (d == 0) {
@@ -517,6 +554,35 @@ __global__ void __launch_bounds__(RowCfg<DT, MT, CUT>::kThreads, RowCfg<DT, MT, 
           slot[C::kRows * DT + C::kRows + r] = sum;
         }
       }
+    }
+    if (shared) {
+      cluster_sync();
+      // The cluster's CTAs share the sums out, in the order of the ranks each.
+      const uint32_t at = smem_u32(slot);
+      for (int i = rank * C::kThreads + threadIdx.x; i < rows * (DT / 4);
+           i += C::kThreads << cshift) {
+        const int r = i / (DT / 4), d = (i - r * (DT / 4)) * 4;
+        float m8[8], top = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          m8[k] = k < cluster ? cluster_load(at + (C::kRows * DT + r) * 4, k) : -INFINITY;
+          top = fmaxf(top, m8[k]);
+        }
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          if (k >= cluster) continue;
+          const float al = m8[k] == -INFINITY ? 0.f : ex2_approx(m8[k] - top);
+          sum += cluster_load(at + (C::kRows * DT + C::kRows + r) * 4, k) * al;
+          const float4 x = cluster_load4(at + (r * DT + d) * 4, k);
+          acc.x += x.x * al;
+          acc.y += x.y * al;
+          acc.z += x.z * al;
+          acc.w += x.w * al;
+        }
+        put(r, d, acc, sum);
+      }
+      cluster_sync();       // nobody's sums are read any more
     }
     cur += nblk;
     if (WHOLE) {
@@ -618,8 +684,8 @@ int launch_rows_kernel(const PagedParams& p, cudaStream_t stream) {
   const int rc = prepare_kernel(
       prep, reinterpret_cast<const void*>(paged_rows_kernel<DT, MT, F16, CUT>), C::kSmem, &dev);
   if (rc != FA_OK) return rc;
-  return launch_after(paged_rows_kernel<DT, MT, F16, CUT>, dim3(p.ctas * p.team), C::kThreads,
-                      C::kSmem, stream, p);
+  return launch_after(paged_rows_kernel<DT, MT, F16, CUT>, dim3((p.ctas * p.team) << p.cluster_shift),
+                      C::kThreads, C::kSmem, 1 << p.cluster_shift, stream, p);
 }
 
 template <int DT, int MT, bool F16>
@@ -629,7 +695,7 @@ int launch_rows(const PagedParams& p, Cut cut, int rows, cudaStream_t stream) {
   const int rc = launch_rows_kernel<DT, MT, F16, kSplit>(p, stream);
   if (rc != FA_OK) return rc;
   return launch_after(paged_rows_join<DT, MT, F16>,
-                      dim3(p.ctas * p.team, (rows + kRowWarps - 1) / kRowWarps), kRowThreads, 0,
+                      dim3(p.ctas * p.team, (rows + kRowWarps - 1) / kRowWarps), kRowThreads, 0, 1,
                       stream, p);
 }
 
@@ -676,9 +742,10 @@ int check_paged_attn(const fa_paged_attn_args* a) {
 }
 
 // Which kernel runs, by sizes that the host knows.
-//  * Few rows over a short table: the row kernel with a CTA per sequence, head and
-//    16 rows, of 16 warps (8 with D > 64), up to 8 steps of each and a CTA per SM.
-//    37 tokens over 1061 keys, 16 heads of 64: 10.4 us, 16.5 split and joined, 21 by
+//  * Few rows: the row kernel with a cluster per sequence, head and 16 rows, of
+//    CTAs of 16 warps (8 with D > 64), as many as get 2 steps or more of their own
+//    and leave a CTA per SM, up to 16 steps of each (8 of a single CTA).
+//    37 tokens over 1061 keys, 16 heads of 64: 10 us, 16.5 split and joined, 21 by
 //    the tile kernel.
 //  * The row kernel takes the other sequences of up to kRowMax rows (single
 //    tokens), and chunks whose products over the whole table are at most kRowWork
@@ -689,23 +756,60 @@ int check_paged_attn(const fa_paged_attn_args* a) {
 constexpr int kRowMax = 32;
 constexpr double kRowWork = 1e9;
 
+// Clusters of 1 << shift CTAs of the wide row kernel that device dev holds at
+// once (clusters lie within one of its parts: 16 of 8 CTAs do not fit 148 SMs).
+int max_clusters(int dev, bool narrow, int shift) {
+  static std::atomic<int> known[64][2][4];
+  if (dev < 0 || dev >= 64) return 0;
+  std::atomic<int>& slot = known[dev][narrow ? 1 : 0][shift];
+  int n = slot.load(std::memory_order_relaxed);
+  if (n > 0) return n;
+  const void* kern = narrow ? reinterpret_cast<const void*>(paged_rows_kernel<64, 1, false, kWholeWide>)
+                            : reinterpret_cast<const void*>(paged_rows_kernel<128, 1, false, kWholeWide>);
+  const int smem = narrow ? RowCfg<64, 1, kWholeWide>::kSmem : RowCfg<128, 1, kWholeWide>::kSmem;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(8 * 148);
+  cfg.blockDim = dim3(narrow ? RowCfg<64, 1, kWholeWide>::kThreads
+                             : RowCfg<128, 1, kWholeWide>::kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = 1 << shift;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n <= 0) {
+    (void)cudaGetLastError();
+    return 0;
+  }
+  slot.store(n, std::memory_order_relaxed);
+  return n;
+}
+
 struct Choice {
   bool tiles;
   bool rows32;          // row tiles of 32 rows, else 16
   Cut cut;
   int tile_ctas;        // whole units: CTAs over a head's row tiles
+  int cluster_shift;    // and CTAs of each: 1 << this
 };
 
-Choice choose(const fa_paged_attn_args* a, int sms) {
+Choice choose(const fa_paged_attn_args* a, int dev, int sms) {
   const int64_t longest = (a->max_q_len < a->T ? a->max_q_len : a->T) * (a->Hq / a->Hkv);
   const int64_t keys = a->max_pages * a->page_size, units = a->B * a->Hkv;
   const int64_t tiles16 = (longest + 15) / 16;
-  const int wide_keys = 8 * (a->D <= 64 ? RowCfg<64, 1, kWholeWide>::kStep
-                                        : RowCfg<128, 1, kWholeWide>::kStep);
-  if (units <= sms && units * tiles16 <= sms && keys <= wide_keys)
-    return {false, false, kWholeWide, static_cast<int>(tiles16)};
+  const int step = a->D <= 64 ? RowCfg<64, 1, kWholeWide>::kStep : RowCfg<128, 1, kWholeWide>::kStep;
+  if (units <= sms && units * tiles16 <= sms) {
+    int shift = 0;
+    while (shift < 3 && keys > (2ll << shift) * step &&
+           units * tiles16 <= max_clusters(dev, a->D <= 64, shift + 1))
+      ++shift;
+    if (keys <= (shift == 0 ? 8 : 16) * (static_cast<int64_t>(step) << shift))
+      return {false, false, kWholeWide, static_cast<int>(tiles16), shift};
+  }
   if (longest <= kRowMax && keys <= 1024 && units <= 0x7fffffffLL)
-    return {false, longest > 16, kWhole, 1};
+    return {false, longest > 16, kWhole, 1, 0};
   // The tile kernel's copies need real strides, its exponent a scale that keeps order.
   const bool flat = (a->q_strides[0] == 0 && a->T > 1) || (a->q_strides[1] == 0 && a->Hq > 1) ||
                     (a->k_cache_strides[0] == 0 && a->pages > 1) || a->k_cache_strides[1] == 0 ||
@@ -713,7 +817,8 @@ Choice choose(const fa_paged_attn_args* a, int sms) {
                     (a->v_cache_strides[0] == 0 && a->pages > 1) || a->v_cache_strides[1] == 0 ||
                     (a->v_cache_strides[2] == 0 && a->Hkv > 1);
   const double most = 4.0 * a->T * a->Hq * a->D * keys;
-  return {longest > kRowMax && most > kRowWork && !flat && a->scale >= 0, longest > 16, kSplit, 1};
+  return {longest > kRowMax && most > kRowWork && !flat && a->scale >= 0, longest > 16, kSplit, 1,
+          0};
 }
 
 // Teams of the row kernel: of the size, up to 16 heads, that fills the device
@@ -744,7 +849,7 @@ extern "C" int64_t fa_paged_attn_workspace(const fa_paged_attn_args* a) {
   if (cudaGetDevice(&dev) != cudaSuccess) return -FA_ERR_CUDA;
   const int sms = sm_count(dev);
   if (sms <= 0) return -FA_ERR_CUDA;
-  const Choice c = choose(a, sms);
+  const Choice c = choose(a, dev, sms);
   if (c.tiles) return paged_tiles_bytes(a, sms);
   if (c.cut != kSplit) return 0;
   const Teams t = row_teams(a, c, sms);
@@ -797,7 +902,7 @@ extern "C" int fa_paged_attn(const fa_paged_attn_args* a, void* workspace,
   const int sms = sm_count(dev);
   const bool f16 = a->dtype == FA_F16;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const Choice c = choose(a, sms);
+  const Choice c = choose(a, dev, sms);
   if (c.tiles) {
     p.ctas = sms;
     return launch_paged_tiles(a, p, workspace, s);
@@ -806,6 +911,7 @@ extern "C" int fa_paged_attn(const fa_paged_attn_args* a, void* workspace,
   p.ctas = t.count;
   p.team = t.heads;
   p.tile_ctas = c.tile_ctas;
+  p.cluster_shift = c.cluster_shift;
   p.part = static_cast<float*>(workspace);
   p.min_blocks = 4;
   // (the join's CTAs go over more rows than these where max_q_len was too small)

@@ -29,6 +29,7 @@ struct PagedParams {
   int min_blocks;                       // least key blocks of a range
   int team;                             // row kernel: heads that stream side by side
   int tile_ctas;                        // row kernel, whole units: CTAs over a head's row tiles
+  int cluster_shift;                    // and CTAs (1 << this) that share a unit's keys
 };
 
 // A sequence's new tokens and keys.

@@ -1137,13 +1137,13 @@ int launch_tiles(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap
   int rc = prepare_kernel(prep, reinterpret_cast<const void*>(paged_tiles_kernel<D, F16>),
                           C::kSmemBytes, &dev);
   if (rc != FA_OK) return rc;
-  rc = launch_after(paged_plan_kernel, dim3(1), kPlanThreads, 0, stream, p);
+  rc = launch_after(paged_plan_kernel, dim3(1), kPlanThreads, 0, 1, stream, p);
   if (rc != FA_OK) return rc;
-  rc = launch_after(paged_tiles_kernel<D, F16>, dim3(p.ctas), kThreads, C::kSmemBytes, stream, mq,
+  rc = launch_after(paged_tiles_kernel<D, F16>, dim3(p.ctas), kThreads, C::kSmemBytes, 1, stream, mq,
                     mk, mv, p);
   if (rc != FA_OK) return rc;
   return launch_after(paged_tiles_join<D, F16>, dim3(2 * p.ctas),
-                      32 * kJoinWarps, 0, stream, p);
+                      32 * kJoinWarps, 0, 1, stream, p);
 }
 
 }  // namespace

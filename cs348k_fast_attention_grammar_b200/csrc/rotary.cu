@@ -354,7 +354,7 @@ int launch_rotary(RotParams& p, int dtype, bool append, bool interleaved, cudaSt
     if (p.status == nullptr) return FA_ERR_CUDA;
   }
   // (as a programmatic dependent: its CTAs come up while the kernel before ends)
-#define FA_ROT(T, A, I) launch_after(rotary_kernel<T, A, I>, dim3(g), kRotThreads, 0, stream, p)
+#define FA_ROT(T, A, I) launch_after(rotary_kernel<T, A, I>, dim3(g), kRotThreads, 0, 1, stream, p)
   if (append) {
     if (dtype == FA_BF16)
       return interleaved ? FA_ROT(FA_BF16, true, true) : FA_ROT(FA_BF16, true, false);

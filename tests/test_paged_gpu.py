@@ -66,6 +66,15 @@ def test_every_length():
     _check([1] * len(lens), lens, 4, 2, 64, 16)
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("Hkv", [1, 2, 8, 24])
+def test_clusters(D, Hkv):
+    """One to eight CTAs over a sequence's keys, and lengths that leave some of them without."""
+    for top in (700, 2500, 5000, 12000):
+        _check([1, 3], [top, 17], 4 * Hkv, Hkv, D, 32)
+        _check([0, 5], [top, top // 3], 2 * Hkv, Hkv, D, 64, F16, causal=False)
+
+
 def test_long_and_many():
     _check([1, 1], [20000, 4097], 8, 1, 128, 64)
     _check([1] * 300, [(37 * i) % 500 for i in range(300)], 4, 2, 64, 16)
