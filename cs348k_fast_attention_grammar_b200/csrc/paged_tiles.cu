@@ -429,9 +429,10 @@ __device__ __forceinline__ void exp2_pair(float x0, float x1, float& r0, float& 
   r1 = __int_as_float(__float_as_int(p1) + (__float_as_int(t1) << 23));
 }
 
+// The largest of three; NaN if one is (the exponentials on the FMA pipe would lose it).
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
 
@@ -845,10 +846,10 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             mx4[i] = max3(mx4[i], __uint_as_float(sr[c + 2 * i]), __uint_as_float(sr[c + 2 * i + 1]));
-        const float m_blk = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * sl2;
+        const float m_blk = max3(max3(mx4[0], mx4[1], mx4[2]), mx4[3], -INFINITY) * sl2;
         // The reference is raised only when a row outgrows it by 2^8, so that
         // O is rarely rescaled; O / l is exact for any reference.
-        const bool need = m_ref == -INFINITY ? m_blk > -INFINITY : m_blk - m_ref > 8.f;
+        const bool need = !(m_blk <= m_ref + 8.f);
         if (__any_sync(0xffffffffu, need)) {
           const float m_use = need ? m_blk : m_ref;
           const float alpha = m_use == -INFINITY   ? 1.f

@@ -237,7 +237,7 @@ __global__ void __launch_bounds__(kRotThreads, kRotCtasPerSm)
         int64_t k = -1, v = -1;
         int place = 0;
         if (b >= 0) {
-          place = p.kv_lens[b] - ((p.cu == nullptr ? b + 1 : p.cu[b + 1]) - t);
+          place = max(p.kv_lens[b], 0) - ((p.cu == nullptr ? b + 1 : p.cu[b + 1]) - t);
           if (place >= 0) {
             const int page = page_at(p.table + b * p.table_stride, place, p.page_shift,
                                      p.max_pages, p.pages);

@@ -83,7 +83,7 @@ def paged_kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor,
     token's place in its sequence or by ``positions`` (``[T]``; ``[axes, T]`` with
     ``sections``).  ``q_out`` may be ``q``.
 
-    Rows of no sequence are neither read nor written, in ``q_out`` too.  Tokens
+    Rows of no sequence have no effect, and ``q_out`` is left as it was there.  Tokens
     before their sequence's start (``kv_lens`` below the number of new tokens, as
     in padding sequences of length 0) are not stored.  A place outside the
     table or the cache is skipped, and ``device_status()`` reports it.

@@ -262,7 +262,7 @@ int fa_rotary(const fa_rotary_args* args, void* stream);
  * fa_paged_append writes the keys, rotated as in fa_rotary when R > 0, and the
  * values of new tokens to their places, and the rotated queries, where there
  * are any, to q_out.  Without `positions` a token is rotated by its place in
- * the sequence.  Rows outside every sequence are neither read nor written; a
+ * the sequence.  Rows outside every sequence have no effect and are not written; a
  * token before its sequence's start (kv_lens[b] < q_len, as in padding
  * sequences of length 0) is not stored.  A place outside the table or a page
  * outside the cache is not written either and leaves FA_ERR_PAGE in the device
@@ -300,7 +300,7 @@ int fa_paged_append(const fa_paged_append_args* args, void* stream);
  * that holds them:  o = softmax(q K^T * scale) V  per token and head, query
  * heads in Hkv groups that share a key/value head.  With `causal` a token sees
  * the keys up to its own place, else all kv_lens[b].  A token that sees no key
- * gets zeros.  Rows outside every sequence are neither read nor written.
+ * gets zeros.  Rows outside every sequence have no effect and are not written.
  * A page outside the cache reads as zeros and a length behind the table is cut
  * there; both leave FA_ERR_PAGE in the device status word.  Cached values that
  * a sequence's tokens see must be finite (a value that only some of a chunk's
@@ -309,7 +309,7 @@ int fa_paged_append(const fa_paged_append_args* args, void* stream);
  *   max_q_len : an upper bound of the tokens per sequence that only guides
  *               which kernels run (T where unknown); results hold for any value.
  *   workspace : fa_paged_attn_workspace(args) bytes, 16-byte aligned, used by
- *               this call alone until it has run.
+ *               this call alone until it has run (may be NULL for 0 bytes).
  */
 typedef struct fa_paged_attn_args {
   const void* q;           /* [T, Hq, D]                                        */

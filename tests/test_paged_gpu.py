@@ -21,19 +21,32 @@ def _randn(shape, dtype, seed=0):
     return torch.randn(shape, generator=g).to(dtype).to(DEV)
 
 
+# Which kernel runs, and how its work is cut, goes by the keys that the table has room for: the
+# sequences' own, 8192, 2^18.
+ROOMS = (0, 8192, 1 << 18)
+
+
+def _with_room(table, page, keys):
+    """The table with entries (outside the cache) for that many keys."""
+    more = -(-keys // page) - table.shape[1]
+    return table if more <= 0 else torch.nn.functional.pad(table, (0, more), value=-3)
+
+
 def _check(q_lens, kv_lens, Hq, Hkv, D, page, dtype=BF16, causal=True, hnd=False, seed=0,
            scale=None, **kw):
     c = Cache(kv_lens, page, Hkv, D, dtype, DEV, seed=seed, hnd=hnd)
     q = _randn((sum(q_lens), Hq, D), dtype, seed + 1)
     cu = borders(q_lens, DEV)
-    out = torch.full_like(q, float("nan"))
-    kw.setdefault("max_q_len", max(q_lens))
-    got = paged_attention(q, c.k, c.v, c.table, c.lens, cu_seqlens=cu, causal=causal, scale=scale,
-                          out=out, **kw)
     want, size = reference(q, c.k, c.v, c.table, kv_lens, q_lens, causal, scale)
-    assert_within(got, want, attention_tolerance(want, size, dtype, max(kv_lens)),
-                  f"{q_lens} over {kv_lens}")
-    assert device_status() == 0
+    tol = attention_tolerance(want, size, dtype, max(kv_lens))
+    kw.setdefault("max_q_len", max(q_lens))
+    for room in ROOMS:
+        table = _with_room(c.table, page, room)
+        out = torch.full_like(q, float("nan"))
+        got = paged_attention(q, c.k, c.v, table, c.lens, cu_seqlens=cu, causal=causal,
+                              scale=scale, out=out, **kw)
+        assert_within(got, want, tol, f"{q_lens} over {kv_lens}, room for {room}")
+        assert device_status() == 0
     return q, c, cu, got
 
 
@@ -150,25 +163,48 @@ def test_scale_and_score_jump():
             q = _randn((q_lens[0], 2, 64), dtype, 3)
             page, row = int(c.table[0, 550 // 64]), 550 % 64
             c.k[page, row, 0] = q[0, 0] * 8
-            got = paged_attention(q, c.k, c.v, c.table, c.lens, cu_seqlens=borders(q_lens, DEV))
             want, size = reference(q, c.k, c.v, c.table, [700], q_lens)
             # scores reach 64 here instead of 8: the score term of the tolerance is 8 times larger
             tol = attention_tolerance(want, size, dtype, 700) + size * 7 * 2.0 ** -12.5
-            assert_within(got, want, tol)
+            for room in ROOMS:
+                got = paged_attention(q, c.k, c.v, _with_room(c.table, 64, room), c.lens,
+                                      cu_seqlens=borders(q_lens, DEV))
+                assert_within(got, want, tol)
+
+
+@pytest.mark.parametrize("room", ROOMS)
+def test_non_finite_rows(room):
+    """A query that is not a number makes its own outputs so and no others; a key that is not, or
+    is infinite, the outputs of the tokens that see it."""
+    q_lens, kv_lens = [1, 60, 40], [300, 60, 90]
+    c = Cache(kv_lens, 16, 1, 64, BF16, DEV)
+    table = _with_room(c.table, 16, room)
+    cu = borders(q_lens, DEV)
+    q = _randn((101, 2, 64), BF16, 1)
+    want, size = reference(q, c.k, c.v, c.table, kv_lens, q_lens)
+    tol = attention_tolerance(want, size, BF16, 300)
+    q[7, 1] = float("nan")
+    c.k[int(c.table[2, 70 // 16]), 70 % 16] = float("nan")     # seen by the last 20 tokens
+    got = paged_attention(q, c.k, c.v, table, c.lens, cu_seqlens=cu, max_q_len=60)
+    bad = torch.zeros((101, 2), dtype=torch.bool, device=DEV)
+    bad[7, 1] = bad[81:, 0] = bad[81:, 1] = True
+    assert got[bad].isnan().all()
+    assert_within(got[~bad], want[~bad], tol[~bad])
 
 
 def test_layouts_and_padded_rows():
     """A [pages, Hkv, page, D] allocation, q inside a fused projection, out inside a wider
     buffer, rows before and behind the sequences."""
     q_lens, kv_lens = [1, 140, 6], [33, 200, 6]
-    for D, page in ((64, 16), (128, 64)):
+    for D, page, room in ((64, 16, 0), (128, 64, 0), (64, 16, 1 << 18), (128, 64, 1 << 18)):
         c = Cache(kv_lens, page, 2, D, BF16, DEV, hnd=True)
         rows = _randn((3 + sum(q_lens) + 5, 12 * D), BF16, 1)
         q = rows[:, 2 * D:10 * D].unflatten(1, (8, D))
         wide = torch.full((q.shape[0], 9, D + 8), 7.0, dtype=BF16, device=DEV)
         out = wide[:, 1:, :D]
         cu = borders(q_lens, DEV, first=3)
-        assert paged_attention(q, c.k, c.v, c.table, c.lens, cu_seqlens=cu, out=out) is out
+        table = _with_room(c.table, page, room)
+        assert paged_attention(q, c.k, c.v, table, c.lens, cu_seqlens=cu, out=out) is out
         want, size = reference(q[3:-5], c.k, c.v, c.table, kv_lens, q_lens)
         assert_within(out[3:-5], want, attention_tolerance(want, size, BF16, 200))
         assert (wide[:3] == 7).all() and (wide[-5:] == 7).all()
@@ -210,12 +246,13 @@ def test_equals_attention_on_a_whole_prompt():
 
 
 def test_repeatable():
-    for q_lens, kv_lens in (([1, 1], [9000, 300]), ([200, 1], [5000, 300])):
-        q, c, cu, first = _check(q_lens, kv_lens, 8, 2, 128, 64)
-        for _ in range(3):
-            again = paged_attention(q, c.k, c.v, c.table, c.lens, cu_seqlens=cu,
-                                    max_q_len=max(q_lens))
-            assert torch.equal(again, first)
+    for q_lens, kv_lens in (([1, 1], [9000, 300]), ([200, 1], [5000, 300]), ([900] * 9, [3000] * 9)):
+        for room in ROOMS:
+            q, c, cu, _ = _check(q_lens, kv_lens, 8, 2, 128, 64)
+            table = _with_room(c.table, 64, room)
+            made = [paged_attention(q, c.k, c.v, table, c.lens, cu_seqlens=cu,
+                                    max_q_len=max(q_lens)) for _ in range(4)]
+            assert all(torch.equal(m, made[0]) for m in made)
 
 
 # --------------------------------------------------------------------------- far places
@@ -234,11 +271,14 @@ def test_cache_beyond_32_bit_offsets():
     assert torch.equal(kc[shift:].nan_to_num(5), small.k.nan_to_num(5))
     assert torch.equal(vc[shift:].nan_to_num(5), small.v.nan_to_num(5))
     for q_lens in ([1, 1], [200, 1]):
-        q = _randn((sum(q_lens), 16, D), BF16, 3)
-        cu = borders(q_lens, DEV)
-        a = paged_attention(q, kc, vc, table, small.lens, cu_seqlens=cu)
-        assert torch.equal(a, paged_attention(q, small.k, small.v, small.table, small.lens,
-                                              cu_seqlens=cu))
+        for room in ROOMS:
+            q = _randn((sum(q_lens), 16, D), BF16, 3)
+            cu = borders(q_lens, DEV)
+            a = paged_attention(q, kc, vc, _with_room(table, page, room), small.lens,
+                                cu_seqlens=cu)
+            assert torch.equal(a, paged_attention(q, small.k, small.v,
+                                                  _with_room(small.table, page, room), small.lens,
+                                                  cu_seqlens=cu))
     assert device_status() == 0
 
 
@@ -319,11 +359,13 @@ def test_places_outside_the_cache():
         c.k[pg, 7], c.v[pg, 7] = kc[pg, 7], vc[pg, 7]
         assert torch.equal(c.k.nan_to_num(9), kc.nan_to_num(9))
         for q_lens in ([1, 1], [19, 40]):
-            qq = q.repeat(30, 1, 1)[:sum(q_lens)]
-            got = paged_attention(qq, c.k, c.v, c.table, c.lens, cu_seqlens=borders(q_lens, DEV))
-            assert device_status() == FA_ERR_PAGE
-            want, size = reference(qq[q_lens[0]:], c.k, c.v, good[1:], [40], q_lens[1:])
-            assert_within(got[q_lens[0]:], want, attention_tolerance(want, size, BF16, 40))
+            for room in ROOMS:
+                qq = q.repeat(30, 1, 1)[:sum(q_lens)]
+                got = paged_attention(qq, c.k, c.v, _with_room(c.table, 16, room), c.lens,
+                                      cu_seqlens=borders(q_lens, DEV))
+                assert device_status() == FA_ERR_PAGE
+                want, size = reference(qq[q_lens[0]:], c.k, c.v, good[1:], [40], q_lens[1:])
+                assert_within(got[q_lens[0]:], want, attention_tolerance(want, size, BF16, 40))
     c.table.copy_(good)
     # a length behind the table: 3 pages hold 48
     lens = torch.tensor([20, 60], dtype=torch.int32, device=DEV)
@@ -343,8 +385,10 @@ def test_borders_outside_the_rows():
     q = _randn((4, 2, 64), BF16, 1)
     for cu in ([0, 1, 900], [-5, 1, 2], [3, 1, 2], [0, 2 ** 31 - 1, 1]):
         t = torch.tensor(cu, dtype=torch.int32, device=DEV)
-        paged_attention(q, c.k, c.v, c.table, c.lens, cu_seqlens=t, out=torch.zeros_like(q))
-        paged_attention(q, c.k, c.v, c.table, c.lens, cu_seqlens=t, max_q_len=200)
+        for room in ROOMS:
+            table = _with_room(c.table, 16, room)
+            for longest in (None, 1, 200):
+                paged_attention(q, c.k, c.v, table, c.lens, cu_seqlens=t, max_q_len=longest)
         paged_kv_append(q[:, :1], q[:, :1], c.k.clone(), c.v.clone(), c.table, c.lens, cu_seqlens=t)
         torch.cuda.synchronize()
     device_status()
@@ -358,9 +402,12 @@ def test_empty_calls():
     assert paged_kv_append(none, none, c.k, c.v, c.table, c.lens, cu_seqlens=cu) is None
     # rows, but no sequence owns one
     q = _randn((3, 2, 64), BF16)
-    out = torch.full_like(q, 2.0)
-    paged_attention(q, c.k, c.v, c.table, c.lens, cu_seqlens=cu, out=out)
-    assert (out == 2).all()
+    for room in ROOMS:
+        for longest in (1, 100):
+            out = torch.full_like(q, 2.0)
+            paged_attention(q, c.k, c.v, _with_room(c.table, 16, room), c.lens, cu_seqlens=cu,
+                            max_q_len=longest, out=out)
+            assert (out == 2).all()
 
 
 # --------------------------------------------------------------------------- a user's program
@@ -395,8 +442,9 @@ def test_generation_matches_one_prompt(D):
     assert device_status() == 0
 
 
+@pytest.mark.parametrize("room", ROOMS)
 @pytest.mark.parametrize("q_lens", [[1, 1, 1], [90, 1, 30]])
-def test_graphs_with_new_lengths(q_lens):
+def test_graphs_with_new_lengths(q_lens, room):
     """Two captured steps with outputs of their own, replayed in two streams at once with lengths
     and tokens changed in place, against eager calls."""
     D, Hq, Hkv, page = 128, 8, 2, 16
@@ -405,6 +453,7 @@ def test_graphs_with_new_lengths(q_lens):
     made = []
     for i, side in enumerate(sides):
         c = Cache([2500, 300, 120], page, Hkv, D, BF16, DEV, seed=i)
+        c.table = _with_room(c.table, page, room)
         T = sum(q_lens)
         q, k, v = (_randn((T, h, D), BF16, 10 * i + h) for h in (Hq, Hkv, Hkv))
         state = (q, k, v, borders(q_lens, DEV), max(q_lens))
@@ -432,18 +481,27 @@ def test_graphs_with_new_lengths(q_lens):
     assert device_status() == 0
 
 
-def test_streams_at_once():
+@pytest.mark.parametrize("room", ROOMS)
+@pytest.mark.parametrize("q_lens", [[1, 1], [150, 1]])
+def test_streams_at_once(q_lens, room):
     """Calls in two streams at once, each with its own inputs, against the calls alone."""
     cs = [Cache([3000, 200], 16, 2, 64, BF16, DEV, seed=i) for i in range(2)]
-    qs = [_randn((2, 8, 64), BF16, i) for i in range(2)]
-    want = [paged_attention(q, c.k, c.v, c.table, c.lens) for q, c in zip(qs, cs)]
+    qs = [_randn((sum(q_lens), 8, 64), BF16, i) for i in range(2)]
+    cu = borders(q_lens, DEV)
+
+    def call(q, c):
+        return paged_attention(q, c.k, c.v, c.table, c.lens, cu_seqlens=cu, max_q_len=q_lens[0])
+
+    for c in cs:
+        c.table = _with_room(c.table, 16, room)
+    want = [call(q, c) for q, c in zip(qs, cs)]
     sides = [torch.cuda.Stream() for _ in range(2)]
     torch.cuda.synchronize()
     got = [[], []]
     for _ in range(20):
         for i, side in enumerate(sides):
             with torch.cuda.stream(side):
-                got[i].append(paged_attention(qs[i], cs[i].k, cs[i].v, cs[i].table, cs[i].lens))
+                got[i].append(call(qs[i], cs[i]))
     torch.cuda.synchronize()
     for i in range(2):
         assert all(torch.equal(o, want[i]) for o in got[i])
