@@ -754,7 +754,7 @@ int check_paged_attn(const fa_paged_attn_args* a) {
 //  * The tile kernel takes chunks, and then the batch's short sequences too: a
 //    second launch for those costs more than a tile kernel's unit of one token.
 constexpr int kRowMax = 32;
-constexpr double kRowWork = 1e9;
+constexpr double kRowWork = 1e8, kWholeWork = 1e9;
 
 // Clusters of 1 << shift CTAs of the wide row kernel that device dev holds at
 // once (clusters lie within one of its parts: 16 of 8 CTAs do not fit 148 SMs).
@@ -798,7 +798,7 @@ struct Choice {
 Choice choose(const fa_paged_attn_args* a, int dev, int sms) {
   const int64_t longest = (a->max_q_len < a->T ? a->max_q_len : a->T) * (a->Hq / a->Hkv);
   const int64_t keys = a->max_pages * a->page_size, units = a->B * a->Hkv;
-  const int64_t tiles16 = (longest + 15) / 16;
+  const int64_t tiles16 = (longest + 15) / 16, tiles32 = (longest + 31) / 32;
   const int step = a->D <= 64 ? RowCfg<64, 1, kWholeWide>::kStep : RowCfg<128, 1, kWholeWide>::kStep;
   if (units <= sms && units * tiles16 <= sms) {
     int shift = 0;
@@ -808,15 +808,15 @@ Choice choose(const fa_paged_attn_args* a, int dev, int sms) {
     if (keys <= (shift == 0 ? 8 : 16) * (static_cast<int64_t>(step) << shift))
       return {false, false, kWholeWide, static_cast<int>(tiles16), shift};
   }
-  if (longest <= kRowMax && keys <= 1024 && units <= 0x7fffffffLL)
-    return {false, longest > 16, kWhole, 1, 0};
+  const double most = 4.0 * a->T * a->Hq * a->D * keys;
+  if (keys <= 1024 && (longest <= kRowMax || most <= kWholeWork) && units <= 0x7fffffffLL / tiles32)
+    return {false, longest > 16, kWhole, static_cast<int>(tiles32), 0};
   // The tile kernel's copies need real strides, its exponent a scale that keeps order.
   const bool flat = (a->q_strides[0] == 0 && a->T > 1) || (a->q_strides[1] == 0 && a->Hq > 1) ||
                     (a->k_cache_strides[0] == 0 && a->pages > 1) || a->k_cache_strides[1] == 0 ||
                     (a->k_cache_strides[2] == 0 && a->Hkv > 1) ||
                     (a->v_cache_strides[0] == 0 && a->pages > 1) || a->v_cache_strides[1] == 0 ||
                     (a->v_cache_strides[2] == 0 && a->Hkv > 1);
-  const double most = 4.0 * a->T * a->Hq * a->D * keys;
   return {longest > kRowMax && most > kRowWork && !flat && a->scale >= 0, longest > 16, kSplit, 1,
           0};
 }
