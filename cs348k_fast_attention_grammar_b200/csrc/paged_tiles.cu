@@ -445,9 +445,9 @@ struct Cfg {
   static constexpr int kStages = D == 128 ? 4 : 8;       // K and V tiles in the ring
   static constexpr int kQOff = 0;
   static constexpr int kKVOff = 2 * kTileBytes;
-  static constexpr int kOutOff = kKVOff + kStages * kTileBytes;   // a warp's 32 x 32 outputs
-  static constexpr int kOutRow = 80;                              // bytes, 16 of them padding
-  static constexpr int kBarOff = kOutOff + 8 * 32 * kOutRow;
+  static constexpr int kOutOff = kKVOff + kStages * kTileBytes;   // each warp's 32 x 64 outputs
+  static constexpr int kOutWarp = 32 * 64 * 2;
+  static constexpr int kBarOff = kOutOff + 8 * kOutWarp;
   // q, kv_full[], kv_empty[], s_full[2], p_full[2], o_full[2], drain, p_half[2],
   // q_empty, unit_full[2], unit_empty[2], v_raw
   static constexpr int kNumBars = 1 + 2 * kStages + 15;
@@ -922,42 +922,42 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(bar_unit_empty(us));
       if (slot < 0) {
-        // 32 x 32 outputs at a time through shared memory, so that a store
-        // covers 64 bytes of each of 8 rows instead of 16 of 32.
-        uint8_t* stage = gbase + C::kOutOff + warp * 32 * C::kOutRow;
+        // 32 rows x 64 outputs at a time through shared memory (16-byte chunks
+        // swizzled by the row), so that a store covers 128 bytes of each of 4
+        // rows instead of 16 of 32.
+        uint8_t* stage = gbase + C::kOutOff + warp * C::kOutWarp;
         const int64_t off = live ? static_cast<int64_t>(q_begin + tok) * p.o_st +
                                        static_cast<int64_t>(h * p.g + row - row_tok * p.g) * p.o_sh
                                  : -1;
-        int64_t to[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) to[i] = __shfl_sync(0xffffffffu, off, i * 8 + lane / 4);
-#pragma unroll
-        for (int c = 0; c < D / 32; ++c) {
-          uint32_t o[32];
+        for (int c = 0; c < D / 64; ++c) {
+          uint32_t o[64];
           if (nt > 0) {
-            tmem_ld32_wait(tO + c * 32, o);
+            tmem_ld64_wait(tO + c * 64, o);
           } else {
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = 0u;
+            for (int e = 0; e < 64; ++e) o[e] = 0u;
           }
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
+          for (int e = 0; e < 8; ++e) {
             uint32_t w[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i)
               w[i] = pack_16x2<F16>(__uint_as_float(o[e * 8 + 2 * i]) * inv,
                                     __uint_as_float(o[e * 8 + 2 * i + 1]) * inv);
-            *reinterpret_cast<uint4*>(stage + lane * C::kOutRow + e * 16) =
+            *reinterpret_cast<uint4*>(stage + lane * 128 + ((e ^ (lane & 7)) * 16)) =
                 make_uint4(w[0], w[1], w[2], w[3]);
           }
           __syncwarp();
-          const int d = c * 32 + (lane & 3) * 8;
+          const int d = c * 64 + (lane & 7) * 8;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint4 v = *reinterpret_cast<const uint4*>(
-                stage + (i * 8 + lane / 4) * C::kOutRow + (lane & 3) * 16);
-            if (to[i] >= 0 && d < p.D)
-              *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.o) + to[i] + d) = v;
+          for (int i = 0; i < 8; ++i) {
+            const int r = i * 4 + lane / 8;
+            const int64_t to = __shfl_sync(0xffffffffu, off, r);
+            const uint4 v = *reinterpret_cast<const uint4*>(stage + r * 128 +
+                                                            (((lane & 7) ^ (r & 7)) * 16));
+            if (to >= 0 && d < p.D)
+              *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.o) + to + d) = v;
           }
           __syncwarp();
         }
