@@ -311,6 +311,7 @@ PyObject* paged_kv_append(PyObject* const* in) {
   a.T = k.size(0);
   a.Hkv = k.size(1);
   a.D = k.size(2);
+  if (a.Hkv == 0) raise(PyExc_ValueError, "k and v must have at least one head");
   const Paged p = paged(a.T, type, a.D, in[2], in[3], in[4], in[5], in[6]);
   if (p.k_cache.size(2) != a.Hkv)
     raise(PyExc_ValueError, "the caches have %lld heads, k has %lld",

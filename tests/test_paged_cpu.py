@@ -91,6 +91,14 @@ def test_append_refusals():
             paged_kv_append(**_append_args(**change))
 
 
+def test_append_of_no_heads():
+    """Queries next to keys of no head have nothing that would write them."""
+    none = _z(3, 0, 64)
+    with pytest.raises(ValueError, match="at least one head"):
+        paged_kv_append(**_append_args(k=none, v=none, k_cache=_z(4, 16, 0, 64),
+                                       v_cache=_z(4, 16, 0, 64), q=_z(3, 4, 64)))
+
+
 def test_attention_refusals():
     good = dict(q=_z(3, 4, 64), k_cache=_z(4, 16, 2, 64), v_cache=_z(4, 16, 2, 64),
                 block_table=_z(3, 2, dtype=torch.int32), kv_lens=_ints(1, 2, 3))
