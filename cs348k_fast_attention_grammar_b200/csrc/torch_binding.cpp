@@ -11,6 +11,7 @@
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <climits>
@@ -447,18 +448,19 @@ PyObject* paged_attention(PyObject* const* in) {
   return out.obj ? given(out.obj) : THPVariable_Wrap(std::move(made));
 }
 
-// Entry: argument count, and C++ exceptions to Python errors.
+// Entry: argument count, and C++ exceptions to torch's Python errors (one for
+// memory that is out).
 template <PyObject* (*F)(PyObject* const*), int N>
 PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (n != N) return PyErr_Format(PyExc_TypeError, "%d arguments expected, got %zd", N, n);
   if (lib.check == nullptr) return PyErr_Format(PyExc_RuntimeError, "the library is not bound");
+  HANDLE_TH_ERRORS
   try {
     return F(args);
   } catch (const Raised&) {
     return nullptr;
-  } catch (const std::exception& e) {
-    return PyErr_Format(PyExc_RuntimeError, "%s", e.what());
   }
+  END_HANDLE_TH_ERRORS
 }
 
 // bind(fa_rotary, fa_paged_append, fa_paged_attn_workspace, fa_paged_attn, check):

@@ -111,3 +111,12 @@ def test_refusals_of_the_library():
         rotary(x, pos, _freq(80))                              # R > D
     with pytest.raises(FaError, match="align"):
         rotary(_x((4, 2, 68), torch.bfloat16)[..., :64], pos, _freq(64))
+
+
+def test_out_of_memory_keeps_its_type():
+    """A broadcast input may ask for an output that no device holds (2^40 values)."""
+    x, pos = _x((1, 1, 64), torch.bfloat16), torch.zeros(1, dtype=torch.int32, device=DEV)
+    with pytest.raises(torch.OutOfMemoryError):
+        rotary(x.expand(1 << 28, 64, 64), pos.expand(1 << 28), _freq(64))
+    y = _x((4, 2, 64), torch.bfloat16)
+    assert torch.equal(rotary(y, pos.expand(4), _freq(64)), y)     # angle 0: x
