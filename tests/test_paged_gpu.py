@@ -505,3 +505,40 @@ def test_streams_at_once(q_lens, room):
     torch.cuda.synchronize()
     for i in range(2):
         assert all(torch.equal(o, want[i]) for o in got[i])
+
+
+@pytest.mark.parametrize("room", ROOMS)
+@pytest.mark.parametrize("q_lens", [[1, 1], [150, 1]])
+def test_handed_from_stream_to_stream(q_lens, room):
+    """Keys stored in one stream and read in another, step by step through events."""
+    c = Cache([3000, 200], 16, 2, 64, BF16, DEV)
+    c.table = _with_room(c.table, 16, room)
+    cu, f = borders(q_lens, DEV), torch.ones(32, device=DEV)
+    n = sum(q_lens)
+    steps = [(_randn((n, 8, 64), BF16, i), _randn((n, 2, 64), BF16, i + 50),
+              _randn((n, 2, 64), BF16, i + 90)) for i in range(10)]
+    r = torch.empty_like(steps[0][0])
+
+    def store(q, k, v):
+        paged_kv_append(k, v, c.k, c.v, c.table, c.lens, cu_seqlens=cu, q=q, inv_freq=f, q_out=r)
+
+    def read(out=None):
+        return paged_attention(r, c.k, c.v, c.table, c.lens, cu_seqlens=cu, max_q_len=q_lens[0],
+                               out=out)
+
+    want = []
+    for step in steps:
+        store(*step)
+        want.append(read())
+    got = [torch.empty_like(o) for o in want]
+    left, right = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for step, out in zip(steps, got):
+        left.wait_stream(right)
+        with torch.cuda.stream(left):
+            store(*step)
+        right.wait_stream(left)
+        with torch.cuda.stream(right):
+            read(out)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
