@@ -213,7 +213,6 @@ __device__ __forceinline__ int rest_cells(const Parts& c) {
 // blocks into the CTAs' shares.  Everything waits for it (6000 clocks, of which
 // each of its prefix sums takes 400), so what it looks up again stays in shared
 // memory and its numbers are packed into 32 bits.
-constexpr int kPlanWarps = kPlanThreads / 32;
 constexpr int kMaxSplitCells = 1 << 23;       // of a batch that is cut up
 constexpr int kMaxSplitCtas = 255;
 __global__ void __launch_bounds__(kPlanThreads)
