@@ -46,6 +46,7 @@ struct Part {
   int64_t dst_sb, dst_sh, dst_ss;
   int heads, rotate;
   int items, count;                     // items of a head, of all heads
+  unsigned by_items;                    // reciprocal of items, for quotient()
 };
 
 struct RotParams {
@@ -55,6 +56,7 @@ struct RotParams {
   int64_t rows;
   int S;                                // rows of one batch entry
   int rows_per_cta, items_per_row;
+  unsigned by_row;                      // reciprocal of items_per_row
   // append only
   const int32_t* table;
   const int32_t* kv_lens;
@@ -145,6 +147,12 @@ __device__ __forceinline__ float2 cos_sin(const Angles& a, int64_t b, int64_t s,
   return cs;
 }
 
+// n / d by the reciprocal r = floor(2^32 / d) + 1, exact while n d < 2^32; r = 0
+// divides (see reciprocal()).
+__device__ __forceinline__ unsigned quotient(unsigned n, unsigned d, unsigned r) {
+  return r != 0 ? __umulhi(n, r) : n / d;
+}
+
 // An item: up to two vectors of one head.
 struct Item {
   const char* src;
@@ -180,7 +188,7 @@ __global__ void __launch_bounds__(kRotThreads, kRotCtasPerSm)
 
   auto locate = [&](unsigned it) {
     Item x;
-    x.row = it / static_cast<unsigned>(p.items_per_row);
+    x.row = quotient(it, p.items_per_row, p.by_row);
     unsigned r = it - x.row * p.items_per_row;
     x.part = 0;
     if (APPEND) {
@@ -190,7 +198,7 @@ __global__ void __launch_bounds__(kRotThreads, kRotCtasPerSm)
       }
     }
     const Part& q = p.part[x.part];
-    const unsigned head = r / static_cast<unsigned>(q.items);
+    const unsigned head = quotient(r, q.items, q.by_items);
     const unsigned chunk = r - head * q.items;
     const int64_t b = APPEND ? 0 : s_batch[x.row];
     const int64_t s = row0 + x.row - b * p.S;
@@ -320,6 +328,12 @@ __global__ void __launch_bounds__(kRotThreads, kRotCtasPerSm)
   }
 }
 
+// For quotients of numbers up to most: 0 where they would not be exact (d = 1
+// among them, whose reciprocal takes 33 bits).
+unsigned reciprocal(int64_t d, int64_t most) {
+  return d > 1 && most * d < (int64_t{1} << 32) ? static_cast<unsigned>(0xffffffffu / d + 1) : 0;
+}
+
 int launch_rotary(RotParams& p, int dtype, bool append, bool interleaved, cudaStream_t stream) {
   int dev = 0;
   const int rc = prepare_device(nullptr, 0, &dev);
@@ -346,6 +360,9 @@ int launch_rotary(RotParams& p, int dtype, bool append, bool interleaved, cudaSt
   const int64_t wave = static_cast<int64_t>(kRotCtasPerSm) * (sm_count(dev) > 0 ? sm_count(dev) : 1);
   const int64_t waves = (p.rows + rows * wave - 1) / (rows * wave);
   p.rows_per_cta = static_cast<int>((p.rows + waves * wave - 1) / (waves * wave));
+  p.by_row = reciprocal(p.items_per_row, static_cast<int64_t>(p.rows_per_cta) * p.items_per_row);
+  for (int i = 0; i < p.parts; ++i)
+    p.part[i].by_items = reciprocal(p.part[i].items, p.items_per_row);
   const int64_t grid = (p.rows + p.rows_per_cta - 1) / p.rows_per_cta;
   if (grid > 0x7fffffffLL) return FA_ERR_SHAPE;
   const unsigned g = static_cast<unsigned>(grid);
