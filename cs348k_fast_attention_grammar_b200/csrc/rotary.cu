@@ -3,12 +3,18 @@
 //     (a, b) -> (a cos t - b sin t, b cos t + a sin t),   t = position * inv_freq[i]
 //
 // Both are bound by HBM: each value is read once and written once.  A CTA of
-// 256 threads takes a few rows (tokens).  It loads its first vectors, finds the
+// 192 threads takes a few rows (tokens).  It loads its first vectors, finds the
 // rows' places and computes their sines and cosines once into shared memory while
 // those loads are in flight, then rotates and stores; a thread's item is two
 // 16-byte vectors R / 2 channels apart, so that the planes (i, i + R / 2) stay
 // inside one thread and the planes (2i, 2i + 1) inside one vector.  Every head of
 // a row shares the row's angles.
+//
+// Measured: 16384 tokens of 32 heads of 128 bf16 channels turned by three axes in
+// 43.6 us, 6.16 TB/s; 4636 tokens of 16 heads, 64 of 128 channels turned, appended
+// with their queries in 22.4 us, 5.1 TB/s (two waves of CTAs, each of which starts
+// with its rows' places: a search in the borders, a length, a table entry); one
+// token, 4 us, the launch.
 //
 // An angle of a far position needs more than fp32: position * inv_freq is
 // formed in fp64 in turns (inv_freq / 2 pi), the whole turns are dropped
@@ -23,9 +29,17 @@
 namespace fa {
 namespace {
 
-constexpr int kRotThreads = 192;        // 192 x 4 items: 2 rows of 384, 3 of 256, 6 of 128
-constexpr int kRotCtasPerSm = 8;        // by registers
-constexpr int kRotBatches = 4;          // goes of a CTA over its items
+constexpr int kRotThreads = 192;        // 192 x 4 items: 3 rows of 256 items, 6 of 128
+// Items of a thread whose loads are in flight together, and CTAs per SM (by
+// registers).  16384 tokens of 32 heads of 128 channels turned: 44.5 us with 1 item
+// and 8 CTAs, 43.6 with 2 and 6, 45.9 with 2 and 5; 4636 tokens of 16 heads appended
+// with their queries, whose CTAs first wait for their rows' places: 23.1, 25.0, 29.0.
+constexpr int rot_ahead(bool append) { return append ? 1 : 2; }
+constexpr int rot_ctas_per_sm(bool append) { return append ? 8 : 6; }
+// Goes of a CTA over its items: a row's place takes a chain of loads that the goes
+// of an append share (those tokens: 24.8 us with 2, 23.0 with 4, 22.4 with 8; the
+// rotation alone 57.7, 43.6, 46.8).
+constexpr int rot_batches(bool append) { return append ? 8 : 4; }
 constexpr int kRotMaxRows = 64;         // rows of one CTA
 constexpr int kRotMaxAngles = 2048;     // angles of one CTA (16 KiB of shared memory)
 
@@ -164,7 +178,7 @@ struct Item {
 
 // APPEND: rows are packed new tokens, keys and values go to their pages.
 template <int TYPE, bool APPEND, bool INTERLEAVED>
-__global__ void __launch_bounds__(kRotThreads, kRotCtasPerSm)
+__global__ void __launch_bounds__(kRotThreads, rot_ctas_per_sm(APPEND))
     rotary_kernel(const RotParams p) {
   constexpr int kSize = Elem<TYPE>::kSize;
   constexpr int V = 16 / kSize;
@@ -224,13 +238,18 @@ __global__ void __launch_bounds__(kRotThreads, kRotCtasPerSm)
     if (x.off1 >= 0) u1 = *reinterpret_cast<const uint4*>(x.src + x.off1);
   };
 
-  // The first item's load is in flight while places and angles are found.
+  // The first items' loads are in flight while places and angles are found.
+  constexpr bool kTwo = rot_ahead(APPEND) == 2;
   unsigned it = threadIdx.x;
-  uint4 a, c;
-  Item item;
+  uint4 a, c, a1, c1;
+  Item item, item1;
   if (it < total) {
     item = locate(it);
     load(item, a, c);
+  }
+  if (kTwo && it + kRotThreads < total) {
+    item1 = locate(it + kRotThreads);
+    load(item1, a1, c1);
   }
   if (APPEND) {
     // Where each row goes: one warp per row.
@@ -320,11 +339,18 @@ __global__ void __launch_bounds__(kRotThreads, kRotCtasPerSm)
     *reinterpret_cast<uint4*>(dst + x.off0) = pack<TYPE>(f);
     *reinterpret_cast<uint4*>(dst + x.off1) = pack<TYPE>(g);
   };
-  if (it < total) finish(item, a, c);
-  for (it += kRotThreads; it < total; it += kRotThreads) {
-    item = locate(it);
-    load(item, a, c);
+  while (it < total) {
     finish(item, a, c);
+    if (kTwo && it + kRotThreads < total) finish(item1, a1, c1);
+    it += rot_ahead(APPEND) * kRotThreads;
+    if (it < total) {
+      item = locate(it);
+      load(item, a, c);
+    }
+    if (kTwo && it + kRotThreads < total) {
+      item1 = locate(it + kRotThreads);
+      load(item1, a1, c1);
+    }
   }
 }
 
@@ -348,16 +374,15 @@ int launch_rotary(RotParams& p, int dtype, bool append, bool interleaved, cudaSt
     q.count = q.heads * q.items;
     p.items_per_row += q.count;
   }
-  // Rows per CTA: at most what its threads take in kRotBatches goes (a row's place
-  // takes a chain of loads that the goes share), within the shared memory for
-  // their angles, and so many that the CTAs fill whole waves of the device: 16
-  // heads, 64 of 128 channels turned, 4636 tokens: 26.3 us in 1.3 waves, 23.7 in
-  // two.
-  int rows = kRotBatches * kRotThreads / p.items_per_row;
+  // Rows per CTA: at most what its threads take in rot_batches() goes, within the
+  // shared memory for their angles, and so many that the CTAs fill whole waves of
+  // the device (the appended tokens above: 26.3 us in 1.3 waves, 23.7 in two).
+  int rows = rot_batches(append) * kRotThreads / p.items_per_row;
   if (half > 0) rows = rows < kRotMaxAngles / half ? rows : kRotMaxAngles / half;
   rows = rows < kRotMaxRows ? rows : kRotMaxRows;
   if (rows < 1) rows = 1;
-  const int64_t wave = static_cast<int64_t>(kRotCtasPerSm) * (sm_count(dev) > 0 ? sm_count(dev) : 1);
+  const int64_t wave =
+      static_cast<int64_t>(rot_ctas_per_sm(append)) * (sm_count(dev) > 0 ? sm_count(dev) : 1);
   const int64_t waves = (p.rows + rows * wave - 1) / (rows * wave);
   p.rows_per_cta = static_cast<int>((p.rows + waves * wave - 1) / (waves * wave));
   p.by_row = reciprocal(p.items_per_row, static_cast<int64_t>(p.rows_per_cta) * p.items_per_row);
