@@ -12,9 +12,9 @@
 //
 // Measured: 16384 tokens of 32 heads of 128 bf16 channels turned by three axes in
 // 43.6 us, 6.16 TB/s; 4636 tokens of 16 heads, 64 of 128 channels turned, appended
-// with their queries in 22.4 us, 5.1 TB/s (two waves of CTAs, each of which starts
-// with its rows' places: a search in the borders, a length, a table entry); one
-// token, 4 us, the launch.
+// with their queries in 22.4 us, 5.1 TB/s (one wave of CTAs, which starts with its
+// rows' places: a search in the borders, a length, a table entry); one token, 4 us,
+// the launch.
 //
 // An angle of a far position needs more than fp32: position * inv_freq is
 // formed in fp64 in turns (inv_freq / 2 pi), the whole turns are dropped
