@@ -21,7 +21,7 @@
 // of all (sequence, group of heads, row tile) units, one after the other, are cut
 // into equal ranges, one per team, whatever the lengths: a unit that crosses a
 // range's border leaves (m, l, O) of its parts in the workspace and
-// paged_rows_join adds them up in the order of the keys, so results do not depend
+// paged_rows_join adds them up in an order of their own, so results do not depend
 // on timing.
 #include <cuda_bf16.h>
 
@@ -79,8 +79,7 @@ __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* red, int64_t* 
   return before + x - v;
 }
 
-// A team's range [start, end) of the key blocks and the sequence that `at`
-// (start, or the range's last block) falls into.
+// A team's range [start, end) of the key blocks and the sequence that it starts in.
 struct Range {
   int64_t start, end, per;
   int64_t base;          // first key block of sequence b
@@ -88,7 +87,6 @@ struct Range {
   RowWork work;          // of sequence b
 };
 
-template <bool LAST>
 __device__ __forceinline__ Range find_range(const PagedParams& p, int team, int tile_rows) {
   __shared__ int64_t red[kRowWarps];
   __shared__ int64_t s_base;
@@ -115,7 +113,6 @@ __device__ __forceinline__ Range find_range(const PagedParams& p, int team, int 
   r.end = min(total, r.start + r.per);
   if (threadIdx.x == 0) s_b = p.B;
   __syncthreads();
-  const int64_t at = LAST ? r.end - 1 : r.start;
   if (r.start < r.end) {
     int64_t base = 0;
     for (int b0 = 0; b0 < p.B; b0 += kRowThreads) {
@@ -127,7 +124,7 @@ __device__ __forceinline__ Range find_range(const PagedParams& p, int team, int 
         if (b < p.B) w = row_work(p, b, tile_rows);
         before = block_scan(weight(p, w), red, &sum);
       }
-      if (base + before <= at && at < base + before + weight(p, w)) {
+      if (base + before <= r.start && r.start < base + before + weight(p, w)) {
         s_b = b;
         s_base = base + before;
         s_work = w;
@@ -265,8 +262,11 @@ __global__ void __launch_bounds__(RowCfg<DT, MT, CUT>::kThreads, RowCfg<DT, MT, 
     if (at < p.max_pages) ahead = p.table[rg.b * p.table_stride + at];
     rg.work = row_work(p, rg.b, C::kRows);
   } else {
-    rg = find_range<false>(p, cta / p.team, C::kRows);
-    if (rg.start >= rg.end) return;
+    rg = find_range(p, cta / p.team, C::kRows);
+    if (rg.start >= rg.end) {
+      if (threadIdx.x == 0) p.open[cta].parts = 0;
+      return;
+    }
   }
   const int page_mask = (1 << p.page_shift) - 1;
   const int crow = lane / CH, cchunk = lane % CH;
@@ -591,6 +591,13 @@ __global__ void __launch_bounds__(RowCfg<DT, MT, CUT>::kThreads, RowCfg<DT, MT, 
       cur = static_cast<int64_t>(tile) * w.blocks;
       rg.end = cur + w.blocks;
     } else if (cur >= rg.end) {
+      // The unit that this CTA begins and others end, for the join.
+      if (threadIdx.x == 0) {
+        OpenUnit u = {0, h, row0, rows, w.begin};
+        if (first && !last)
+          u.parts = 1 + static_cast<int>((w.blocks - nblk + rg.per - 1) / rg.per);
+        p.open[cta] = u;
+      }
       break;
     }
     __syncthreads();        // the ring is free again
@@ -603,73 +610,97 @@ __global__ void __launch_bounds__(RowCfg<DT, MT, CUT>::kThreads, RowCfg<DT, MT, 
   }
 }
 
-// Adds up the parts of the unit that the range of CTA blockIdx.x's team ends in,
-// when the unit begins in that range and goes on behind it.  One warp per row.
+// Adds up the parts of the unit that CTA blockIdx.x of the row kernel began and
+// others ended, row by row: the warps share the parts out, each with the loads of
+// kJoinAhead of them in flight, and their sums are added in the warps' order.
+constexpr int kJoinAhead = 8;
+constexpr int kJoinRows = 8;            // CTAs over a unit's rows, at most
 template <int DT, int MT, bool F16>
 __global__ void __launch_bounds__(kRowThreads)
     paged_rows_join(const PagedParams p) {
   using C = RowCfg<DT, MT>;
-  const int lane = threadIdx.x & 31;
-  // The row kernel starts when all before it is done, so lengths and tables can
-  // be read ahead of the wait for its parts.
-  const Range rg = find_range<true>(p, blockIdx.x / p.team, C::kRows);
+  constexpr int E = DT / 32;            // channels of a lane
+  __shared__ __align__(16) float s_acc[kRowWarps][DT];
+  __shared__ float s_top[kRowWarps], s_sum[kRowWarps];
   grid_dependency_wait();
   grid_dependents_launch();
-  if (rg.start >= rg.end) return;
-  const RowWork w = rg.work;
-  const int unit = static_cast<int>((rg.end - 1 - rg.base) / w.blocks);
-  const int64_t us = rg.base + static_cast<int64_t>(unit) * w.blocks, ue = us + w.blocks;
-  if (us < rg.start || ue <= rg.end) return;
-  const int group = unit / w.tiles;
-  const int h = group * p.team + blockIdx.x % p.team;
-  const int row0 = (unit - group * w.tiles) * C::kRows;
-  const int rows = min(C::kRows, w.q_len * p.g - row0);
-  const int parts = 1 + static_cast<int>((ue - rg.end + rg.per - 1) / rg.per);
+  const OpenUnit u = p.open[blockIdx.x];
+  if (u.parts == 0) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // Part 0 is slot 1 of this CTA, part i slot 0 of its head's in the i-th team behind.
   auto slot = [&](int i) {
     return p.part +
            static_cast<int64_t>(2 * (blockIdx.x + i * p.team) + (i == 0 ? 1 : 0)) * C::kSlot;
   };
-  for (int r = blockIdx.y * kRowWarps + (threadIdx.x >> 5); r < rows; r += gridDim.y * kRowWarps) {
-    float top = -INFINITY;
-    for (int i = lane; i < parts; i += 32) top = fmaxf(top, slot(i)[C::kRows * DT + r]);
+  for (int r = blockIdx.y; r < u.rows; r += gridDim.y) {
+    float top = -INFINITY, sum = 0.f, acc[E];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    float sum = 0.f;
-    float acc[DT / 32];
+    for (int e = 0; e < E; ++e) acc[e] = 0.f;
+    for (int i0 = warp; i0 < u.parts; i0 += kRowWarps * kJoinAhead) {
+      float m[kJoinAhead], l[kJoinAhead], x[kJoinAhead][E];
 #pragma unroll
-    for (int e = 0; e < DT / 32; ++e) acc[e] = 0.f;
-#pragma unroll 8
-    for (int i = 0; i < parts; ++i) {
-      const float* s = slot(i);
-      const float mi = s[C::kRows * DT + r];
-      const float al = mi == -INFINITY ? 0.f : ex2_approx(mi - top);
-      sum += s[C::kRows * DT + C::kRows + r] * al;
-      if constexpr (DT == 128) {
-        const float4 x = *reinterpret_cast<const float4*>(s + r * DT + lane * 4);
-        acc[0] += x.x * al;
-        acc[1] += x.y * al;
-        acc[2] += x.z * al;
-        acc[3] += x.w * al;
-      } else {
-        const float2 x = *reinterpret_cast<const float2*>(s + r * DT + lane * 2);
-        acc[0] += x.x * al;
-        acc[1] += x.y * al;
+      for (int k = 0; k < kJoinAhead; ++k) {
+        const int i = i0 + k * kRowWarps;
+        const bool in = i < u.parts;
+        const float* s = slot(in ? i : i0);
+        m[k] = in ? s[C::kRows * DT + r] : -INFINITY;
+        l[k] = s[C::kRows * DT + C::kRows + r];
+        if constexpr (DT == 128) {
+          const float4 v = *reinterpret_cast<const float4*>(s + r * DT + lane * 4);
+          x[k][0] = v.x;
+          x[k][1] = v.y;
+          x[k][2] = v.z;
+          x[k][3] = v.w;
+        } else {
+          const float2 v = *reinterpret_cast<const float2*>(s + r * DT + lane * 2);
+          x[k][0] = v.x;
+          x[k][1] = v.y;
+        }
       }
+      float now = top;
+#pragma unroll
+      for (int k = 0; k < kJoinAhead; ++k) now = fmaxf(now, m[k]);
+      const float keep = top == -INFINITY ? 0.f : ex2_approx(top - now);
+      sum *= keep;
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] *= keep;
+#pragma unroll
+      for (int k = 0; k < kJoinAhead; ++k) {
+        if (i0 + k * kRowWarps >= u.parts) continue;
+        // (a part that saw only scores that are no numbers has no maximum, but its O)
+        const float al = m[k] == -INFINITY ? 0.f : ex2_approx(m[k] - now);
+        sum += l[k] * al;
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] += x[k][e] * al;
+      }
+      top = now;
     }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    const int tok = (row0 + r) / p.g, hd = (row0 + r) - tok * p.g;
-    uint16_t* dst = static_cast<uint16_t*>(p.o) + static_cast<int64_t>(w.begin + tok) * p.o_st +
-                    static_cast<int64_t>(h * p.g + hd) * p.o_sh;
-    if constexpr (DT == 128) {
-      if (lane * 4 < p.D)
-        *reinterpret_cast<uint2*>(dst + lane * 4) =
-            make_uint2(pack_16x2<F16>(acc[0] * inv, acc[1] * inv),
-                       pack_16x2<F16>(acc[2] * inv, acc[3] * inv));
-    } else {
-      if (lane * 2 < p.D)
-        *reinterpret_cast<uint32_t*>(dst + lane * 2) = pack_16x2<F16>(acc[0] * inv, acc[1] * inv);
+#pragma unroll
+    for (int e = 0; e < E; ++e) s_acc[warp][lane * E + e] = acc[e];
+    if (lane == 0) {
+      s_top[warp] = top;
+      s_sum[warp] = sum;
     }
+    __syncthreads();
+    const int d = threadIdx.x * 2;
+    if (d < p.D) {
+      float most = -INFINITY, total = 0.f, a0 = 0.f, a1 = 0.f;
+#pragma unroll
+      for (int k = 0; k < kRowWarps; ++k) most = fmaxf(most, s_top[k]);
+#pragma unroll
+      for (int k = 0; k < kRowWarps; ++k) {
+        const float al = s_top[k] == -INFINITY ? 0.f : ex2_approx(s_top[k] - most);
+        total += s_sum[k] * al;
+        a0 += s_acc[k][d] * al;
+        a1 += s_acc[k][d + 1] * al;
+      }
+      const float inv = total == 0.f ? 0.f : 1.f / total;
+      const int tok = (u.row0 + r) / p.g, hd = (u.row0 + r) - tok * p.g;
+      uint16_t* dst = static_cast<uint16_t*>(p.o) + static_cast<int64_t>(u.begin + tok) * p.o_st +
+                      static_cast<int64_t>(u.h * p.g + hd) * p.o_sh + d;
+      *reinterpret_cast<uint32_t*>(dst) = pack_16x2<F16>(a0 * inv, a1 * inv);
+    }
+    __syncthreads();
   }
 }
 
@@ -695,7 +726,7 @@ int launch_rows(const PagedParams& p, Cut cut, int rows, cudaStream_t stream) {
   const int rc = launch_rows_kernel<DT, MT, F16, kSplit>(p, stream);
   if (rc != FA_OK) return rc;
   return launch_after(paged_rows_join<DT, MT, F16>,
-                      dim3(p.ctas * p.team, (rows + kRowWarps - 1) / kRowWarps), kRowThreads, 0, 1,
+                      dim3(p.ctas * p.team, rows < kJoinRows ? rows : kJoinRows), kRowThreads, 0, 1,
                       stream, p);
 }
 
@@ -838,6 +869,11 @@ Teams row_teams(const fa_paged_attn_args* a, const Choice& c, int sms) {
   return best;
 }
 
+// A CTA's parts of units: of the one that its range begins in and of the last.
+int64_t part_bytes(const fa_paged_attn_args* a, const Choice& c) {
+  return 2 * (c.rows32 ? 32 : 16) * ((a->D <= 64 ? 64 : 128) + 2) * 4;
+}
+
 }  // namespace
 }  // namespace fa
 
@@ -853,8 +889,7 @@ extern "C" int64_t fa_paged_attn_workspace(const fa_paged_attn_args* a) {
   if (c.tiles) return paged_tiles_bytes(a, sms);
   if (c.cut != kSplit) return 0;
   const Teams t = row_teams(a, c, sms);
-  return 2ll * t.heads * t.count * (c.rows32 ? 32 : 16) *
-         ((a->D <= 64 ? 64 : 128) + 2) * 4;
+  return t.heads * t.count * (static_cast<int64_t>(sizeof(OpenUnit)) + part_bytes(a, c));
 }
 
 extern "C" int fa_paged_attn(const fa_paged_attn_args* a, void* workspace,
@@ -913,6 +948,8 @@ extern "C" int fa_paged_attn(const fa_paged_attn_args* a, void* workspace,
   p.tile_ctas = c.tile_ctas;
   p.cluster_shift = c.cluster_shift;
   p.part = static_cast<float*>(workspace);
+  p.open = reinterpret_cast<OpenUnit*>(static_cast<char*>(workspace) +
+                                       t.heads * t.count * part_bytes(a, c));
   p.min_blocks = 4;
   // (the join's CTAs go over more rows than these where max_q_len was too small)
   const int64_t longest = (a->max_q_len < a->T ? a->max_q_len : a->T) * p.g;

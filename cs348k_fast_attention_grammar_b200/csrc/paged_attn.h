@@ -7,6 +7,13 @@
 
 namespace fa {
 
+// Row kernel: the unit (rows of one head) that a CTA begins and others end.
+struct OpenUnit {
+  int parts;                            // 0: there is none
+  int h, row0, rows, begin;             // head, rows of the sequence, its first token
+  int pad[3];
+};
+
 struct PagedParams {
   const void* q;
   void* o;
@@ -25,6 +32,7 @@ struct PagedParams {
   float scale_log2;
   int* status;
   float* part;                          // partial results of split units
+  OpenUnit* open;                       // row kernel: one of each CTA, for the join
   int ctas;                             // ranges the key blocks are cut into
   int min_blocks;                       // least key blocks of a range
   int team;                             // row kernel: heads that stream side by side
