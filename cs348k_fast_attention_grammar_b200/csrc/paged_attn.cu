@@ -7,12 +7,13 @@
 //
 // paged_rows_kernel takes sequences of few rows (a generation step).  It is
 // bound by HBM: two passes' worth of arithmetic per key and row is far below
-// what even warp-level matrix instructions deliver, so the kernel is built
-// around its loads.  A CTA has four warps (more for short tables, below); per
-// 64-key block each warp owns 16 keys, loads their K and V rows with 16-byte
-// asynchronous copies into a ring of its own (no barrier between warps), and
-// keeps its own running maximum, sum and output, joined over the warps when the
-// CTA leaves a tile.
+// what even warp-level matrix instructions deliver (tcgen05 would put its 16 rows
+// into tiles of 128), so the kernel is built around its loads.  A CTA has four warps
+// (more for short tables, below); per 64-key block each warp owns 16 keys, loads
+// their K and V rows with 16-byte asynchronous copies into a ring of its own (no
+// barrier between warps), and keeps its own running maximum, sum and output, joined
+// over the warps when the CTA leaves a tile.  32 sequences of up to 8192 keys, 32/8
+// heads of 128: 111 us, 6.15 TB/s; 3 of up to 131072, 32/4 heads: 106 us, 6.0 TB/s.
 //
 // CTAs work in teams of up to 16 key heads, a head each, that walk the same keys
 // side by side: a cached token's heads lie next to each other, and DRAM is read
@@ -487,7 +488,7 @@ __global__ void __launch_bounds__(RowCfg<DT, MT, CUT>::kThreads, RowCfg<DT, MT, 
     }
     cp_async_wait<0>();
 
-    // Join the warps: everything against the largest of the four maxima.
+    // Join the warps: everything against the largest of their maxima.
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -775,13 +776,19 @@ int check_paged_attn(const fa_paged_attn_args* a) {
 // Which kernel runs, by sizes that the host knows.
 //  * Few rows: the row kernel with a cluster per sequence, head and 16 rows, of
 //    CTAs of 16 warps (8 with D > 64), as many as get 2 steps or more of their own
-//    and leave a CTA per SM, up to 16 steps of each (8 of a single CTA).
-//    37 tokens over 1061 keys, 16 heads of 64: 10 us, 16.5 split and joined, 21 by
-//    the tile kernel.
-//  * The row kernel takes the other sequences of up to kRowMax rows (single
-//    tokens), and chunks whose products over the whole table are at most kRowWork
-//    operations; over up to 1024 keys again without a join (256 sequences of 512
-//    keys, 8 heads of 64: 36 us against 51).
+//    and leave a CTA per SM, up to 8 steps of each.  37 tokens over 1061 keys, 16
+//    heads of 64: 9.6 us, 16.5 split and joined, 21 by the tile kernel.  8 sequences
+//    of up to 2000 keys, 32/8 heads of 128: 12.3 us, split 14.8; 2 of up to 8192
+//    (16 steps): 18.2, split 13.1.
+//  * Over up to 1024 keys again no join: a CTA per sequence, head and 32 rows, for
+//    sequences of up to kRowMax rows (256 sequences of 512 keys, 8 heads of 64: 36
+//    us, split 51) and for calls of up to kWholeWork operations over the whole
+//    table (28 sequences of up to 30 tokens over 73 keys, 24/2 heads of 80: 11.4 us,
+//    15.7 by the tile kernel, 33.6 split; 5 of up to 188 tokens, 32/2 heads of 96,
+//    above it: 25, 16.8 by the tile kernel).
+//  * Split and joined, the row kernel takes the other sequences of up to kRowMax
+//    rows (single tokens), and chunks of up to kRowWork operations, where the tile
+//    kernel's plan and join cost more than its products save.
 //  * The tile kernel takes chunks, and then the batch's short sequences too: a
 //    second launch for those costs more than a tile kernel's unit of one token.
 constexpr int kRowMax = 32;
@@ -836,7 +843,7 @@ Choice choose(const fa_paged_attn_args* a, int dev, int sms) {
     while (shift < 3 && keys > (2ll << shift) * step &&
            units * tiles16 <= max_clusters(dev, a->D <= 64, shift + 1))
       ++shift;
-    if (keys <= (shift == 0 ? 8 : 16) * (static_cast<int64_t>(step) << shift))
+    if (keys <= 8 * (static_cast<int64_t>(step) << shift))
       return {false, false, kWholeWide, static_cast<int>(tiles16), shift};
   }
   const double most = 4.0 * a->T * a->Hq * a->D * keys;
