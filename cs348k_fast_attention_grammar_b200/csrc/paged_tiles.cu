@@ -12,8 +12,17 @@
 //   warp 9          TMEM allocation and the single thread that issues tcgen05.mma
 //   warp 10         loads V by pages into the ring
 // S_t lives in TMEM columns [128 t, 128 t + 128), P_t over its first half as 16-bit
-// pairs, O_t at 256 + D t.  The kernel is bound by the chain S -> softmax -> P of
-// each tile, about 2900 clocks per 128 keys for 2048 clocks of tensor work.
+// pairs, O_t at 256 + D t.
+//
+// Bound by the power limit and by the chain S -> softmax -> P of each tile: 2800
+// clocks per 128 keys for 2048 clocks of tensor work (D = 128).  512 tokens over
+// 32768 keys, 32/8 heads of 128: 214 us, 1270 TFLOP/s, the tensor pipe 72 % active at
+// 1.56 GHz, which is where the power limit holds the clock; a causal prompt of 8192
+// tokens, 32 heads of 128: 430 us, 1280 TFLOP/s.  With D = 64 the softmax alone
+// takes the 2800 clocks (half the issue slots, 58 % of the exponential unit), 635
+// TFLOP/s: room for P beside S, so that S comes a block ahead, did not change that
+// (chunk above: 223 us, 232), and neither did four tiles of 64 keys (203 and 191,
+// but 114 and 131 over shorter lists).
 //
 // Pages: a load box is min(page_size, 128) rows of one page, so a 128-key tile
 // takes 128 / page_size boxes whose pages come from the block table, one lane of
@@ -32,7 +41,7 @@
 //    cut into equal ranges for the other CTAs.  The parts of one head's units begin
 //    at the same keys, so the CTAs that read them run side by side in the L2: with
 //    plain equal ranges 512 tokens over 32768 keys (8 key heads of 128) read the
-//    cache from DRAM once for each of a head's 8 units (244 us, now 221).
+//    cache from DRAM once for each of a head's 8 units (244 us against 221).
 // A unit's parts leave (m, l, O) in the workspace and paged_tiles_join adds them
 // in the order of the keys.
 // Results depend on the lengths alone, never on timing.
