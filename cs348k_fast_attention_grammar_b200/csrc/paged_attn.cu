@@ -612,8 +612,9 @@ __global__ void __launch_bounds__(RowCfg<DT, MT, CUT>::kThreads, RowCfg<DT, MT, 
 }
 
 // Adds up the parts of the unit that CTA blockIdx.x of the row kernel began and
-// others ended, row by row: the warps share the parts out, each with the loads of
-// kJoinAhead of them in flight, and their sums are added in the warps' order.
+// others ended.  A warp has the loads of kJoinAhead parts of a row in flight; of more
+// parts the CTA's warps take a share each, and their sums are added in the warps'
+// order.
 constexpr int kJoinAhead = 8;
 constexpr int kJoinRows = 8;            // CTAs over a unit's rows, at most
 template <int DT, int MT, bool F16>
@@ -633,15 +634,18 @@ __global__ void __launch_bounds__(kRowThreads)
     return p.part +
            static_cast<int64_t>(2 * (blockIdx.x + i * p.team) + (i == 0 ? 1 : 0)) * C::kSlot;
   };
-  for (int r = blockIdx.y; r < u.rows; r += gridDim.y) {
-    float top = -INFINITY, sum = 0.f, acc[E];
+  float top, sum, acc[E];
+  // Parts first, first + step, ... of row r.
+  auto add = [&](int r, int first, int step) {
+    top = -INFINITY;
+    sum = 0.f;
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] = 0.f;
-    for (int i0 = warp; i0 < u.parts; i0 += kRowWarps * kJoinAhead) {
+    for (int i0 = first; i0 < u.parts; i0 += step * kJoinAhead) {
       float m[kJoinAhead], l[kJoinAhead], x[kJoinAhead][E];
 #pragma unroll
       for (int k = 0; k < kJoinAhead; ++k) {
-        const int i = i0 + k * kRowWarps;
+        const int i = i0 + k * step;
         const bool in = i < u.parts;
         const float* s = slot(in ? i : i0);
         m[k] = in ? s[C::kRows * DT + r] : -INFINITY;
@@ -667,7 +671,7 @@ __global__ void __launch_bounds__(kRowThreads)
       for (int e = 0; e < E; ++e) acc[e] *= keep;
 #pragma unroll
       for (int k = 0; k < kJoinAhead; ++k) {
-        if (i0 + k * kRowWarps >= u.parts) continue;
+        if (i0 + k * step >= u.parts) continue;
         // (a part that saw only scores that are no numbers has no maximum, but its O)
         const float al = m[k] == -INFINITY ? 0.f : ex2_approx(m[k] - now);
         sum += l[k] * al;
@@ -676,6 +680,26 @@ __global__ void __launch_bounds__(kRowThreads)
       }
       top = now;
     }
+  };
+  auto row_out = [&](int r) {
+    const int tok = (u.row0 + r) / p.g, hd = (u.row0 + r) - tok * p.g;
+    return static_cast<uint16_t*>(p.o) + static_cast<int64_t>(u.begin + tok) * p.o_st +
+           static_cast<int64_t>(u.h * p.g + hd) * p.o_sh;
+  };
+  if (u.parts <= kJoinAhead) {
+    for (int r = blockIdx.y * kRowWarps + warp; r < u.rows; r += gridDim.y * kRowWarps) {
+      add(r, 0, 1);
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+      for (int e = 0; e < E; e += 2)
+        if (lane * E < p.D)
+          *reinterpret_cast<uint32_t*>(row_out(r) + lane * E + e) =
+              pack_16x2<F16>(acc[e] * inv, acc[e + 1] * inv);
+    }
+    return;
+  }
+  for (int r = blockIdx.y; r < u.rows; r += gridDim.y) {
+    add(r, warp, kRowWarps);
 #pragma unroll
     for (int e = 0; e < E; ++e) s_acc[warp][lane * E + e] = acc[e];
     if (lane == 0) {
@@ -696,10 +720,7 @@ __global__ void __launch_bounds__(kRowThreads)
         a1 += s_acc[k][d + 1] * al;
       }
       const float inv = total == 0.f ? 0.f : 1.f / total;
-      const int tok = (u.row0 + r) / p.g, hd = (u.row0 + r) - tok * p.g;
-      uint16_t* dst = static_cast<uint16_t*>(p.o) + static_cast<int64_t>(u.begin + tok) * p.o_st +
-                      static_cast<int64_t>(u.h * p.g + hd) * p.o_sh + d;
-      *reinterpret_cast<uint32_t*>(dst) = pack_16x2<F16>(a0 * inv, a1 * inv);
+      *reinterpret_cast<uint32_t*>(row_out(r) + d) = pack_16x2<F16>(a0 * inv, a1 * inv);
     }
     __syncthreads();
   }
