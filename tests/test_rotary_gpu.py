@@ -120,3 +120,13 @@ def test_out_of_memory_keeps_its_type():
         rotary(x.expand(1 << 28, 64, 64), pos.expand(1 << 28), _freq(64))
     y = _x((4, 2, 64), torch.bfloat16)
     assert torch.equal(rotary(y, pos.expand(4), _freq(64)), y)     # angle 0: x
+
+
+@pytest.mark.parametrize("B,H,S,D,R", [(1, 4096, 2, 256, 256), (1, 2, 5000, 64, 32),
+                                       (3, 7, 1999, 128, 128), (1, 65536, 1, 16, 16)])
+def test_wide_rows_and_many(B, H, S, D, R):
+    """Rows of more items than a CTA takes at once, and more rows than one wave of CTAs."""
+    x, f = _x((B, H, S, D), torch.bfloat16), _freq(R)
+    pos = torch.arange(S, device=DEV) * 3
+    want, size = rotate(x, pos.double()[:, None] * f.double())
+    assert_within(rotary(x, pos, f), want, rotary_tolerance(want, size, x.dtype))
