@@ -13,7 +13,7 @@
 // their K and V rows with 16-byte asynchronous copies into a ring of its own (no
 // barrier between warps), and keeps its own running maximum, sum and output, joined
 // over the warps when the CTA leaves a tile.  32 sequences of up to 8192 keys, 32/8
-// heads of 128: 111 us, 6.15 TB/s; 3 of up to 131072, 32/4 heads: 106 us, 6.0 TB/s.
+// heads of 128: 110.5 us, 6.2 TB/s; 3 of up to 131072, 32/4 heads: 104.7 us, 6.1 TB/s.
 //
 // CTAs work in teams of up to 16 key heads, a head each, that walk the same keys
 // side by side: a cached token's heads lie next to each other, and DRAM is read
@@ -24,6 +24,11 @@
 // range's border leaves (m, l, O) of its parts in the workspace and
 // paged_rows_join adds them up in an order of their own, so results do not depend
 // on timing.
+//
+// Neither kernel lets its dependents start before it ends: CTAs that wait beside it
+// cost more than they save (32 sequences of up to 8192 keys, 16 heads of 64: 138
+// us with early starts, where the next call's CTAs then all begin at one moment, 112
+// without; 3 of up to 131072, 32/4 heads of 128: 106.2, 104.7).
 #include <cuda_bf16.h>
 
 #include <atomic>
@@ -239,7 +244,6 @@ __global__ void __launch_bounds__(RowCfg<DT, MT, CUT>::kThreads, RowCfg<DT, MT, 
   constexpr int RPI = 32 / CH;          // rows one warp-wide copy covers
   extern __shared__ __align__(128) uint8_t smem[];
   grid_dependency_wait();
-  grid_dependents_launch();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t ring = smem_u32(smem) + warp * C::kWarp;
   float* s_o = reinterpret_cast<float*>(smem);
@@ -625,7 +629,6 @@ __global__ void __launch_bounds__(kRowThreads)
   __shared__ __align__(16) float s_acc[kRowWarps][DT];
   __shared__ float s_top[kRowWarps], s_sum[kRowWarps];
   grid_dependency_wait();
-  grid_dependents_launch();
   const OpenUnit u = p.open[blockIdx.x];
   if (u.parts == 0) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -798,7 +801,7 @@ int check_paged_attn(const fa_paged_attn_args* a) {
 //  * Few rows: the row kernel with a cluster per sequence, head and 16 rows, of
 //    CTAs of 16 warps (8 with D > 64), as many as get 2 steps or more of their own
 //    and leave a CTA per SM, up to 8 steps of each.  37 tokens over 1061 keys, 16
-//    heads of 64: 9.6 us, 16.5 split and joined, 21 by the tile kernel.  8 sequences
+//    heads of 64: 9.4 us, 16.5 split and joined, 21 by the tile kernel.  8 sequences
 //    of up to 2000 keys, 32/8 heads of 128: 12.3 us, split 14.8; 2 of up to 8192
 //    (16 steps): 18.2, split 13.1.
 //  * Over up to 1024 keys again no join: a CTA per sequence, head and 32 rows, for

