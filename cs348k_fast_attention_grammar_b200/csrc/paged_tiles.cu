@@ -418,23 +418,25 @@ __global__ void __launch_bounds__(kPlanThreads)
 // Exponentials: a quarter of them on the FMA pipe
 // ---------------------------------------------------------------------------
 // 2^x for two values: x = j + f with j the nearest whole number (the addition of
-// 1.5 * 2^23 leaves it in the low mantissa bits), 2^f by the degree-3 minimax
-// polynomial of fit_exp2_poly.py (relative error 7.5e-5), j added to the exponent.
-// x is held at -125, so a masked score gives 2^-125 instead of 0.
+// 1.5 * 2^23 + 127 leaves j + 127 in the low mantissa bits), 2^f by the degree-3
+// minimax polynomial of fit_exp2_poly.py (relative error 7.5e-5), times 2^j made of
+// those bits.  x is held at -127, where 2^j is 0: a masked score weighs exactly
+// nothing, whatever finite value it would multiply.  (Adding j to the exponent
+// instead saves a product of every 2 values, but can give no less than 2^-125.)
 __device__ __forceinline__ void exp2_pair(float x0, float x1, float& r0, float& r1) {
-  const uint64_t x = f2_pack(fmaxf(x0, -125.f), fmaxf(x1, -125.f));
-  const uint64_t t = fadd2(x, f2_pack(12582912.f, 12582912.f));
-  const uint64_t j = fadd2(t, f2_pack(-12582912.f, -12582912.f));
+  const uint64_t x = f2_pack(fmaxf(x0, -127.f), fmaxf(x1, -127.f));
+  const uint64_t t = fadd2(x, f2_pack(12583039.f, 12583039.f));
+  const uint64_t j = fadd2(t, f2_pack(-12583039.f, -12583039.f));
   const uint64_t f = ffma2(j, f2_pack(-1.f, -1.f), x);
   uint64_t q = ffma2(f2_pack(0.0551716685295105f, 0.0551716685295105f), f,
                      f2_pack(0.2426111251115799f, 0.2426111251115799f));
   q = ffma2(q, f, f2_pack(0.6932609677314758f, 0.6932609677314758f));
   q = ffma2(q, f, f2_pack(0.9999280571937561f, 0.9999280571937561f));
-  float p0, p1, t0, t1;
-  f2_unpack(q, p0, p1);
+  float t0, t1;
   f2_unpack(t, t0, t1);
-  r0 = __int_as_float(__float_as_int(p0) + (__float_as_int(t0) << 23));
-  r1 = __int_as_float(__float_as_int(p1) + (__float_as_int(t1) << 23));
+  q = fmul2(q, f2_pack(__int_as_float(__float_as_int(t0) << 23),
+                       __int_as_float(__float_as_int(t1) << 23)));
+  f2_unpack(q, r0, r1);
 }
 
 // The largest of three; NaN if one is (the exponentials on the FMA pipe would lose it).
@@ -920,9 +922,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_after();
         ++ou;
       }
-      // A row that saw no key holds 2^-125 of it per masked exponential: zero.
-      // (l is NaN where the scores were, and stays so.)
-      if (m_ref == -INFINITY && l == l) l = 0.f;
       const float inv = l == 0.f ? 0.f : 1.f / l;
       const int h = ring[us].h, q_begin = ring[us].q_begin, slot = ring[us].slot;
       const int tok = ring[us].tok0 + t * p.tq + row_tok;

@@ -1,0 +1,93 @@
+"""Edges of the paged operators against their definitions in fp64: infinite scores, weights of
+masked keys, scales near zero, lengths and pages that the table does not hold, borders outside the
+packed rows, the order of what the status word reports."""
+
+import math
+
+import pytest
+import torch
+
+from cs348k_fast_attention_grammar_b200 import (_lib, device_status, paged_attention,
+                                                paged_kv_append)
+from paged_reference import (Cache, assert_within, attention as reference, attention_tolerance,
+                             borders)
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+FA_ERR_TIMEOUT, FA_ERR_PAGE = 11, 14
+BF16, F16 = torch.bfloat16, torch.float16
+INF = float("inf")
+
+# (tokens, lengths, query heads, key heads, room in the table): clusters of the row kernel, its whole
+# units, its split ranges; the tile kernel with whole units and with cut ones.
+PATHS = {
+    "clusters": ([1, 60, 40], [300, 60, 90], 2, 1, 0),
+    "whole": ([3, 16, 9] * 40, [300, 60, 90] * 40, 8, 4, 0),
+    "split": ([3, 16, 9], [300, 60, 90], 2, 1, 1 << 18),
+    "tiles": ([1, 60, 40], [300, 60, 90], 8, 4, 1 << 18),
+    "tiles cut": ([200, 3], [5000, 700], 8, 2, 1 << 18),
+}
+
+
+def _randn(shape, dtype, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    return torch.randn(shape, generator=g).to(dtype).to(DEV)
+
+
+def _problem(path, dtype=BF16, D=64, page=16):
+    q_lens, kv_lens, Hq, Hkv, room = PATHS[path]
+    c = Cache(kv_lens, page, Hkv, D, dtype, DEV)
+    more = max(0, -(-room // page) - c.table.shape[1])
+    c.table = torch.nn.functional.pad(c.table, (0, more), value=-3)
+    q = _randn((sum(q_lens), Hq, D), dtype, 1)
+    return c, q, q_lens, kv_lens
+
+
+def _call(c, q, q_lens, **kw):
+    return paged_attention(q, c.k, c.v, c.table, c.lens, cu_seqlens=borders(q_lens, DEV),
+                           max_q_len=max(q_lens), **kw)
+
+
+def _slot(c, b, key):
+    page = c.k.shape[1]
+    return int(c.table[b, key // page]), key % page
+
+
+def _definition(c, q, q_lens, kv_lens):
+    """Causal attention in fp64 as it is written, and sum_j p_j |v_j|: a score of +inf or NaN makes
+    its row NaN, one of -inf has no weight, a row all of whose scores are -inf is zero."""
+    scale = 1.0 / math.sqrt(q.shape[2])
+    out, size, g, row = [], [], q.shape[1] // c.k.shape[2], 0
+    for b, (n, kv) in enumerate(zip(q_lens, kv_lens)):
+        ids = c.table[b, :-(-kv // c.k.shape[1])].long()
+        k, v = (t[ids].flatten(0, 1)[:kv].double().repeat_interleave(g, 1) for t in (c.k, c.v))
+        # (products and their sum one by one: a matrix product may order infinities otherwise)
+        s = (q[row:row + n, None].double() * k[None]).sum(-1).movedim(2, 1) * scale
+        hidden = torch.arange(kv, device=DEV) > torch.arange(kv - n, kv, device=DEV)[:, None]
+        s = s.masked_fill(hidden[:, None], -INF)
+        p = torch.softmax(s, -1)
+        p = torch.where((s == -INF).all(-1, keepdim=True), 0.0, p)
+        out.append(torch.einsum("nhk,khe->nhe", p, v))
+        size.append(torch.einsum("nhk,khe->nhe", p, v.abs()))
+        row += n
+    return torch.cat(out), torch.cat(size)
+
+
+# --------------------------------------------------------------------------- masked keys
+@pytest.mark.parametrize("path", PATHS)
+def test_masked_keys_have_no_weight(path):
+    """Tokens that see values of zero get zeros, whatever finite values the later ones hold."""
+    c, q, q_lens, kv_lens = _problem(path)
+    row = 0
+    for b, (n, kv) in enumerate(zip(q_lens, kv_lens)):
+        ids = c.table[b, :-(-kv // 16)].long()
+        v = c.v[ids].flatten(0, 1)
+        v[:kv] = 0
+        v[kv - n // 2:kv] = 2.0 ** 110
+        c.v[ids] = v.unflatten(0, (len(ids), 16))
+    want, size = reference(q, c.k, c.v, c.table, kv_lens, q_lens)
+    got = _call(c, q, q_lens)
+    assert_within(got, want, attention_tolerance(want, size, BF16, max(kv_lens)), path)
+    for n in q_lens:
+        assert not got[row:row + n - n // 2].any(), f"{path}, rows {row}.."
+        row += n
