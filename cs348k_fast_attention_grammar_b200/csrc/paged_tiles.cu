@@ -417,14 +417,27 @@ __global__ void __launch_bounds__(kPlanThreads)
 // ---------------------------------------------------------------------------
 // Exponentials: a quarter of them on the FMA pipe
 // ---------------------------------------------------------------------------
+// The largest of two or three; NaN if one is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
 // 2^x for two values: x = j + f with j the nearest whole number (the addition of
 // 1.5 * 2^23 + 127 leaves j + 127 in the low mantissa bits), 2^f by the degree-3
 // minimax polynomial of fit_exp2_poly.py (relative error 7.5e-5), times 2^j made of
 // those bits.  x is held at -127, where 2^j is 0: a masked score weighs exactly
 // nothing, whatever finite value it would multiply.  (Adding j to the exponent
 // instead saves a product of every 2 values, but can give no less than 2^-125.)
+// NaN, which an infinite score less an infinite reference is, stays NaN.
 __device__ __forceinline__ void exp2_pair(float x0, float x1, float& r0, float& r1) {
-  const uint64_t x = f2_pack(fmaxf(x0, -127.f), fmaxf(x1, -127.f));
+  const uint64_t x = f2_pack(max_nan(x0, -127.f), max_nan(x1, -127.f));
   const uint64_t t = fadd2(x, f2_pack(12583039.f, 12583039.f));
   const uint64_t j = fadd2(t, f2_pack(-12583039.f, -12583039.f));
   const uint64_t f = ffma2(j, f2_pack(-1.f, -1.f), x);
@@ -437,13 +450,6 @@ __device__ __forceinline__ void exp2_pair(float x0, float x1, float& r0, float& 
   q = fmul2(q, f2_pack(__int_as_float(__float_as_int(t0) << 23),
                        __int_as_float(__float_as_int(t1) << 23)));
   f2_unpack(q, r0, r1);
-}
-
-// The largest of three; NaN if one is (the exponentials on the FMA pipe would lose it).
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
 }
 
 // ---------------------------------------------------------------------------

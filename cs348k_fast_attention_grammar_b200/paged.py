@@ -103,8 +103,9 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
 
     Caches, table and lengths as in ``paged_kv_append``; query head ``i`` reads
     key head ``i // (Hq // Hkv)``.  With ``causal`` a token sees the keys up to
-    its own place in the sequence, else all ``kv_lens[b]``; one that sees none
-    gets zeros.  ``scale`` defaults to ``1/sqrt(D)``.  ``max_q_len``, the longest
+    its own place in the sequence, else all ``kv_lens[b]``; one that sees none,
+    or none with a score above -infinity, gets zeros.  A score of +infinity or NaN
+    makes its token's output NaN.  ``scale`` defaults to ``1/sqrt(D)``.  ``max_q_len``, the longest
     sequence's number of new tokens, lets the call choose its kernels (default:
     one without ``cu_seqlens``, else unknown); it never changes what is computed.
     Rows of no sequence are left as they were in ``out``.  Cached values that a

@@ -299,8 +299,9 @@ int fa_paged_append(const fa_paged_append_args* args, void* stream);
  * Attention of new tokens (one or a chunk per sequence) over the paged cache
  * that holds them:  o = softmax(q K^T * scale) V  per token and head, query
  * heads in Hkv groups that share a key/value head.  With `causal` a token sees
- * the keys up to its own place, else all kv_lens[b].  A token that sees no key
- * gets zeros.  Rows outside every sequence have no effect and are not written.
+ * the keys up to its own place, else all kv_lens[b].  A token that sees no key,
+ * or none with a score above -infinity, gets zeros; a score of +infinity or NaN
+ * makes its output NaN.  Rows outside every sequence have no effect and are not written.
  * A page outside the cache reads as zeros and a length behind the table is cut
  * there; both leave FA_ERR_PAGE in the device status word.  Cached values that
  * a sequence's tokens see must be finite (a value that only some of a chunk's

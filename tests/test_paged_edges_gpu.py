@@ -73,6 +73,62 @@ def _definition(c, q, q_lens, kv_lens):
     return torch.cat(out), torch.cat(size)
 
 
+# --------------------------------------------------------------------------- infinite scores
+def _assert_nan_alike(got, want, tol, what):
+    bad = want.isnan()
+    assert torch.equal(got.isnan(), bad), f"{what}: {int((got.isnan() != bad).sum())} values"
+    assert_within(got[~bad], want[~bad], tol[~bad], what)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("path", PATHS)
+def test_infinite_keys(path, dtype):
+    """One infinite channel of one key, at every place of 16: a token that sees it gets NaN where
+    its score is +inf, and no weight of it where the score is -inf."""
+    for place in range(16):
+        c, q, q_lens, kv_lens = _problem(path, dtype)
+        b = q_lens.index(max(q_lens))
+        key = kv_lens[b] - 16 + place
+        pg, r = _slot(c, b, key)
+        c.k[pg, r, 0, 3] = INF if place % 4 < 2 else -INF
+        q[sum(q_lens[:b + 1]) - 1, 0, 3] = 1 if place % 4 < 2 else -1
+        want, size = _definition(c, q, q_lens, kv_lens)
+        tol = attention_tolerance(want, size, dtype, max(kv_lens))
+        assert want.isnan().any() and not want.isnan().all()
+        _assert_nan_alike(_call(c, q, q_lens), want, tol, f"{path}, key {key}")
+    assert device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("path", PATHS)
+def test_infinite_queries(path, dtype):
+    """One infinite channel of a query: its row is NaN if a key that it sees has that channel on
+    the same side of zero."""
+    c, q, q_lens, kv_lens = _problem(path, dtype)
+    at = torch.arange(q.shape[0], device=DEV) % 3 == 1
+    q[at, :, 5] = INF
+    want, size = _definition(c, q, q_lens, kv_lens)
+    tol = attention_tolerance(want, size, dtype, max(kv_lens))
+    assert want.isnan().any()
+    _assert_nan_alike(_call(c, q, q_lens), want, tol, path)
+
+
+def test_an_infinite_score_of_rows_that_see_few_keys():
+    """A prompt whose tokens see 1, 2, 3, ... keys, each key's score +inf in turn."""
+    n = 40
+    for Hkv, room in ((1, 0), (8, 1 << 18)):
+        for place in range(16):
+            c = Cache([n], 16, Hkv, 64, BF16, DEV)
+            c.table = torch.nn.functional.pad(c.table, (0, room // 16), value=-3)
+            q = _randn((n, 2 * Hkv, 64), BF16, 2)
+            q[:, :, 9] = 1
+            pg, r = _slot(c, 0, place)
+            c.k[pg, r, :, 9] = INF
+            got = _call(c, q, [n])
+            assert got[place:].isnan().all(), (Hkv, place)
+            assert got[:place].isfinite().all(), (Hkv, place)
+
+
 # --------------------------------------------------------------------------- masked keys
 @pytest.mark.parametrize("path", PATHS)
 def test_masked_keys_have_no_weight(path):
