@@ -849,6 +849,10 @@ int max_clusters(int dev, bool narrow, int shift) {
   return n;
 }
 
+float scale_log2(const fa_paged_attn_args* a) {
+  return static_cast<float>(a->scale * 1.4426950408889634);
+}
+
 struct Choice {
   bool tiles;
   bool rows32;          // row tiles of 32 rows, else 16
@@ -873,14 +877,15 @@ Choice choose(const fa_paged_attn_args* a, int dev, int sms) {
   const double most = 4.0 * a->T * a->Hq * a->D * keys;
   if (keys <= 1024 && (longest <= kRowMax || most <= kWholeWork) && units <= 0x7fffffffLL / tiles32)
     return {false, longest > 16, kWhole, static_cast<int>(tiles32), 0};
-  // The tile kernel's copies need real strides, its exponent a scale that keeps order.
+  // The tile kernel's copies need real strides; it masks scores before it scales them
+  // and takes the maximum before, so its scale has to keep their order and -infinity.
   const bool flat = (a->q_strides[0] == 0 && a->T > 1) || (a->q_strides[1] == 0 && a->Hq > 1) ||
                     (a->k_cache_strides[0] == 0 && a->pages > 1) || a->k_cache_strides[1] == 0 ||
                     (a->k_cache_strides[2] == 0 && a->Hkv > 1) ||
                     (a->v_cache_strides[0] == 0 && a->pages > 1) || a->v_cache_strides[1] == 0 ||
                     (a->v_cache_strides[2] == 0 && a->Hkv > 1);
-  return {longest > kRowMax && most > kRowWork && !flat && a->scale >= 0, longest > 16, kSplit, 1,
-          0};
+  const bool ordered = scale_log2(a) > 0.f;
+  return {longest > kRowMax && most > kRowWork && !flat && ordered, longest > 16, kSplit, 1, 0};
 }
 
 // Teams of the row kernel: of the size, up to 16 heads, that fills the device
@@ -962,7 +967,7 @@ extern "C" int fa_paged_attn(const fa_paged_attn_args* a, void* workspace,
   p.page_shift = __builtin_ctzll(static_cast<unsigned long long>(a->page_size));
   p.max_pages = static_cast<int>(a->max_pages);
   p.causal = a->causal != 0;
-  p.scale_log2 = static_cast<float>(a->scale * 1.4426950408889634);
+  p.scale_log2 = scale_log2(a);
   p.status = device_status_ptr();
   if (p.status == nullptr) return FA_ERR_CUDA;
   const int sms = sm_count(dev);

@@ -1172,8 +1172,6 @@ int launch_paged_tiles(const fa_paged_attn_args* a, const PagedParams& q, void* 
   static_cast<PagedParams&>(p) = q;
   p.tq = tile_tokens(a);
   p.box_rows = a->page_size < kKeys ? static_cast<int>(a->page_size) : kKeys;
-  // (the exponent's scale is kept off zero: -inf * 0 of a masked score is no number)
-  if (p.scale_log2 < 1e-30f) p.scale_log2 = 1e-30f;
   const PlanOffsets o = plan_offsets(a, p.ctas);
   char* ws = static_cast<char*>(workspace);
   p.plan = reinterpret_cast<int*>(ws);

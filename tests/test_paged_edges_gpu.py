@@ -147,3 +147,27 @@ def test_masked_keys_have_no_weight(path):
     for n in q_lens:
         assert not got[row:row + n - n // 2].any(), f"{path}, rows {row}.."
         row += n
+
+
+# --------------------------------------------------------------------------- scales
+@pytest.mark.parametrize("path", PATHS)
+def test_scales_near_zero(path):
+    """Scores of 10^35 under a scale of 10^-36, and no scale at all."""
+    c, q, q_lens, kv_lens = _problem(path)
+    want, size = reference(q, c.k, c.v, c.table, kv_lens, q_lens)
+    tol = attention_tolerance(want, size, BF16, max(kv_lens))
+    # powers of two change no rounding: (2^57 q) (2^60 k) 2^-120 = q k / 8
+    big_q, kept = q * 2.0 ** 57, c.k.clone()
+    c.k.mul_(2.0 ** 60)
+    assert_within(_call(c, big_q, q_lens, scale=2.0 ** -120), want, tol, path)
+    c.k.copy_(kept)
+    # a scale of zero weighs all keys alike, and an infinite score is no number then
+    want, size = reference(q, c.k, c.v, c.table, kv_lens, q_lens, True, 0.0)
+    assert_within(_call(c, q, q_lens, scale=0.0), want,
+                  attention_tolerance(want, size, BF16, max(kv_lens)), path)
+    pg, r = _slot(c, 0, kv_lens[0] - 1)
+    c.k[pg, r, :, 7] = -INF
+    last = q_lens[0] - 1
+    q[last, :, 7] = 1
+    got = _call(c, q, q_lens, scale=0.0)
+    assert got[last].isnan().all() and got[:last].isfinite().all()
