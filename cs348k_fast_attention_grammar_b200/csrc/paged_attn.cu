@@ -771,6 +771,11 @@ bool strides_ok(const int64_t* st, const int64_t* sizes, int n, bool written) {
   return true;
 }
 
+// The scale of the exponent to base 2, as the kernels have it.
+float scale_log2(const fa_paged_attn_args* a) {
+  return static_cast<float>(a->scale * 1.4426950408889634);
+}
+
 int check_paged_attn(const fa_paged_attn_args* a) {
   constexpr int64_t kMax = 0x7fffffffLL, kMaxPlaces = kMax - 4096;
   if (!a || !a->q || !a->o || !a->k_cache || !a->v_cache || !a->block_table || !a->kv_lens)
@@ -782,7 +787,7 @@ int check_paged_attn(const fa_paged_attn_args* a) {
     return FA_ERR_SHAPE;
   if (!a->cu_seqlens && a->T != a->B) return FA_ERR_SHAPE;
   if (a->D < 8 || a->D > 128 || a->D % 8) return FA_ERR_HEAD_DIM;
-  if (!std::isfinite(a->scale)) return FA_ERR_ARG;
+  if (!std::isfinite(scale_log2(a))) return FA_ERR_ARG;
   if (a->pages <= 0 || a->pages > kMax || a->max_pages <= 0 || a->max_pages > kMax ||
       a->page_size < 16 || a->page_size > 1024 || (a->page_size & (a->page_size - 1)) ||
       a->max_pages * a->page_size > kMaxPlaces)
@@ -847,10 +852,6 @@ int max_clusters(int dev, bool narrow, int shift) {
   }
   slot.store(n, std::memory_order_relaxed);
   return n;
-}
-
-float scale_log2(const fa_paged_attn_args* a) {
-  return static_cast<float>(a->scale * 1.4426950408889634);
 }
 
 struct Choice {

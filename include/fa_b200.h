@@ -307,6 +307,7 @@ int fa_paged_append(const fa_paged_append_args* args, void* stream);
  * a sequence's tokens see must be finite (a value that only some of a chunk's
  * tokens see may reach the others as value * 0); rows behind kv_lens[b] may
  * hold anything.
+ *   scale     : any whose product with log2(e) is finite in fp32.
  *   max_q_len : an upper bound of the tokens per sequence that only guides
  *               which kernels run (T where unknown); results hold for any value.
  *   workspace : fa_paged_attn_workspace(args) bytes, 16-byte aligned, used by
