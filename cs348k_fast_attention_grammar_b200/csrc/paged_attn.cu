@@ -297,7 +297,7 @@ __global__ void __launch_bounds__(RowCfg<DT, MT, CUT>::kThreads, RowCfg<DT, MT, 
     const int row0 = (unit - group * w.tiles) * C::kRows;
     const int rows = min(C::kRows, w.q_len * p.g - row0);      // of this tile
 
-    const int tile_seen = min(w.kv_len, seen_keys(p, w, (row0 + rows - 1) / p.g));
+    const int tile_seen = seen_keys(p, w, (row0 + rows - 1) / p.g);
 
     // This warp's 16-key steps of the blocks: those that some row sees.
     const int key00 = blk0 * kRowKeys + warp_key;

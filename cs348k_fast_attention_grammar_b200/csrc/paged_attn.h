@@ -40,10 +40,11 @@ struct PagedParams {
   int cluster_shift;                    // and CTAs (1 << this) that share a unit's keys
 };
 
-// A sequence's new tokens and keys.
+// A sequence's new tokens and the keys that its table holds.
 struct SeqWork {
   int begin, q_len, kv_len;
-};
+  int place0;            // the first new token's place: negative before the start, behind the
+};                       // held keys where the length goes beyond the table
 
 __device__ __forceinline__ SeqWork seq_work(const PagedParams& p, int b) {
   SeqWork w;
@@ -53,12 +54,13 @@ __device__ __forceinline__ SeqWork seq_work(const PagedParams& p, int b) {
   const int len = p.lens[b];
   w.kv_len = held_len(len, p.page_shift, p.max_pages);
   if (len > w.kv_len && len > 0) atomicExch(p.status, kDevBadPage);
+  w.place0 = max(len, 0) - w.q_len;
   return w;
 }
 
 // Keys [0, limit) that token i of the sequence sees.
 __device__ __forceinline__ int seen_keys(const PagedParams& p, const SeqWork& w, int i) {
-  return p.causal ? max(0, w.kv_len - w.q_len + i + 1) : w.kv_len;
+  return p.causal ? min(w.kv_len, max(0, w.place0 + i + 1)) : w.kv_len;
 }
 
 // The tile kernel: bytes of its workspace, and its launches (p.ctas = SMs).

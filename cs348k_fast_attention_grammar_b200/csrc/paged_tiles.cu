@@ -75,7 +75,8 @@ struct Piece {
   int blk0;              // first key block
   int nt[2];             // key blocks of each tile from there (0: it sees none of them)
   int slot;              // where its part goes, -1: the whole unit
-  int pad[2];
+  int place0;            // the sequence's first new token's place
+  int pad;
 };
 static_assert(sizeof(Piece) == 48, "pieces are copied as three 16-byte words");
 
@@ -133,14 +134,15 @@ __device__ __forceinline__ Piece make_piece(const TileParams& p, const SeqWork& 
   for (int t = 0; t < 2; ++t)
     x.nt[t] = max(0, min(blocks_of(p, w, x.tok0 + t * p.tq, p.tq), blk1) - blk0);
   x.slot = slot;
-  x.pad[0] = x.pad[1] = 0;
+  x.place0 = w.place0;
+  x.pad = 0;
   return x;
 }
 __device__ __forceinline__ void put_piece(Piece* to, const Piece& x) {
   int4* d = reinterpret_cast<int4*>(to);
   d[0] = make_int4(x.b, x.h, x.tok0, x.q_begin);
   d[1] = make_int4(x.q_len, x.kv_len, x.blk0, x.nt[0]);
-  d[2] = make_int4(x.nt[1], x.slot, 0, 0);
+  d[2] = make_int4(x.nt[1], x.slot, x.place0, 0);
 }
 __device__ __forceinline__ void put_join(JoinUnit* to, int slot0, int parts, int tok0,
                                          const SeqWork& w, int h) {
@@ -669,6 +671,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           d->nt[0] = x.nt[0];
           d->nt[1] = x.nt[1];
           d->slot = x.slot;
+          d->place0 = x.place0;
           mbar_arrive(bar_unit_full(us));
         }
         if (x.h < 0) break;
@@ -831,8 +834,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       {
         const int tok_t = ring[us].tok0 + t * p.tq, q_len = ring[us].q_len;
         const bool live = row_tok < p.tq && tok_t + row_tok < q_len;
-        if (p.causal) lim0 = kv_len - q_len + tok_t + 1;
-        if (p.causal && live) lim = lim0 + row_tok;
+        if (p.causal && tok_t < q_len) lim0 = ring[us].place0 + tok_t + 1;
+        if (p.causal && live) lim = min(kv_len, lim0 + row_tok);
         any_live = __any_sync(0xffffffffu, live);
       }
       float m_ref = -INFINITY;   // reference maximum (scaled, log2 domain)

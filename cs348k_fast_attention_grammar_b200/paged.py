@@ -25,8 +25,8 @@ One step of a layer::
 
 Errors are those of ``operators``: ``TypeError``/``ValueError`` for what Python
 sees, ``FaError`` for what the C ABI rejects.  What only the device sees -- a page
-outside the cache, a length behind its table -- is skipped there and reported by
-``device_status()``.
+outside the cache, a length beyond its table -- is never written or read outside;
+the operators say what they do instead, and ``device_status()`` reports it.
 """
 
 from __future__ import annotations
@@ -110,7 +110,10 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     one without ``cu_seqlens``, else unknown); it never changes what is computed.
     Rows of no sequence are left as they were in ``out``.  Cached values that a
     sequence's tokens see must be finite; rows behind ``kv_lens`` may hold
-    anything.
+    anything.  A page outside the cache reads as keys and values of zero, with
+    their share of the weights; where a length goes beyond the table, tokens keep
+    their places and see the keys that the table holds (``device_status()``
+    reports both).
     """
     return (_binding or _native()).paged_attention(
         q, k_cache, v_cache, block_table, kv_lens, cu_seqlens, max_q_len, causal, scale, out)

@@ -302,8 +302,10 @@ int fa_paged_append(const fa_paged_append_args* args, void* stream);
  * the keys up to its own place, else all kv_lens[b].  A token that sees no key,
  * or none with a score above -infinity, gets zeros; a score of +infinity or NaN
  * makes its output NaN.  Rows outside every sequence have no effect and are not written.
- * A page outside the cache reads as zeros and a length behind the table is cut
- * there; both leave FA_ERR_PAGE in the device status word.  Cached values that
+ * A page outside the cache reads as keys and values of zero, which have their
+ * share of the weights.  Where a length goes beyond the table, tokens keep their
+ * places (those fa_paged_append stores them by) and see the keys that the table
+ * holds.  Both leave FA_ERR_PAGE in the device status word.  Cached values that
  * a sequence's tokens see must be finite (a value that only some of a chunk's
  * tokens see may reach the others as value * 0); rows behind kv_lens[b] may
  * hold anything.

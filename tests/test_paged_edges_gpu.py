@@ -171,3 +171,37 @@ def test_scales_near_zero(path):
     q[last, :, 7] = 1
     got = _call(c, q, q_lens, scale=0.0)
     assert got[last].isnan().all() and got[:last].isfinite().all()
+
+
+# --------------------------------------------------------------------------- outside the table
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("q_lens,Hkv,pages", [([1, 1], 2, 3), ([20, 9], 2, 3), ([100, 90], 8, 3),
+                                              ([16, 9], 2, 3000), ([20, 16], 8, 400),
+                                              ([100, 90], 8, 400),
+                                              ([100, 90], 1, 400), ([300, 20], 1, 900)])
+def test_lengths_beyond_the_table(q_lens, Hkv, pages, causal):
+    """Tokens keep their places, which append stores them by; they see the keys that the table
+    holds."""
+    held = 16 * pages
+    beyond = 12
+    kv_lens = [held, held - 5]
+    c = Cache(kv_lens, 16, Hkv, 64, BF16, DEV, wider=0)
+    q = _randn((sum(q_lens), 2 * Hkv, 64), BF16, 3)
+    c.lens[0] += beyond
+    got = _call(c, q, q_lens, causal=causal)
+    assert device_status() == FA_ERR_PAGE
+    # the first sequence again, with its table as long as its length (the keys there hidden below)
+    n = q_lens[0]
+    seen = torch.arange(held, device=DEV) <= torch.arange(held + beyond - n, held + beyond,
+                                                           device=DEV)[:, None]
+    if not causal:
+        seen = torch.ones_like(seen)
+    k, v = (t[c.table[0].long()].flatten(0, 1).double().repeat_interleave(2, 1)
+            for t in (c.k, c.v))
+    s = torch.einsum("nhe,khe->nhk", q[:n].double(), k) / 8
+    p = torch.softmax(s.masked_fill(~seen[:, None], -INF), -1)
+    want = torch.einsum("nhk,khe->nhe", p, v)
+    size = torch.einsum("nhk,khe->nhe", p, v.abs())
+    assert_within(got[:n], want, attention_tolerance(want, size, BF16, held), "beyond")
+    want, size = reference(q[n:], c.k, c.v, c.table[1:], kv_lens[1:], q_lens[1:], causal)
+    assert_within(got[n:], want, attention_tolerance(want, size, BF16, held), "the other")
