@@ -205,3 +205,16 @@ def test_lengths_beyond_the_table(q_lens, Hkv, pages, causal):
     assert_within(got[:n], want, attention_tolerance(want, size, BF16, held), "beyond")
     want, size = reference(q[n:], c.k, c.v, c.table[1:], kv_lens[1:], q_lens[1:], causal)
     assert_within(got[n:], want, attention_tolerance(want, size, BF16, held), "the other")
+
+
+@pytest.mark.parametrize("path", PATHS)
+def test_pages_outside_the_cache_read_as_zeros(path):
+    """Their keys have a score and a value of zero, and their share of the weights."""
+    c, q, q_lens, kv_lens = _problem(path)
+    c.table[0, 1], c.table[0, 2] = -1, c.pages
+    got = _call(c, q, q_lens)
+    assert device_status() == FA_ERR_PAGE
+    c.k, c.v = (torch.cat([t, torch.zeros_like(t[:1])]) for t in (c.k, c.v))
+    c.table[0, 1] = c.pages
+    want, size = reference(q, c.k, c.v, c.table, kv_lens, q_lens)
+    assert_within(got, want, attention_tolerance(want, size, BF16, max(kv_lens)), path)
