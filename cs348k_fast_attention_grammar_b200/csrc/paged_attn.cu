@@ -310,7 +310,7 @@ __global__ void __launch_bounds__(RowCfg<DT, MT, CUT>::kThreads, RowCfg<DT, MT, 
       const int pg = WHOLE && s < 32 ? (ahead >= 0 && ahead < p.pages ? ahead : -1)
                                      : page_at(trow, key00 + s * step_keys, p.page_shift,
                                                p.max_pages, p.pages);
-      if (pg < 0) atomicExch(p.status, kDevBadPage);
+      if (pg < 0) atomicMax(p.status, kDevBadPage);
       return pg;
     };
     int ids = page_of(lane), ids_next = page_of(32 + lane);

@@ -53,7 +53,7 @@ __device__ __forceinline__ SeqWork seq_work(const PagedParams& p, int b) {
   w.q_len = r.end - r.begin;
   const int len = p.lens[b];
   w.kv_len = held_len(len, p.page_shift, p.max_pages);
-  if (len > w.kv_len && len > 0) atomicExch(p.status, kDevBadPage);
+  if (len > w.kv_len && len > 0) atomicMax(p.status, kDevBadPage);
   w.place0 = max(len, 0) - w.q_len;
   return w;
 }

@@ -579,7 +579,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int key = j * kKeys + lane * p.box_rows;
       if (lane >= boxes || key >= kv_len) return p.pages;
       const int pg = page_at(trow, key, p.page_shift, p.max_pages, p.pages);
-      if (pg < 0) atomicExch(p.status, kDevBadPage);
+      if (pg < 0) atomicMax(p.status, kDevBadPage);
       return pg < 0 ? p.pages : pg;
     };
     int page = page_for(blk0);

@@ -272,7 +272,7 @@ __global__ void __launch_bounds__(kRotThreads, rot_ctas_per_sm(APPEND))
               k = page * p.kc_page + in * p.part[0].dst_ss;
               v = page * p.vc_page + in * p.part[1].dst_ss;
             } else {
-              atomicExch(p.status, kDevBadPage);
+              atomicMax(p.status, kDevBadPage);
             }
           }
         }

@@ -12,12 +12,14 @@ namespace fa {
 
 // ----------------------------------------------------------------------------
 // Status words.  Kernels never trap: a wait that runs out sets an error word
-// that the host reads back with fa_device_status().
+// that the host reads back with fa_device_status().  The word keeps the largest
+// code: after a wait that ran out the output is incomplete, after a bad page it is
+// what the operator documents.
 // ----------------------------------------------------------------------------
 enum : int {
   kDevOk = 0,
-  kDevTimeout = 1,   // an mbarrier wait exceeded kWaitLimitNs
-  kDevBadPage = 2,   // a block table entry or a length points outside the cache
+  kDevBadPage = 1,   // a block table entry or a length points outside the cache
+  kDevTimeout = 2,   // an mbarrier wait exceeded kWaitLimitNs
 };
 
 // One second is ~1000x longer than any legitimate wait in these kernels.
@@ -127,7 +129,7 @@ __device__ __forceinline__ bool mbar_wait_limit(uint32_t bar, uint32_t parity,
       if (*abort_flag) return false;
       if (globaltimer_ns() - t0 > limit_ns) {
         *abort_flag = 1;
-        atomicExch(status, kDevTimeout);
+        atomicMax(status, kDevTimeout);
         return false;
       }
     }

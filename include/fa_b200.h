@@ -367,7 +367,7 @@ int fa_selftest_exp2(const float* x, float* out, int n, void* stream);
 /*
  * Reads and clears the device-side status word of the current device
  * (FA_OK, FA_ERR_TIMEOUT when a kernel's bounded wait ran out, or FA_ERR_PAGE
- * when a paged operator met a place outside the cache).
+ * when a paged operator met a place outside the cache; a timeout outranks it).
  * Synchronises the device.
  */
 int fa_device_status(void);

@@ -218,3 +218,47 @@ def test_pages_outside_the_cache_read_as_zeros(path):
     c.table[0, 1] = c.pages
     want, size = reference(q, c.k, c.v, c.table, kv_lens, q_lens)
     assert_within(got, want, attention_tolerance(want, size, BF16, max(kv_lens)), path)
+
+
+# --------------------------------------------------------------------------- the status word
+def test_a_wait_that_ran_out_outranks_a_bad_page():
+    """A bad page leaves a usable result, a wait that gave up does not: the word keeps it."""
+    lib = _lib.load()
+    c = Cache([20, 40], 16, 1, 64, BF16, DEV, wider=0)
+    q, k = _randn((2, 2, 64), BF16), _randn((2, 1, 64), BF16)
+    good = c.table.clone()
+    c.table[0, 1] = c.pages
+
+    def wait():
+        stream = torch.cuda.current_stream(DEV).cuda_stream
+        assert lib.fa_selftest_wait_timeout(2000, stream) == 0
+
+    def attend():
+        paged_attention(q, c.k, c.v, c.table, c.lens)
+
+    def long():
+        c.lens[1] = 60
+        attend()
+        c.lens[1] = 40
+
+    def append():
+        paged_kv_append(k, k, c.k, c.v, c.table, c.lens)
+
+    def chunk():
+        _call(Paged(c), q.repeat(20, 4, 1), [20, 20])
+
+    class Paged:
+        def __init__(self, c):
+            self.k, self.v, self.lens = c.k.repeat(1, 1, 4, 1), c.v.repeat(1, 1, 4, 1), c.lens
+            self.table = torch.nn.functional.pad(c.table, (0, 1 << 14), value=-3)
+
+    assert device_status() == 0
+    for bad in (attend, long, append, chunk):
+        bad()
+        assert device_status() == FA_ERR_PAGE and device_status() == 0
+        for first, second in ((wait, bad), (bad, wait)):
+            first()
+            second()
+            assert device_status() == FA_ERR_TIMEOUT, bad.__name__
+            assert device_status() == 0
+    c.table.copy_(good)
