@@ -260,10 +260,14 @@ __global__ void __launch_bounds__(kRotThreads, rot_ctas_per_sm(APPEND))
         return __popc(__ballot_sync(0xffffffffu, at < hi && p.cu[at < hi ? at : lo] <= t));
       });
       if (lane == 0) {
+        // (borders that are not rising may lead to a sequence without this row)
+        const int len = b < 0 ? 0 : p.kv_lens[b];
+        const SeqRows sr = b < 0 ? SeqRows{0, 0} : seq_rows(p.cu, b, static_cast<int>(p.rows));
+        const bool owned = sr.begin <= t && t < sr.end;
         int64_t k = -1, v = -1;
         int place = 0;
-        if (b >= 0) {
-          place = max(p.kv_lens[b], 0) - ((p.cu == nullptr ? b + 1 : p.cu[b + 1]) - t);
+        if (owned) {
+          place = max(len, 0) - (sr.end - t);
           if (place >= 0) {
             const int page = page_at(p.table + b * p.table_stride, place, p.page_shift,
                                      p.max_pages, p.pages);
@@ -278,7 +282,7 @@ __global__ void __launch_bounds__(kRotThreads, rot_ctas_per_sm(APPEND))
         }
         s_dst[0][r] = k;
         s_dst[1][r] = v;
-        s_dst[2][r] = b < 0 ? -1 : t * p.part[2].dst_ss;
+        s_dst[2][r] = owned ? t * p.part[2].dst_ss : -1;
         s_place[r] = place;
       }
     }

@@ -11,7 +11,8 @@ A cache is ``[pages, page_size, Hkv, D]`` (permuted views such as a
 ``[pages, Hkv, page_size, D]`` allocation's are taken as they are); key ``j`` of
 sequence ``b`` is row ``j % page_size`` of page ``block_table[b, j // page_size]``.
 New tokens of all sequences are packed along their first dimension:
-``cu_seqlens [B + 1]`` holds the borders (without it every sequence has one),
+``cu_seqlens [B + 1]`` holds the borders (without it every sequence has one; those
+outside the rows are held to them),
 ``kv_lens [B]`` each sequence's length with its new tokens counted.  Lengths and
 tables stay on the device, so a captured CUDA graph serves later steps whose
 lengths and pages have changed in place.

@@ -258,6 +258,7 @@ int fa_rotary(const fa_rotary_args* args, void* stream);
  * T: those of sequence b are rows [cu_seqlens[b], cu_seqlens[b + 1]) (row b
  * alone when cu_seqlens is NULL), and kv_lens[b] is the sequence's length with
  * them counted, so new token i of q_len sits at kv_lens[b] - q_len + i.
+ * Borders outside [0, T] are held to it.
  *
  * fa_paged_append writes the keys, rotated as in fa_rotary when R > 0, and the
  * values of new tokens to their places, and the rotated queries, where there

@@ -220,6 +220,30 @@ def test_pages_outside_the_cache_read_as_zeros(path):
     assert_within(got, want, attention_tolerance(want, size, BF16, max(kv_lens)), path)
 
 
+@pytest.mark.parametrize("cu,stored", [
+    # (sequence, row, place) of lengths 20, 40 and 30
+    ([0, 2, 900], [(0, 0, 18), (0, 1, 19), (1, 2, 36), (1, 3, 37), (1, 4, 38), (1, 5, 39)]),
+    ([-5, 1, 3], [(0, 0, 19), (1, 1, 38), (1, 2, 39)]),
+    ([0, 3, 2 ** 31 - 1], [(0, 0, 17), (0, 1, 18), (0, 2, 19), (1, 3, 37), (1, 4, 38), (1, 5, 39)]),
+    # not rising: a row is stored for a sequence that owns it or not at all
+    ([4, 1, 3], []),
+    ([0, 5, 2, 6], [(0, 0, 15), (0, 1, 16), (2, 5, 29)])])
+def test_borders_outside_the_rows_store_what_attention_reads(cu, stored):
+    """Borders are held to the packed rows, and tokens stored by what is left of their sequence."""
+    lens = [20, 40, 30][:len(cu) - 1]
+    c = Cache(lens, 16, 1, 64, BF16, DEV)
+    kc, vc = c.k.clone(), c.v.clone()
+    k, v = _randn((6, 1, 64), BF16, 4), _randn((6, 1, 64), BF16, 5)
+    paged_kv_append(k, v, c.k, c.v, c.table, c.lens,
+                    cu_seqlens=torch.tensor(cu, dtype=torch.int32, device=DEV))
+    for b, t, place in stored:
+        pg, r = _slot(c, b, place)
+        kc[pg, r], vc[pg, r] = k[t], v[t]
+    assert torch.equal(c.k.nan_to_num(9), kc.nan_to_num(9))
+    assert torch.equal(c.v.nan_to_num(9), vc.nan_to_num(9))
+    assert device_status() == 0
+
+
 # --------------------------------------------------------------------------- the status word
 def test_a_wait_that_ran_out_outranks_a_bad_page():
     """A bad page leaves a usable result, a wait that gave up does not: the word keeps it."""
