@@ -76,8 +76,8 @@ def load(build_if_stale: bool = True) -> ctypes.CDLL:
     with _lock:
         if _lib is not None:
             return _lib
-        if build_if_stale and (_build.is_stale()):
-            _build.build()
+        if build_if_stale and _build.library_stale():
+            _build.build(binding=False)
         if not os.path.exists(_build.LIB_PATH):
             raise RuntimeError(f"{_build.LIB_PATH} is missing; run "
                                "python -m cs348k_fast_attention_grammar_b200.build")
@@ -91,11 +91,14 @@ def load(build_if_stale: bool = True) -> ctypes.CDLL:
 
 
 def load_binding():
-    """The torch binding (csrc/torch_binding.cpp), bound to the loaded library."""
+    """The torch binding (csrc/torch_binding.cpp), built if it is stale and bound
+    to the loaded library."""
     global _binding
     lib = load()
     with _lock:
         if _binding is None:
+            if _build.binding_stale():
+                _build.build(library=False)
             import torch  # noqa: F401  (its libraries are what the binding links to)
             spec = importlib.util.spec_from_file_location("_fa_torch", _build.BINDING_PATH)
             module = importlib.util.module_from_spec(spec)

@@ -56,16 +56,16 @@ def _older(path, inputs) -> bool:
     return any(os.path.getmtime(p) > t for p in inputs if os.path.exists(p))
 
 
-def _library_stale() -> bool:
+def library_stale() -> bool:
     return _older(LIB_PATH, _inputs())
 
 
-def _binding_stale() -> bool:
+def binding_stale() -> bool:
     return _older(BINDING_PATH, [BINDING_SOURCE, PUBLIC_HEADER])
 
 
 def is_stale() -> bool:
-    return _library_stale() or _binding_stale()
+    return library_stale() or binding_stale()
 
 
 def _library_command(verbose: bool) -> list:
@@ -89,23 +89,30 @@ def _binding_command() -> list:
              "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-lc10", "-lc10_cuda"])
 
 
-def build(force: bool = False, verbose: bool = False) -> str:
-    """Compile the library and the binding if they are missing or older than
-    their sources; returns the library's path.
+def build(force: bool = False, verbose: bool = False, library: bool = True,
+          binding: bool = True) -> str:
+    """Compile the library and the binding (or one of them) if they are missing
+    or older than their sources; returns the library's path.  Neither needs the
+    other: the library loads where there is no g++ or no torch to build the
+    binding against.
 
     Safe when several processes (the ranks of one job) call it at once: an
     exclusive lock on a file beside the library lets one of them compile, the
     others wait and then find the library fresh; each compile writes its own
     temporary file and renames it over the library atomically."""
-    if not force and not is_stale():
+    def wanted():
+        return (library and (force or library_stale()), binding and (force or binding_stale()))
+
+    if not any(wanted()):
         return LIB_PATH
     with open(LIB_PATH + ".lock", "a+") as lock:
         fcntl.flock(lock, fcntl.LOCK_EX)
         try:
             jobs = []
-            if force or _library_stale():
+            want_library, want_binding = wanted()
+            if want_library:
                 jobs.append((LIB_PATH, _library_command(verbose)))
-            if force or _binding_stale():
+            if want_binding:
                 jobs.append((BINDING_PATH, _binding_command()))
             running = []
             for path, cmd in jobs:
