@@ -114,15 +114,17 @@ def build(force: bool = False, verbose: bool = False, library: bool = True,
                 jobs.append((LIB_PATH, _library_command(verbose)))
             if want_binding:
                 jobs.append((BINDING_PATH, _binding_command()))
-            running = []
+            running, failed = [], []
             for path, cmd in jobs:
                 tmp = f"{path}.{os.getpid()}.tmp"
                 cmd = cmd + ["-o", tmp]
                 if verbose:
                     print(" ".join(cmd), file=sys.stderr)
-                running.append((path, tmp, cmd[0], subprocess.Popen(
-                    cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))
-            failed = []
+                try:
+                    running.append((path, tmp, cmd[0], subprocess.Popen(
+                        cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))
+                except OSError as e:                # (the others end before this is raised)
+                    failed.append(f"{os.path.basename(cmd[0])} cannot be run: {e}")
             for path, tmp, tool, proc in running:
                 out, _ = proc.communicate()
                 if verbose or proc.returncode != 0:

@@ -55,3 +55,17 @@ def test_the_binding_builds_when_it_is_asked_for(tree):
                    "assert m is _lib.load_binding() and not build.is_stale()\n"
                    "print(m.__name__)\n")
     assert r.returncode == 0 and "_fa_torch" in r.stdout, r.stdout + r.stderr
+
+
+def test_a_missing_compiler_leaves_no_other_behind(tree):
+    """One compiler that cannot be started: the other ends its work, and nothing is left over."""
+    fake = tree / "nvcc"
+    fake.write_text("#!/bin/sh\nsleep 1\nwhile [ \"$1\" != -o ]; do shift; done\necho made > \"$2\"\n")
+    fake.chmod(0o755)
+    r = _run(tree, "try:\n"
+                   "    build.build(force=True)\n"
+                   "except RuntimeError as e:\n"
+                   "    print('failed:', e)\n", NVCC=str(fake), CXX=str(tree / "none" / "g++"))
+    assert r.returncode == 0 and "failed: g++" in r.stdout, r.stdout + r.stderr
+    assert (tree / PACKAGE / "libfa_b200.so").read_text() == "made\n"
+    assert not _left_over(tree)
