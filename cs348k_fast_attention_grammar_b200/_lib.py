@@ -100,7 +100,7 @@ def load_binding():
             if _build.binding_stale():
                 _build.build(library=False)
             import torch  # noqa: F401  (its libraries are what the binding links to)
-            spec = importlib.util.spec_from_file_location("_fa_torch", _build.BINDING_PATH)
+            spec = importlib.util.spec_from_file_location("_fa_torch", _build.binding_path())
             module = importlib.util.module_from_spec(spec)
             spec.loader.exec_module(module)
             module.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value

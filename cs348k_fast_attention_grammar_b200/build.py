@@ -5,7 +5,7 @@
 The library is a plain C-ABI shared object (no torch types in its
 signatures), so it is compiled by nvcc directly rather than as a torch
 extension.  It links the CUDA runtime statically and needs no libcuda at link
-time (tensor maps are encoded through cudaGetDriverEntryPoint).  _fa_torch.so
+time (tensor maps are encoded through cudaGetDriverEntryPoint).  _fa_torch*.so
 is a CPython module (g++, torch's headers) that holds no kernels: the host side
 of the operators whose small calls are host bound.
 """
@@ -25,8 +25,6 @@ LIB_NAME = "libfa_b200.so"
 LIB_PATH = os.path.join(PKG_DIR, LIB_NAME)
 SOURCES = ["common.cu", "attn_fwd.cu", "gemm.cu", "rotary.cu", "paged_attn.cu",
            "paged_tiles.cu"]
-BINDING_NAME = "_fa_torch.so"
-BINDING_PATH = os.path.join(PKG_DIR, BINDING_NAME)
 BINDING_SOURCE = os.path.join(CSRC, "torch_binding.cpp")
 HEADERS = ["sm100_ptx.cuh", "sm100_tmem_wide.cuh", "sm100_2sm.cuh", "fa_internal.h",
            "paged.cuh", "paged_attn.h"]
@@ -56,12 +54,23 @@ def _older(path, inputs) -> bool:
     return any(os.path.getmtime(p) > t for p in inputs if os.path.exists(p))
 
 
+def binding_path() -> str:
+    """Where the binding for this Python and this torch lies: it holds their
+    layouts through inlined code, so another version's is another file."""
+    import sysconfig
+
+    import torch
+    tags = (sysconfig.get_config_var("SOABI"), "torch" + torch.__version__,
+            f"abi{int(torch._C._GLIBCXX_USE_CXX11_ABI)}")
+    return os.path.join(PKG_DIR, "_fa_torch." + ".".join(map(str, tags)) + ".so")
+
+
 def library_stale() -> bool:
     return _older(LIB_PATH, _inputs())
 
 
 def binding_stale() -> bool:
-    return _older(BINDING_PATH, [BINDING_SOURCE, PUBLIC_HEADER])
+    return _older(binding_path(), [BINDING_SOURCE, PUBLIC_HEADER])
 
 
 def is_stale() -> bool:
@@ -113,7 +122,7 @@ def build(force: bool = False, verbose: bool = False, library: bool = True,
             if want_library:
                 jobs.append((LIB_PATH, _library_command(verbose)))
             if want_binding:
-                jobs.append((BINDING_PATH, _binding_command()))
+                jobs.append((binding_path(), _binding_command()))
             running, failed = [], []
             for path, cmd in jobs:
                 tmp = f"{path}.{os.getpid()}.tmp"

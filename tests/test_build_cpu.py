@@ -69,3 +69,21 @@ def test_a_missing_compiler_leaves_no_other_behind(tree):
     assert r.returncode == 0 and "failed: g++" in r.stdout, r.stdout + r.stderr
     assert (tree / PACKAGE / "libfa_b200.so").read_text() == "made\n"
     assert not _left_over(tree)
+
+
+def test_a_binding_of_another_torch_is_stale(tree):
+    """The binding reads torch's objects through inlined code: one that another torch or Python
+    built is not loaded."""
+    for built in (p for p in os.listdir(os.path.join(ROOT, PACKAGE)) if p.startswith("_fa_torch")):
+        shutil.copy(os.path.join(ROOT, PACKAGE, built), tree / PACKAGE)      # (for its time)
+    r = _run(tree, "import torch\n"
+                   "_lib.load_binding()\n"
+                   "assert not build.binding_stale()\n"
+                   "mine, torch.__version__ = torch.__version__, '0.0.1'\n"
+                   "assert build.binding_stale()\n"
+                   "torch.__version__ = mine\n"
+                   "assert not build.binding_stale()\n"
+                   "import sysconfig\n"
+                   "sysconfig.get_config_vars()['SOABI'] = 'other'\n"
+                   "assert build.binding_stale()\n")
+    assert r.returncode == 0, r.stdout + r.stderr
