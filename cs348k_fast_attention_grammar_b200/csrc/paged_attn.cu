@@ -13,7 +13,9 @@
 // their K and V rows with 16-byte asynchronous copies into a ring of its own (no
 // barrier between warps), and keeps its own running maximum, sum and output, joined
 // over the warps when the CTA leaves a tile.  32 sequences of up to 8192 keys, 32/8
-// heads of 128: 110.5 us, 6.2 TB/s; 3 of up to 131072, 32/4 heads: 104.7 us, 6.1 TB/s.
+// heads of 128: 109 to 111 us, 6.2 TB/s; 3 of up to 131072, 32/4 heads: 103 to 106
+// us, 6.1 TB/s.  The weights are rounded to the 16-bit type that the matrix
+// instructions take; their sum is of the unrounded ones, in fp32 like the output.
 //
 // CTAs work in teams of up to 16 key heads, a head each, that walk the same keys
 // side by side: a cached token's heads lie next to each other, and DRAM is read

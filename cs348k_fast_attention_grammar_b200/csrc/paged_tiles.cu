@@ -16,13 +16,19 @@
 //
 // Bound by the power limit and by the chain S -> softmax -> P of each tile: 2800
 // clocks per 128 keys for 2048 clocks of tensor work (D = 128).  512 tokens over
-// 32768 keys, 32/8 heads of 128: 214 us, 1270 TFLOP/s, the tensor pipe 72 % active at
-// 1.56 GHz, which is where the power limit holds the clock; a causal prompt of 8192
-// tokens, 32 heads of 128: 430 us, 1280 TFLOP/s.  With D = 64 the softmax alone
-// takes the 2800 clocks (half the issue slots, 58 % of the exponential unit), 635
-// TFLOP/s: room for P beside S, so that S comes a block ahead, did not change that
-// (chunk above: 223 us, 232), and neither did four tiles of 64 keys (203 and 191,
-// but 114 and 131 over shorter lists).
+// 32768 keys, 32/8 heads of 128: 217 to 223 us, 1240 TFLOP/s, the tensor pipe 72 %
+// active at 1.56 GHz; a causal prompt of 8192 tokens, 32 heads of 128: 433 to 443 us,
+// 1255 TFLOP/s.  After a tenth of a second of nothing else the power limit takes the
+// clock further down: 256 and 506 us.  With D = 64 the softmax alone takes the 2800
+// clocks (half the issue slots, 58 % of the exponential unit), 178 us and 766
+// TFLOP/s for that chunk: room for P beside S, so that S comes a block ahead, did not
+// change an earlier 223 us (232), and four tiles of 64 keys took 191 for 203, but 131
+// for 114 over shorter lists.
+//
+// P is rounded to the 16-bit type that the matrix instruction takes, while the sum l
+// adds the unrounded weights, in fp32 like O; fp16 weights below 2^-24 of the row's
+// reference vanish from P.  The outputs' error against fp64 is 0.0023 of their size in
+// bf16 and 0.00029 in fp16, where fp32 arithmetic rounded once has 0.0017 and 0.00021.
 //
 // Pages: a load box is min(page_size, 128) rows of one page, so a 128-key tile
 // takes 128 / page_size boxes whose pages come from the block table, one lane of

@@ -11,8 +11,9 @@
 // a row shares the row's angles.
 //
 // Measured: 16384 tokens of 32 heads of 128 bf16 channels turned by three axes in
-// 43.1 us, 6.23 TB/s; 4636 tokens of 16 heads, 64 of 128 channels turned, appended
-// with their queries in 22.1 us, 5.15 TB/s (one wave of CTAs, which starts with its
+// 42.8 us, 6.28 TB/s (45.2 when nothing else runs for a second, with a lower clock);
+// 4636 tokens of 16 heads, 64 of 128 channels turned, appended
+// with their queries in 21.5 to 22.8 us, 5.1 TB/s (one wave of CTAs, which starts with its
 // rows' places: a search in the borders, a length, a table entry); one token, 4 us,
 // the launch.
 //

@@ -24,6 +24,9 @@ One step of a layer::
     o = paged_attention(q, k_cache, v_cache, block_table, kv_lens,
                         cu_seqlens=cu, max_q_len=longest)
 
+Forward only, like ``operators``: no gradient is recorded.  What a call writes must
+not overlap itself or what it reads, but for ``out`` and ``q_out`` as documented.
+
 Errors are those of ``operators``: ``TypeError``/``ValueError`` for what Python
 sees, ``FaError`` for what the C ABI rejects.  What only the device sees -- a page
 outside the cache, a length beyond its table -- is never written or read outside;
